@@ -153,6 +153,10 @@ __global__ void __launch_bounds__(64 * WAVES) gemv_kernel(const TX* __restrict__
                 }
                 acc[r][c] = a0 + a1;
             }
+            // one channel's table reads and sums at a time: without the fence the compiler (no packed float32 instructions) interleaves many
+            // channels, up to 512 registers with spills (1 x 16384^2: 28 us against 19)
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r) asm volatile("" : "+v"(acc[r][c]) : : "memory");
         }
         k0 += kstride;
         if (k0 < k) fetch(k0);
