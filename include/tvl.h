@@ -206,6 +206,100 @@ int tvl_popcount_matmul(const uint32_t* xb, int64_t m, int64_t ld_xb, const uint
 int tvl_ternary_mm_f32(const float* x, int64_t m, int64_t k, int64_t ld_x, const float* tm,
                        int64_t n, int64_t ld_tm, float* res, int64_t ld_res, void* stream);
 
+/* ---- what stands between a decoder block's packed products: positions, cache, attention ------------------------ */
+
+/* The reference evaluates these steps as separate tensor operations (impl/tf/moondream/layers.py:244-268 rotation and cache,
+ * impl/tf/attention.py:87-105 mask, the softmax after it).  Every argument block is a HOST structure that is read before the
+ * call returns; the pointers inside it are device pointers.  `struct_bytes` is sizeof the structure as the caller knows it.
+ * Strides are in elements; the last dimension (the elements of a head) is dense.  All of f32 / f16 / bf16; every sum,
+ * maximum and angle is held in float32, each result rounded once to its type. */
+
+/* Rotary positions.  y[b,t,h,:] = x[b,t,h,:] with the first `rotary_dim` elements of every head turned by its token's angles;
+ * the remaining elements are copied.  Pair i of a head is elements (i, i + rotary_dim/2), or (2i, 2i+1) when `interleaved`:
+ *   (a, c) -> (a cos - c sin, c cos + a sin),   cos = table[p, i], sin = table[p, rotary_dim/2 + i]
+ * with p the token's position.  `inverse` != 0 negates sin: the transposed map, which is the gradient.  A position
+ * outside [0, table_rows) gives a row of NaN. */
+typedef struct tvl_rotary_args {
+    uint64_t struct_bytes;
+    const void* x;             /* [batch, tokens, heads, dim] */
+    void* y;                   /* the same shape; may be x itself */
+    const int64_t* positions;  /* element (b, t) at b * pos_batch + t * pos_token */
+    const float* table;        /* [table_rows, ld_table >= rotary_dim] */
+    int64_t batch, tokens, heads, dim, rotary_dim, table_rows, ld_table;
+    int64_t x_batch, x_token, x_head, y_batch, y_token, y_head, pos_batch, pos_token;
+    int32_t dtype, interleaved, inverse, reserved;
+} tvl_rotary_args;
+int tvl_rotary(const tvl_rotary_args* args, void* stream);
+
+/* The serving form: the joint projection's output goes into the cache in one launch.  qkv[b,t,:] holds `heads` query heads, then
+ * `kv_heads` key heads, then `kv_heads` value heads.  Token t of sequence b has position (= cache slot) cache_len[b] + t:
+ * rotated query heads go to q, rotated key heads to k_cache, value heads to v_cache.  Tokens t >= count[b] are padding: their
+ * rows of q are zero and nothing is written to the caches.  A position that is negative or beyond the table or the cache
+ * gives a row of NaN in q and writes nothing to the caches. */
+typedef struct tvl_rotary_cache_args {
+    uint64_t struct_bytes;
+    const void* qkv;            /* [batch, tokens, (heads + 2 kv_heads) * dim] */
+    void* q;                    /* [batch, tokens, heads, dim], dense */
+    void* k_cache;              /* [batch, kv_heads, slots, dim] */
+    void* v_cache;
+    const float* table;         /* [table_rows, ld_table >= rotary_dim] */
+    const int64_t* cache_len;   /* one value per sequence, at b * cache_len_stride; NULL: cache_len_value for all */
+    const int64_t* count;       /* [batch]; NULL: every token is real */
+    int64_t batch, tokens, heads, kv_heads, dim, rotary_dim, slots, table_rows, ld_table;
+    int64_t x_batch, x_token, k_batch, k_head, k_slot, v_batch, v_head, v_slot;
+    int64_t cache_len_stride, cache_len_value;
+    int32_t dtype, interleaved;
+} tvl_rotary_cache_args;
+int tvl_rotary_cache(const tvl_rotary_cache_args* args, void* stream);
+
+/* Attention.  For query i and key j of one sequence and head (key head = query head / (heads / kv_heads)):
+ *   s = scale * q_i . k_j;   s = softcap * tanh(s / softcap) if softcap > 0;   s -= slopes[head] * |p_i - j|
+ *   out_i = sum_j softmax_j(s) v_j over the keys that query i sees;   lse_i = log sum_j exp(s)
+ * p_i, the query's place among the keys, is i + keys - queries.  Query i sees key j if
+ *   (not causal  or  j <= p_i  or  j < prefix)   and   (no documents  or  documents[i] == documents[j] >= 0).
+ * A query that sees nothing gives zeros and lse = -inf, and passes no gradient.  A key whose weight is zero adds nothing,
+ * whatever its row holds (infinities and NaN behind a mask stay there).
+ *
+ * tvl_cached_attention: k and v are caches of `keys` slots.  Query i of sequence b sits at p_i = cache_len[b] + i; count[b] of
+ * the queries are real (rows beyond give zeros); the cache holds cache_len[b] + count[b] keys, and query i sees key j of
+ * them if j <= p_i or j < prefix.  A query whose place is negative or beyond the cache gives NaN.  `causal`, `documents`, `lse` unused. */
+typedef struct tvl_attention_args {
+    uint64_t struct_bytes;
+    const void* q;              /* [batch, queries, heads, dim] */
+    const void* k;              /* [batch, keys, kv_heads, dim] */
+    const void* v;
+    void* out;                  /* [batch, queries, heads, dim] */
+    float* lse;                 /* [batch, heads, queries] dense; written by tvl_attention (NULL: not wanted), read by its backward */
+    const float* slopes;        /* [heads] or NULL */
+    const int64_t* prefix;      /* one value per sequence or NULL: prefix_value for all */
+    const int64_t* documents;   /* [batch, queries] (queries == keys), rows documents_batch apart, or NULL */
+    const int64_t* cache_len;   /* as in tvl_rotary_cache_args */
+    const int64_t* count;
+    int64_t batch, queries, keys, heads, kv_heads, dim;
+    int64_t q_batch, q_token, q_head, k_batch, k_token, k_head, v_batch, v_token, v_head, o_batch, o_token, o_head;
+    int64_t prefix_value, documents_batch, cache_len_stride, cache_len_value;
+    float scale, softcap;
+    int32_t dtype, causal;
+} tvl_attention_args;
+/* Gradients of tvl_attention: `args` as in the forward call (out and lse as it wrote them), grad_out given, dq, dk, dv written.
+ * k and v heads that several query heads share get the sum over them.  dq, or dk and dv together, may be NULL (not wanted).  Same bits on every call: no atomics on the results. */
+typedef struct tvl_attention_grads {
+    uint64_t struct_bytes;
+    const void* grad_out;       /* [batch, queries, heads, dim] */
+    void* dq;                   /* shaped like q, k, v; dense */
+    void* dk;
+    void* dv;
+    int64_t g_batch, g_token, g_head;
+} tvl_attention_grads;
+/* `workspace`: tvl_*_workspace_bytes(args) bytes of device memory (256-byte aligned; 0 = none needed); contents need no
+ * initialisation and are not preserved. */
+int tvl_attention(const tvl_attention_args* args, void* workspace, size_t workspace_bytes, void* stream);
+size_t tvl_attention_workspace_bytes(const tvl_attention_args* args);
+int tvl_attention_backward(const tvl_attention_args* args, const tvl_attention_grads* grads, void* workspace, size_t workspace_bytes, void* stream);
+size_t tvl_attention_backward_workspace_bytes(const tvl_attention_args* args);
+int tvl_cached_attention(const tvl_attention_args* args, void* workspace, size_t workspace_bytes, void* stream);
+size_t tvl_cached_attention_workspace_bytes(const tvl_attention_args* args);
+
 /* ---- scale fits (one-time) -------------------------------------------------------------------- */
 
 /* Ternary scale by the reference's masked-mean fixed point (binary/modules.py:280-293):

@@ -67,6 +67,14 @@ SIGNATURES = {
     "tvl_fit_binary_scale_f32": (_c_int, [_c_vp, _c_i64, _c_i64, _c_i64, _c_int, _c_int, _c_f32, _c_int, _c_vp, _c_vp,
                                           _c_i64, _c_vp, _c_sz, _c_vp]),
     "tvl_fit_scale_workspace_bytes": (_c_sz, [_c_i64, _c_i64]),
+    "tvl_rotary": (_c_int, [_c_vp, _c_vp]),
+    "tvl_rotary_cache": (_c_int, [_c_vp, _c_vp]),
+    "tvl_attention": (_c_int, [_c_vp, _c_vp, _c_sz, _c_vp]),
+    "tvl_attention_workspace_bytes": (_c_sz, [_c_vp]),
+    "tvl_attention_backward": (_c_int, [_c_vp, _c_vp, _c_vp, _c_sz, _c_vp]),
+    "tvl_attention_backward_workspace_bytes": (_c_sz, [_c_vp]),
+    "tvl_cached_attention": (_c_int, [_c_vp, _c_vp, _c_sz, _c_vp]),
+    "tvl_cached_attention_workspace_bytes": (_c_sz, [_c_vp]),
     "tvl_zero_out_i32": (_c_int, [_c_vp, _c_i64, _c_vp, _c_vp]),
     "tvl_prevent_folding_u8": (_c_int, [_c_vp, _c_i64, _c_vp, _c_vp, _c_vp]),
 }
