@@ -1,0 +1,435 @@
+// Backward attention: delta = rowsum(out * grad_out), then dq per query tile and dk, dv per key tile.  The scores are formed again from
+// q, k and the saved log-sum, twice (14 instead of 10 products per pair, head and element): every gradient is then summed in
+// the registers of one workgroup, in a fixed order, without atomics.
+#include "attention_tiles.h"
+
+namespace tvl {
+
+constexpr int GT = 64;    // rows of a staged tile
+
+// power of two that brings float16 score gradients into the type's range: near the largest output gradient, in steps of 2^8 so that it
+// rarely moves; float32 and bfloat16 need none
+__device__ __forceinline__ int range_exponent(float top) {
+    if (!(top > 0.0f)) return 0;
+    const int e = (int)((__builtin_bit_cast(uint32_t, top) >> 23) & 255) - 127;
+    const int m = ((e + 4) >> 3) * 8;
+    return m < -112 ? -112 : (m > 112 ? 112 : m);
+}
+__device__ __forceinline__ float power_of_two(int e) { return __builtin_bit_cast(float, (uint32_t)(e + 127) << 23); }
+
+// delta[row] and, for float16, the largest finite |grad_out| of every 64 rows.  16 lanes per row, 16 bytes each: bound by HBM.
+template <typename T>
+__global__ void __launch_bounds__(256) attention_delta_kernel(tvl_attention_args a, tvl_attention_grads gr, float* __restrict__ delta, float* __restrict__ maxima, int blocks, bool wide) {
+    constexpr int PER = 16 / (int)sizeof(T);
+    const int bh = blockIdx.x / blocks, n = blockIdx.x % blocks, h = bh % (int)a.heads, b = bh / (int)a.heads;
+    const int lane = threadIdx.x % 16, row = threadIdx.x / 16, dim = (int)a.dim, queries = (int)a.queries;
+    float top = 0.0f;
+#pragma unroll
+    for (int p = 0; p < GT / 16; ++p) {
+        const int i = n * GT + p * 16 + row;
+        float sum = 0.0f;
+        if (i < queries) {
+            const T* op = (const T*)a.out + b * a.o_batch + (int64_t)i * a.o_token + h * a.o_head;
+            const T* gp = (const T*)gr.grad_out + b * gr.g_batch + (int64_t)i * gr.g_token + h * gr.g_head;
+            for (int u = lane; u * PER < dim; u += 16) {
+                const u32x4 x = load_unit<T>(op, u, dim, wide), y = load_unit<T>(gp, u, dim, wide);
+                const T *xe = reinterpret_cast<const T*>(&x), *ye = reinterpret_cast<const T*>(&y);
+#pragma unroll
+                for (int e = 0; e < PER; ++e) {
+                    const float gv = to_float(ye[e]);
+                    sum += to_float(xe[e]) * gv;
+                    if (!not_finite(gv)) top = fmaxf(top, fabsf(gv));
+                }
+            }
+        }
+        for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+        if (i < queries && lane == 0) delta[(int64_t)bh * queries + i] = sum;
+    }
+    if constexpr (__is_same(T, f16)) {      // no other type has memory for them
+        __shared__ float part[4];
+        for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+        if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = top;
+        __syncthreads();
+        if (threadIdx.x == 0) maxima[blockIdx.x] = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+    }
+}
+
+// dq.  4 waves x 32 queries; per 32 keys: S^T = K Q^T, dP^T = V dO^T, dS^T = P (dP - delta) bend (a lane holds one query), dQ^T += K^T dS^T.
+template <typename T, int DP>
+__global__ void __launch_bounds__(256) attention_dq_kernel(tvl_attention_args a, tvl_attention_grads gr, const DocumentSpan* __restrict__ spans, const float* __restrict__ delta,
+                                                           int tiles, bool wide) {
+    constexpr int R = 32, QB = 128, CK = CHUNK<R>;
+    typedef Tile<T, DP> L;
+    typedef typename Operand<T>::elem E;
+    extern __shared__ __align__(16) char lds[];
+    constexpr int TILE = GT * L::ROW;
+
+    const int group = (int)(a.heads / a.kv_heads), pairs = (int)(a.batch * a.kv_heads);
+    const Place at = place_of(blockIdx.x, pairs, group, tiles);
+    const int b = at.pair / (int)a.kv_heads, hk = at.pair % (int)a.kv_heads, h = hk * group + at.head;
+    const int wave = threadIdx.x / 64, lane = threadIdx.x % 64, r = lane % R, g = lane / R;
+    const int q0 = at.tile * QB, qw = q0 + wave * R, i = qw + r;
+    const int dim = (int)a.dim, queries = (int)a.queries;
+    bool lost;
+    const Sequence seq = sequence_of<false>(a, b, lost);
+    const int last = q0 + QB < queries ? q0 + QB : queries, reach = seq.limit(last - 1);
+    const int wlast = qw + R < queries ? qw + R : queries;
+    const int wreach = wlast > qw ? seq.limit(wlast - 1) : 0, wall = wlast > qw ? seq.limit(qw) : 0;
+    const int mine = i < queries ? seq.limit(i) : 0;
+    const T* kp = (const T*)a.k + b * a.k_batch + hk * a.k_head;
+    const T* vp = (const T*)a.v + b * a.v_batch + hk * a.v_head;
+    const int64_t* docs = a.documents;
+    int64_t doc = -1, dlo = 0, dhi = -1;
+    if (docs) {
+        docs += b * a.documents_batch;
+        spans += (int64_t)b * ((queries + SPAN - 1) / SPAN);
+        if (i < queries) doc = docs[i];
+        const DocumentSpan s0 = spans[q0 / SPAN], s1 = q0 + SPAN < queries ? spans[q0 / SPAN + 1] : s0;
+        dlo = s0.lo < s1.lo ? s0.lo : s1.lo;
+        dhi = s0.hi > s1.hi ? s0.hi : s1.hi;
+    }
+    Frag<T> qf[DP / CK], gf[DP / CK];
+    float lse = 0.0f, dl = 0.0f, top = 0.0f;
+#pragma unroll
+    for (int c = 0; c < DP / CK; ++c) {
+        qf[c] = gf[c] = Frag<T>{};
+        if (i < queries) {
+            qf[c] = load_frag<T>((const T*)a.q + b * a.q_batch + (int64_t)i * a.q_token + h * a.q_head, g + (64 / R) * c, dim, wide);
+            gf[c] = load_frag<T>((const T*)gr.grad_out + b * gr.g_batch + (int64_t)i * gr.g_token + h * gr.g_head, g + (64 / R) * c, dim, wide);
+        }
+        if constexpr (__is_same(T, f16)) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (!not_finite((float)gf[c][e])) top = fmaxf(top, fabsf((float)gf[c][e]));
+        }
+    }
+    if (i < queries) {
+        const int64_t row = ((int64_t)b * a.heads + h) * queries + i;
+        lse = a.lse[row] * LOG2E;
+        dl = delta[row];
+    }
+    // float16: every query's own power of two
+    int e = 0;
+    if constexpr (__is_same(T, f16)) e = range_exponent(column_max<R>(top));
+    const float fit = power_of_two(-e);
+    dl *= fit;
+    const float slope = a.slopes ? a.slopes[h] * LOG2E : 0.0f;
+    const bool capped = a.softcap > 0.0f, biased = a.slopes != nullptr;
+    const float to_log2 = a.scale * LOG2E, to_cap = capped ? a.scale / a.softcap : 0.0f, from_cap = a.softcap * LOG2E;
+    Acc<R> acc[DP / R] = {};
+
+    auto skip = [&](int j0) { return docs && (spans[j0 / SPAN].hi < dlo || spans[j0 / SPAN].lo > dhi || spans[j0 / SPAN].hi < 0); };
+    auto next = [&](int j0) {
+        while (j0 < reach && skip(j0)) j0 += GT;
+        return j0;
+    };
+    Stage<T, DP, GT, 256> sk, sv;
+    int j0 = next(0), buf = 0;
+    if (j0 < reach) {
+        sk.load(kp, a.k_token, j0, seq.end, dim, wide);
+        sv.load(vp, a.v_token, j0, seq.end, dim, wide);
+        sk.store(lds);
+        sv.store(lds + TILE);
+    }
+    __syncthreads();
+    while (j0 < reach) {
+        const int j1 = next(j0 + GT);
+        if (j1 < reach) {
+            sk.load(kp, a.k_token, j1, seq.end, dim, wide);
+            sv.load(vp, a.v_token, j1, seq.end, dim, wide);
+        }
+        const char *kt = lds + buf * 2 * TILE, *vt = kt + TILE;
+        const bool one_document = !docs || (dlo == dhi && dlo >= 0 && spans[j0 / SPAN].lo == dlo && spans[j0 / SPAN].hi == dlo);
+#pragma unroll 1
+        for (int t = 0; t < GT; t += R) {
+            const int jt = j0 + t;
+            if (jt >= wreach) break;
+            Acc<R> s = {}, dp = {};
+#pragma unroll
+            for (int c = 0; c < DP / CK; ++c) {
+                s = mma(L::read(kt, t + r, g + (64 / R) * c), qf[c], s);
+                dp = mma(L::read(vt, t + r, g + (64 / R) * c), gf[c], dp);
+            }
+            const bool masked = jt + R > wall || !one_document;
+            Frag<T> df[R / CK];
+#pragma unroll
+            for (int x = 0; x < REGS<R>; ++x) {
+                const int j = jt + result_row<R>(x, g);
+                float v = s[x], bend = 1.0f;
+                if (capped) {
+                    const float th = cap_tanh<T>(v * to_cap);
+                    v = from_cap * th;
+                    bend = 1.0f - th * th;
+                } else {
+                    v *= to_log2;
+                }
+                if (biased) {
+                    const int away = i + seq.shift - j;
+                    v -= slope * (float)(away < 0 ? -away : away);
+                }
+                float d = __builtin_amdgcn_exp2f(v - lse) * __builtin_fmaf(dp[x], fit, -dl) * bend;
+                if (masked) {
+                    bool sees = j < mine;
+                    if (!one_document) sees = sees && doc >= 0 && docs[j < seq.end ? j : 0] == doc;
+                    d = sees ? d : 0.0f;
+                }
+                // score gradients are rounded to the operands' type for the last product; its sum is float32
+                df[x / 8][x % 8] = (E)d;
+            }
+            bool guard = false;
+            if (!one_document || (jt + R > wall && wall < wreach)) {
+                bool bad = false;
+#pragma unroll
+                for (int c = 0; c < R / CK; ++c)
+#pragma unroll
+                    for (int d = 0; d < DP / R; ++d) bad |= any_not_finite<T>(L::template read_across<R>(kt, t + c * CK, d * R, lane));
+                guard = __any(bad);
+            }
+#pragma unroll
+            for (int c = 0; c < R / CK; ++c)
+#pragma unroll
+                for (int d = 0; d < DP / R; ++d) {
+                    const Frag<T> kf = L::template read_across<R>(kt, t + c * CK, d * R, lane);
+                    if (!guard) acc[d] = mma(kf, df[c], acc[d]);
+                    else acc[d] = mma_behind_mask<T, R, true>(kf, df[c], acc[d]);
+                }
+        }
+        if (j1 < reach) {
+            sk.store(lds + (buf ^ 1) * 2 * TILE);
+            sv.store(lds + (buf ^ 1) * 2 * TILE + TILE);
+        }
+        __syncthreads();
+        buf ^= 1;
+        j0 = j1;
+    }
+    if (i >= queries) return;
+    const float back = a.scale * power_of_two(e);
+    T* op = (T*)gr.dq + (((int64_t)b * queries + i) * a.heads + h) * dim;
+#pragma unroll
+    for (int d = 0; d < DP / R; ++d)
+#pragma unroll
+        for (int x = 0; x < REGS<R>; ++x) {
+            const int col = d * R + result_row<R>(x, g);
+            if (col < dim) op[col] = from_float<T>(acc[d][x] * back);
+        }
+}
+
+// dk, dv.  4 waves x 32 keys; over the heads that share them and tiles of 64 queries: S = Q K^T, dP = dO V^T (a lane holds one key, K and V stay in
+// registers), dV^T += dO^T P, dK^T += Q^T dS.
+template <typename T, int DP>
+__global__ void __launch_bounds__(256) attention_dkv_kernel(tvl_attention_args a, tvl_attention_grads gr, const DocumentSpan* __restrict__ spans, const float* __restrict__ delta,
+                                                            const float* __restrict__ maxima, int tiles, bool wide) {
+    constexpr int R = 32, KB = 128, CK = CHUNK<R>;
+    typedef Tile<T, DP> L;
+    typedef typename Operand<T>::elem E;
+    extern __shared__ __align__(16) char lds[];
+    constexpr int TILE = GT * L::ROW, STEP = 2 * TILE + 2 * GT * 4;     // q, grad_out, log-sums, deltas
+
+    const int group = (int)(a.heads / a.kv_heads), pairs = (int)(a.batch * a.kv_heads);
+    const Place at = place_of(blockIdx.x, pairs, 1, tiles);
+    const int b = at.pair / (int)a.kv_heads, hk = at.pair % (int)a.kv_heads;
+    const int wave = threadIdx.x / 64, lane = threadIdx.x % 64, r = lane % R, g = lane / R;
+    const int k0 = (tiles - 1 - at.tile) * KB, kw = k0 + wave * R, j = kw + r;    // with a causal mask the first keys have the most queries
+    const int dim = (int)a.dim, queries = (int)a.queries, keys = (int)a.keys;
+    bool lost;
+    const Sequence seq = sequence_of<false>(a, b, lost);
+    const int64_t* docs = a.documents;
+    int64_t doc = -1, dlo = 0, dhi = -1;
+    if (docs) {
+        docs += b * a.documents_batch;
+        spans += (int64_t)b * ((queries + SPAN - 1) / SPAN);
+        if (j < keys) doc = docs[j];
+        const DocumentSpan s0 = spans[k0 / SPAN], s1 = k0 + SPAN < keys ? spans[k0 / SPAN + 1] : s0;
+        dlo = s0.lo < s1.lo ? s0.lo : s1.lo;
+        dhi = s0.hi > s1.hi ? s0.hi : s1.hi;
+    }
+    Frag<T> kf[DP / CK], vf[DP / CK];
+#pragma unroll
+    for (int c = 0; c < DP / CK; ++c) {
+        kf[c] = vf[c] = Frag<T>{};
+        if (j < keys) {
+            kf[c] = load_frag<T>((const T*)a.k + b * a.k_batch + (int64_t)j * a.k_token + hk * a.k_head, g + (64 / R) * c, dim, wide);
+            vf[c] = load_frag<T>((const T*)a.v + b * a.v_batch + (int64_t)j * a.v_token + hk * a.v_head, g + (64 / R) * c, dim, wide);
+        }
+    }
+    // float16: one power of two for all that this workgroup adds up
+    int e = 0;
+    if constexpr (__is_same(T, f16)) {
+        const int n = group * ((queries + GT - 1) / GT);
+        const float* mp = maxima + ((int64_t)b * a.heads + hk * group) * ((queries + GT - 1) / GT);
+        float top = 0.0f;
+        for (int x = lane; x < n; x += 64) top = fmaxf(top, mp[x]);
+        for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+        e = range_exponent(top);
+    }
+    const float fit = power_of_two(-e);
+    const bool capped = a.softcap > 0.0f, biased = a.slopes != nullptr;
+    const float to_log2 = a.scale * LOG2E, to_cap = capped ? a.scale / a.softcap : 0.0f, from_cap = a.softcap * LOG2E;
+    Acc<R> dk[DP / R] = {}, dv[DP / R] = {};
+
+    // query i sees key j from i = j - shift on (all of them for keys in the prefix)
+    int begin = seq.causal && k0 >= seq.prefix ? k0 - seq.shift : 0;
+    begin = begin < 0 ? 0 : begin / GT * GT;
+    const int steps = begin < queries ? (queries - begin + GT - 1) / GT : 0, total = steps * group;
+    auto skip = [&](int n) {
+        if (!docs) return false;
+        const DocumentSpan s = spans[(begin + (n % steps) * GT) / SPAN];
+        return s.hi < dlo || s.lo > dhi || s.hi < 0;
+    };
+    auto next = [&](int n) {
+        while (n < total && skip(n)) ++n;
+        return n;
+    };
+    Stage<T, DP, GT, 256> sq, sg;
+    float side = 0.0f;      // threads 0..63: a log-sum, 64..127: a delta
+    auto fetch = [&](int n) {
+        const int h = hk * group + n / steps, i0 = begin + (n % steps) * GT;
+        sq.load((const T*)a.q + b * a.q_batch + h * a.q_head, a.q_token, i0, queries, dim, wide);
+        sg.load((const T*)gr.grad_out + b * gr.g_batch + h * gr.g_head, gr.g_token, i0, queries, dim, wide);
+        const int i = i0 + (threadIdx.x & 63);
+        const int64_t row = ((int64_t)b * a.heads + h) * queries + i;
+        // a query behind the last gets weights exp(-inf) = 0
+        if (threadIdx.x < 64) side = i < queries ? a.lse[row] * LOG2E : __builtin_inff();
+        else if (threadIdx.x < 128) side = i < queries ? delta[row] * fit : 0.0f;
+    };
+    auto put = [&](char* to) {
+        sq.store(to);
+        sg.store(to + TILE);
+        if (threadIdx.x < 128) *reinterpret_cast<float*>(to + 2 * TILE + 4 * threadIdx.x) = side;
+    };
+    int n = next(0), buf = 0;
+    if (n < total) {
+        fetch(n);
+        put(lds);
+    }
+    __syncthreads();
+    while (n < total) {
+        const int n1 = next(n + 1);
+        if (n1 < total) fetch(n1);
+        const char *qt = lds + buf * STEP, *gt = qt + TILE;
+        const float *lses = reinterpret_cast<const float*>(qt + 2 * TILE), *deltas = lses + GT;
+        const int h = hk * group + n / steps, i0 = begin + (n % steps) * GT;
+        const float slope = biased ? a.slopes[h] * LOG2E : 0.0f;
+        const bool one_document = !docs || (dlo == dhi && dlo >= 0 && spans[i0 / SPAN].lo == dlo && spans[i0 / SPAN].hi == dlo);
+#pragma unroll 1
+        for (int t = 0; t < GT; t += R) {
+            const int it = i0 + t;
+            const int ilast = it + R < queries ? it + R - 1 : queries - 1;
+            if (it >= queries || kw >= keys) break;
+            if (seq.limit(ilast) <= kw) continue;                              // none of these queries sees a key of the wave
+            Acc<R> s = {}, dp = {};
+#pragma unroll
+            for (int c = 0; c < DP / CK; ++c) {
+                s = mma(L::read(qt, t + r, g + (64 / R) * c), kf[c], s);
+                dp = mma(L::read(gt, t + r, g + (64 / R) * c), vf[c], dp);
+            }
+            const bool edge = seq.limit(it) < kw + R, masked = edge || !one_document;
+            Frag<T> pf[R / CK], df[R / CK];
+#pragma unroll
+            for (int x = 0; x < REGS<R>; ++x) {
+                const int row = t + result_row<R>(x, g), i = i0 + row;
+                float v = s[x], bend = 1.0f;
+                if (capped) {
+                    const float th = cap_tanh<T>(v * to_cap);
+                    v = from_cap * th;
+                    bend = 1.0f - th * th;
+                } else {
+                    v *= to_log2;
+                }
+                if (biased) {
+                    const int away = i + seq.shift - j;
+                    v -= slope * (float)(away < 0 ? -away : away);
+                }
+                float w = __builtin_amdgcn_exp2f(v - lses[row]);
+                float d = w * __builtin_fmaf(dp[x], fit, -deltas[row]) * bend;
+                if (masked) {
+                    bool sees = i < queries && j < seq.limit(i);
+                    if (!one_document) sees = sees && doc >= 0 && docs[i < queries ? i : 0] == doc;
+                    w = sees ? w : 0.0f;
+                    d = sees ? d : 0.0f;
+                }
+                // weights and score gradients are rounded to the operands' type for the last products; their sums are float32
+                pf[x / 8][x % 8] = (E)w;
+                df[x / 8][x % 8] = (E)d;
+            }
+            bool guard = false;
+            if (masked) {
+                bool bad = false;
+#pragma unroll
+                for (int c = 0; c < R / CK; ++c)
+#pragma unroll
+                    for (int d = 0; d < DP / R; ++d)
+                        bad |= any_not_finite<T>(L::template read_across<R>(gt, t + c * CK, d * R, lane)) | any_not_finite<T>(L::template read_across<R>(qt, t + c * CK, d * R, lane));
+                guard = __any(bad);
+            }
+#pragma unroll
+            for (int c = 0; c < R / CK; ++c)
+#pragma unroll
+                for (int d = 0; d < DP / R; ++d) {
+                    const Frag<T> gf = L::template read_across<R>(gt, t + c * CK, d * R, lane), qf = L::template read_across<R>(qt, t + c * CK, d * R, lane);
+                    if (!guard) {
+                        dv[d] = mma(gf, pf[c], dv[d]);
+                        dk[d] = mma(qf, df[c], dk[d]);
+                    } else {
+                        dv[d] = mma_behind_mask<T, R, false>(gf, pf[c], dv[d]);
+                        dk[d] = mma_behind_mask<T, R, true>(qf, df[c], dk[d]);
+                    }
+                }
+        }
+        if (n1 < total) put(lds + (buf ^ 1) * STEP);
+        __syncthreads();
+        buf ^= 1;
+        n = n1;
+    }
+    if (j >= keys) return;
+    const float back = a.scale * power_of_two(e);
+    const int64_t row = (((int64_t)b * keys + j) * a.kv_heads + hk) * dim;
+#pragma unroll
+    for (int d = 0; d < DP / R; ++d)
+#pragma unroll
+        for (int x = 0; x < REGS<R>; ++x) {
+            const int col = d * R + result_row<R>(x, g);
+            if (col < dim) {
+                ((T*)gr.dk)[row + col] = from_float<T>(dk[d][x] * back);
+                ((T*)gr.dv)[row + col] = from_float<T>(dv[d][x]);
+            }
+        }
+}
+
+template <typename T, int DP>
+static int launch_backward(const tvl_attention_args& a, const tvl_attention_grads& g, const DocumentSpan* spans, float* delta, float* maxima, hipStream_t st) {
+    const size_t z = sizeof(T);
+    const int blocks = (int)ceil_div(a.queries, GT);
+    const bool grad = wide_rows(g.grad_out, a.dim, g.g_batch, g.g_token, g.g_head, z);
+    const bool wide = grad && wide_rows(a.q, a.dim, a.q_batch, a.q_token, a.q_head, z) && wide_rows(a.k, a.dim, a.k_batch, a.k_token, a.k_head, z) &&
+                      wide_rows(a.v, a.dim, a.v_batch, a.v_token, a.v_head, z);
+    if (a.queries > 0) {
+        hipLaunchKernelGGL((attention_delta_kernel<T>), dim3((unsigned)(a.batch * a.heads * blocks)), dim3(256), 0, st, a, g, delta, maxima, blocks,
+                           grad && wide_rows(a.out, a.dim, a.o_batch, a.o_token, a.o_head, z));
+        TVL_LAUNCH_CHECK();
+    }
+    if (g.dq && a.queries > 0) {
+        const int tiles = (int)ceil_div(a.queries, 128);
+        const size_t bytes = 4 * GT * (size_t)Tile<T, DP>::ROW;
+        if (bytes > 65536) TVL_HIP_CHECK(hipFuncSetAttribute((const void*)attention_dq_kernel<T, DP>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+        hipLaunchKernelGGL((attention_dq_kernel<T, DP>), dim3((unsigned)(a.batch * a.heads * tiles)), dim3(256), bytes, st, a, g, spans, delta, tiles, wide);
+        TVL_LAUNCH_CHECK();
+    }
+    if (g.dk && a.keys > 0) {
+        const int tiles = (int)ceil_div(a.keys, 128);
+        const size_t bytes = 2 * (2 * GT * (size_t)Tile<T, DP>::ROW + 2 * GT * 4);
+        if (bytes > 65536) TVL_HIP_CHECK(hipFuncSetAttribute((const void*)attention_dkv_kernel<T, DP>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+        hipLaunchKernelGGL((attention_dkv_kernel<T, DP>), dim3((unsigned)(a.batch * a.kv_heads * tiles)), dim3(256), bytes, st, a, g, spans, delta, maxima, tiles, wide);
+        TVL_LAUNCH_CHECK();
+    }
+    return TVL_OK;
+}
+
+int launch_attention_backward(const tvl_attention_args& a, const tvl_attention_grads& g, const DocumentSpan* spans, float* delta, float* maxima, hipStream_t st) {
+    const bool small = a.dim <= 64;
+    if (a.dtype == TVL_F32) return small ? launch_backward<float, 64>(a, g, spans, delta, maxima, st) : launch_backward<float, 128>(a, g, spans, delta, maxima, st);
+    if (a.dtype == TVL_F16) return small ? launch_backward<f16, 64>(a, g, spans, delta, maxima, st) : launch_backward<f16, 128>(a, g, spans, delta, maxima, st);
+    return small ? launch_backward<bf16_t, 64>(a, g, spans, delta, maxima, st) : launch_backward<bf16_t, 128>(a, g, spans, delta, maxima, st);
+}
+
+}  // namespace tvl

@@ -1,0 +1,240 @@
+// Forward attention over tiles: tvl_attention, and tvl_cached_attention for chunks of many tokens.
+#include "attention_tiles.h"
+
+namespace tvl {
+
+// One workgroup: 4 waves x 32 queries of one head; keys and values come in tiles of 64 through LDS, two buffers, the next tile's loads in
+// flight while this one is used.  Per wave and tile: S^T = K Q^T (a lane holds 32 scores of ONE query: maximum and sum are plain loops
+// over its registers plus one exchange with the other half), weights 2^(s - m) rounded to the operands' type as the second product's operand,
+// O^T += V^T P^T.  m is kept until a score exceeds it by 8 (in powers of two): the weights stay below 2^8, exact in float32 sums, and the
+// accumulator is almost never rescaled.
+template <typename T, int DP, bool CACHED>
+__global__ void __launch_bounds__(256) attention_forward_kernel(tvl_attention_args a, const DocumentSpan* __restrict__ spans, int tiles, bool wide) {
+    constexpr int R = 32, KT = 64, QB = 128, CK = CHUNK<R>;
+    typedef Tile<T, DP> L;
+    extern __shared__ __align__(16) char lds[];
+    constexpr int TILE = KT * L::ROW;
+
+    const int group = (int)(a.heads / a.kv_heads), pairs = (int)(a.batch * a.kv_heads);
+    const Place at = place_of(blockIdx.x, pairs, group, tiles);
+    const int b = at.pair / (int)a.kv_heads, hk = at.pair % (int)a.kv_heads, h = hk * group + at.head;
+    const int wave = threadIdx.x / 64, lane = threadIdx.x % 64, r = lane % R, g = lane / R;
+    const int q0 = at.tile * QB, qw = q0 + wave * R, i = qw + r;
+    const int dim = (int)a.dim, queries = (int)a.queries;
+
+    bool lost;
+    const Sequence seq = sequence_of<CACHED>(a, b, lost);
+    const int last = q0 + QB < seq.real ? q0 + QB : seq.real;                  // real queries of this block end here
+    const int reach = last > q0 ? seq.limit(last - 1) : 0;                      // limits grow with the query
+    const int wlast = qw + R < seq.real ? qw + R : seq.real;
+    const int wreach = wlast > qw ? seq.limit(wlast - 1) : 0, wall = wlast > qw ? seq.limit(qw) : 0;   // keys some / every query of the wave sees
+    const int mine = i < seq.real ? seq.limit(i) : 0;
+
+    const T* kp = (const T*)a.k + b * a.k_batch + hk * a.k_head;
+    const T* vp = (const T*)a.v + b * a.v_batch + hk * a.v_head;
+    const T* qp = (const T*)a.q + b * a.q_batch + h * a.q_head + (int64_t)i * a.q_token;
+    const int64_t* docs = CACHED ? nullptr : a.documents;
+    int64_t doc = -1, dlo = 0, dhi = -1;
+    if (docs) {
+        docs += b * a.documents_batch;
+        spans += (int64_t)b * ((queries + SPAN - 1) / SPAN);
+        if (i < queries) doc = docs[i];
+        const DocumentSpan s0 = spans[q0 / SPAN], s1 = q0 + SPAN < queries ? spans[q0 / SPAN + 1] : s0;
+        dlo = s0.lo < s1.lo ? s0.lo : s1.lo;
+        dhi = s0.hi > s1.hi ? s0.hi : s1.hi;
+    }
+
+    // a negative scale goes into the queries' sign, so that the largest product is the largest score
+    const float scale = fabsf(a.scale);
+    Frag<T> qf[DP / CK];
+#pragma unroll
+    for (int c = 0; c < DP / CK; ++c) {
+        qf[c] = Frag<T>{};
+        if (i < seq.real) qf[c] = load_frag<T>(qp, g + (64 / R) * c, dim, wide);
+        if (a.scale < 0.0f) qf[c] = -qf[c];
+    }
+    const float slope = a.slopes ? a.slopes[h] * LOG2E : 0.0f;
+    const bool capped = a.softcap > 0.0f, biased = a.slopes != nullptr;
+    const float to_log2 = scale * LOG2E, to_cap = capped ? scale / a.softcap : 0.0f, from_cap = a.softcap * LOG2E;
+
+    Acc<R> acc[DP / R] = {};
+    float m = -__builtin_inff(), base = 0.0f, sum = 0.0f;
+
+    // tiles that no query of the block meets are skipped
+    auto skip = [&](int j0) { return docs && (spans[j0 / SPAN].hi < dlo || spans[j0 / SPAN].lo > dhi || spans[j0 / SPAN].hi < 0); };
+    auto next = [&](int j0) {
+        while (j0 < reach && skip(j0)) j0 += KT;
+        return j0;
+    };
+    Stage<T, DP, KT, 256> sk, sv;
+    int j0 = next(0), buf = 0;
+    if (j0 < reach) {
+        sk.load(kp, a.k_token, j0, seq.end, dim, wide);
+        sv.load(vp, a.v_token, j0, seq.end, dim, wide);
+        sk.store(lds);
+        sv.store(lds + TILE);
+    }
+    __syncthreads();
+    while (j0 < reach) {
+        const int j1 = next(j0 + KT);
+        if (j1 < reach) {
+            sk.load(kp, a.k_token, j1, seq.end, dim, wide);
+            sv.load(vp, a.v_token, j1, seq.end, dim, wide);
+        }
+        const char *kt = lds + buf * 2 * TILE, *vt = kt + TILE;
+        if (j0 < wreach) {
+            Acc<R> s[KT / R];
+#pragma unroll
+            for (int t = 0; t < KT / R; ++t) {
+                s[t] = Acc<R>{};
+#pragma unroll
+                for (int c = 0; c < DP / CK; ++c) s[t] = mma(L::read(kt, t * R + r, g + (64 / R) * c), qf[c], s[t]);
+            }
+            // scores in powers of two
+            const bool one_document = !docs || (dlo == dhi && dlo >= 0 && spans[j0 / SPAN].lo == dlo && spans[j0 / SPAN].hi == dlo);
+            const bool masked = j0 + KT > wall || !one_document;
+#pragma unroll
+            for (int t = 0; t < KT / R; ++t)
+#pragma unroll
+                for (int x = 0; x < REGS<R>; ++x) {
+                    float v = s[t][x];
+                    const int j = j0 + t * R + result_row<R>(x, g);
+                    v = capped ? from_cap * cap_tanh<T>(v * to_cap) : v * to_log2;
+                    if (biased) {
+                        const int away = i + seq.shift - j;
+                        v -= slope * (float)(away < 0 ? -away : away);
+                    }
+                    if (masked) {
+                        bool sees = j < mine;
+                        if (!one_document) sees = sees && doc >= 0 && docs[j < seq.end ? j : 0] == doc;
+                        v = sees ? v : -__builtin_inff();
+                    }
+                    s[t][x] = v;
+                }
+            float top = s[0][0];
+#pragma unroll
+            for (int t = 0; t < KT / R; ++t)
+#pragma unroll
+                for (int x = 0; x < REGS<R>; ++x) top = fmaxf(top, s[t][x]);
+            top = column_max<R>(top);
+            const bool grow = top > m + 8.0f;
+            if (__any(grow)) {
+                const float now = grow ? top : m, shrink = grow ? __builtin_amdgcn_exp2f(m - now) : 1.0f;
+                m = now;
+                base = m == -__builtin_inff() ? 0.0f : m;
+                sum *= shrink;
+#pragma unroll
+                for (int d = 0; d < DP / R; ++d) acc[d] *= shrink;
+            }
+            Frag<T> pf[KT / CK];
+#pragma unroll
+            for (int t = 0; t < KT / R; ++t)
+#pragma unroll
+                for (int x = 0; x < REGS<R>; ++x) {
+                    const float w = __builtin_amdgcn_exp2f(s[t][x] - base);
+                    sum += w;
+                    // weights are rounded to the operands' type for the second product (relative 2^-11 / 2^-8 each, the sum stays float32)
+                    pf[(t * REGS<R> + x) / 8][x % 8] = (typename Operand<T>::elem)w;
+                }
+            // queries of the wave that see different keys of this tile: an infinity or NaN in a value must not reach the others
+            bool guard = false;
+            if (!one_document || (j0 + KT > wall && wall < wreach)) {
+                bool bad = false;
+#pragma unroll
+                for (int c = 0; c < KT / CK; ++c)
+#pragma unroll
+                    for (int d = 0; d < DP / R; ++d) bad |= any_not_finite<T>(L::template read_across<R>(vt, c * CK, d * R, lane));
+                guard = __any(bad);
+            }
+            if (!guard) {
+#pragma unroll
+                for (int c = 0; c < KT / CK; ++c)
+#pragma unroll
+                    for (int d = 0; d < DP / R; ++d) acc[d] = mma(L::template read_across<R>(vt, c * CK, d * R, lane), pf[c], acc[d]);
+            } else {
+#pragma unroll
+                for (int c = 0; c < KT / CK; ++c)
+#pragma unroll
+                    for (int d = 0; d < DP / R; ++d)
+                        acc[d] = mma_behind_mask<T, R, false>(L::template read_across<R>(vt, c * CK, d * R, lane), pf[c], acc[d]);
+            }
+        }
+        if (j1 < reach) {
+            sk.store(lds + (buf ^ 1) * 2 * TILE);
+            sv.store(lds + (buf ^ 1) * 2 * TILE + TILE);
+        }
+        __syncthreads();
+        buf ^= 1;
+        j0 = j1;
+    }
+
+    sum = column_sum<R>(sum);
+    if (i >= queries) return;
+    const bool empty = sum == 0.0f || i >= seq.real;      // sees nothing, or padding (whose registers hold what unmasked tiles gave it)
+    const float inv = 1.0f / sum;
+    const bool nan = CACHED && i < seq.real && (lost || seq.shift + i >= (int)a.keys);
+    T* op = (T*)a.out + b * a.o_batch + (int64_t)i * a.o_token + h * a.o_head;
+#pragma unroll
+    for (int d = 0; d < DP / R; ++d)
+#pragma unroll
+        for (int x = 0; x < REGS<R>; x += 4) {
+            const int col = d * R + result_row<R>(x, g);
+            T v[4];
+#pragma unroll
+            for (int y = 0; y < 4; ++y) v[y] = from_float<T>(nan ? __builtin_nanf("") : (empty ? 0.0f : acc[d][x + y] * inv));
+            if (wide) {
+                typedef uint32_t quad __attribute__((ext_vector_type(sizeof(T))));
+                if (col < dim) *reinterpret_cast<quad*>(op + col) = *reinterpret_cast<const quad*>(v);
+            } else {
+#pragma unroll
+                for (int y = 0; y < 4; ++y)
+                    if (col + y < dim) op[col + y] = v[y];
+            }
+        }
+    if (!CACHED && a.lse && g == 0) a.lse[((int64_t)b * a.heads + h) * queries + i] = sum == 0.0f ? -__builtin_inff() : (base + __builtin_amdgcn_logf(sum)) * LN2;
+}
+
+// spans[b][n]: smallest and largest document of tokens 64 n .. 64 n + 63
+__global__ void __launch_bounds__(64) document_spans_kernel(const int64_t* __restrict__ documents, int64_t stride, int tokens, int blocks, DocumentSpan* __restrict__ spans) {
+    const int b = blockIdx.x / blocks, n = blockIdx.x % blocks, i = n * SPAN + threadIdx.x;
+    int64_t lo = documents[b * stride + (i < tokens ? i : n * SPAN)], hi = lo;
+    for (int o = 32; o > 0; o >>= 1) {
+        const int64_t l = __shfl_xor((long long)lo, o), u = __shfl_xor((long long)hi, o);
+        lo = l < lo ? l : lo;
+        hi = u > hi ? u : hi;
+    }
+    if (threadIdx.x == 0) spans[blockIdx.x] = DocumentSpan{lo, hi};
+}
+
+int launch_document_spans(const tvl_attention_args& a, DocumentSpan* spans, hipStream_t st) {
+    const int blocks = (int)ceil_div(a.queries, SPAN);
+    hipLaunchKernelGGL(document_spans_kernel, dim3((unsigned)(a.batch * blocks)), dim3(64), 0, st, a.documents, a.documents_batch, (int)a.queries, blocks, spans);
+    TVL_LAUNCH_CHECK();
+    return TVL_OK;
+}
+
+template <typename T, int DP, bool CACHED>
+static int launch_forward(const tvl_attention_args& a, const DocumentSpan* spans, hipStream_t st) {
+    const int tiles = (int)ceil_div(a.queries, 128);
+    const size_t z = sizeof(T), bytes = 4 * 64 * (size_t)Tile<T, DP>::ROW;
+    const bool wide = wide_rows(a.q, a.dim, a.q_batch, a.q_token, a.q_head, z) && wide_rows(a.k, a.dim, a.k_batch, a.k_token, a.k_head, z) &&
+                      wide_rows(a.v, a.dim, a.v_batch, a.v_token, a.v_head, z) && wide_rows(a.out, a.dim, a.o_batch, a.o_token, a.o_head, z);
+    if (bytes > 65536) TVL_HIP_CHECK(hipFuncSetAttribute((const void*)attention_forward_kernel<T, DP, CACHED>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+    hipLaunchKernelGGL((attention_forward_kernel<T, DP, CACHED>), dim3((unsigned)(a.batch * a.heads * tiles)), dim3(256), bytes, st, a, spans, tiles, wide);
+    TVL_LAUNCH_CHECK();
+    return TVL_OK;
+}
+
+template <typename T>
+static int launch_forward_t(const tvl_attention_args& a, bool cached, const DocumentSpan* spans, hipStream_t st) {
+    if (a.dim <= 64) return cached ? launch_forward<T, 64, true>(a, spans, st) : launch_forward<T, 64, false>(a, spans, st);
+    return cached ? launch_forward<T, 128, true>(a, spans, st) : launch_forward<T, 128, false>(a, spans, st);
+}
+
+int launch_attention_forward(const tvl_attention_args& a, bool cached, const DocumentSpan* spans, hipStream_t st) {
+    if (a.dtype == TVL_F32) return launch_forward_t<float>(a, cached, spans, st);
+    if (a.dtype == TVL_F16) return launch_forward_t<f16>(a, cached, spans, st);
+    return launch_forward_t<bf16_t>(a, cached, spans, st);
+}
+
+}  // namespace tvl

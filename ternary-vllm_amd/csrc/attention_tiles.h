@@ -1,0 +1,302 @@
+// Shared parts of the attention kernels: matrix-core fragments, tiles in LDS, what a query sees, scores.
+//
+// All products run on the matrix cores in R x R output tiles (R = 32: v_mfma_f32_32x32x16, R = 16: v_mfma_f32_16x16x32; float32
+// operands: v_mfma_f32_32x32x2 / 16x16x4, eight of them in place of one 16-bit instruction).  Lane l of a wave is r = l % R, g = l / R:
+//   an operand fragment is 8 elements of row r at 8 g .. 8 g + 7 of a chunk of K = 512 / R contracted elements;
+//   register x of the result holds row 4 (64 / R) (x / 4) + 4 g + x % 4 of column r.
+// A product's result therefore feeds the next product's second operand from the registers it is in, if the first operand
+// lists the contracted elements in the same order: fragment element 4 u + y of chunk c is element K c + (K / 2) u + 4 g + y.  read_across() reads
+// a tile of LDS in that order down its rows; the scores never leave the registers of the lanes that hold them.
+#pragma once
+#include "tvl_common.h"
+
+namespace tvl {
+
+constexpr int ATTENTION_MAX_DIM = 128;
+
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+template <typename T> struct Operand;
+template <> struct Operand<f16> { typedef f16x8 frag; typedef _Float16 elem; };
+template <> struct Operand<bf16_t> { typedef bf16x8 frag; typedef __bf16 elem; };
+template <> struct Operand<float> { typedef f32x8 frag; typedef float elem; };
+template <typename T> using Frag = typename Operand<T>::frag;
+
+template <int R> struct Result;
+template <> struct Result<32> { typedef f32x16 type; };
+template <> struct Result<16> { typedef f32x4 type; };
+template <int R> using Acc = typename Result<R>::type;
+template <int R> constexpr int REGS = R * R / 64;       // result registers of a lane
+template <int R> constexpr int CHUNK = 512 / R;         // contracted elements of one fragment pair
+
+__device__ __forceinline__ f32x16 mma(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x16 mma(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x16 mma(f32x8 a, f32x8 b, f32x16 c) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
+    return c;
+}
+__device__ __forceinline__ f32x4 mma(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x4 mma(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x4 mma(f32x8 a, f32x8 b, f32x4 c) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], c, 0, 0, 0);
+    return c;
+}
+
+// row of result register x (of lane group g)
+template <int R> __device__ __forceinline__ constexpr int result_row(int x, int g) { return 4 * (64 / R) * (x >> 2) + 4 * g + (x & 3); }
+
+__device__ __forceinline__ bool not_finite(float v) { return (__builtin_bit_cast(uint32_t, v) & 0x7F800000u) == 0x7F800000u; }
+
+// some element of the fragment is an infinity or NaN (fragments of small tiles only: not on the main path)
+template <typename T> __device__ __forceinline__ bool any_not_finite(Frag<T> a) {
+    bool bad = false;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) bad |= not_finite((float)a[e]);
+    return bad;
+}
+
+// acc += a * w where a holds infinities or NaN: pairs whose weight is zero add nothing, whatever a holds; the others add what they must
+// (an infinity of the element's sign for weights that cannot be negative, else NaN)
+template <typename T, int R, bool SIGNED>
+__device__ __forceinline__ Acc<R> mma_behind_mask(Frag<T> a, Frag<T> w, Acc<R> acc) {
+    Frag<T> clean, up, down, none, seen;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const float v = (float)a[e];
+        const bool bad = not_finite(v), nan = v != v;
+        clean[e] = bad ? (typename Operand<T>::elem)0.0f : a[e];
+        up[e] = (typename Operand<T>::elem)(bad && !nan && v > 0.0f ? 1.0f : 0.0f);
+        down[e] = (typename Operand<T>::elem)(bad && !nan && v < 0.0f ? 1.0f : 0.0f);
+        none[e] = (typename Operand<T>::elem)(nan ? 1.0f : 0.0f);
+        seen[e] = (typename Operand<T>::elem)((float)w[e] != 0.0f ? 1.0f : 0.0f);   // a NaN weight is not zero
+    }
+    acc = mma(clean, w, acc);
+    Acc<R> zero = {};
+    const Acc<R> ups = mma(up, seen, zero), downs = mma(down, seen, zero), nones = mma(none, seen, zero);
+#pragma unroll
+    for (int x = 0; x < REGS<R>; ++x) {
+        if (SIGNED ? ups[x] + downs[x] + nones[x] > 0.0f : nones[x] > 0.0f) acc[x] += __builtin_nanf("");
+        if (!SIGNED && ups[x] > 0.0f) acc[x] += __builtin_inff();
+        if (!SIGNED && downs[x] > 0.0f) acc[x] -= __builtin_inff();
+    }
+    return acc;
+}
+
+// ---- tiles in LDS ------------------------------------------------------------------------------
+// Rows of DP elements in 16-byte units.  A unit lies at its place with the low bits exchanged by the row's, so that the 8 rows a
+// b128 read takes at a time, and the 4 rows x 2 units of a transposing read, fall on different banks (rows of 128 bytes and
+// their multiples: 3 bits; rows of 64 and 192 bytes: 2 bits).
+template <typename T, int DP> struct Tile {
+    static constexpr int UNITS = DP * (int)sizeof(T) / 16;
+    static constexpr int PER = 16 / (int)sizeof(T);          // elements of a unit
+    static constexpr int ROW = DP * (int)sizeof(T);
+    __device__ static __forceinline__ int swap_bits(int row) { return UNITS % 8 == 0 ? ((row & 3) << 1) | ((row >> 2) & 1) : (row & 2) | ((row >> 2) & 1); }
+    __device__ static __forceinline__ int at(int row, int unit) { return row * ROW + ((unit ^ swap_bits(row)) << 4); }
+
+    // fragment of row `row`, elements 8 c8 .. 8 c8 + 7
+    __device__ static __forceinline__ Frag<T> read(const char* tile, int row, int c8) {
+        if constexpr (sizeof(T) == 2) {
+            return __builtin_bit_cast(Frag<T>, *reinterpret_cast<const u32x4*>(tile + at(row, c8)));
+        } else {
+            const f32x4 lo = *reinterpret_cast<const f32x4*>(tile + at(row, 2 * c8)), hi = *reinterpret_cast<const f32x4*>(tile + at(row, 2 * c8 + 1));
+            return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+    }
+
+    // fragment down the rows: element 4 u + y is row row0 + (K / 2) u + 4 g + y, column col0 + r  (K = CHUNK<R>, col0 a multiple of R)
+    template <int R> __device__ static __forceinline__ Frag<T> read_across(const char* tile, int row0, int col0, int lane) {
+        const int r = lane % R, g = lane / R;
+        if constexpr (sizeof(T) == 2) {
+            // ds_read_b64_tr_b16: 16 lanes point at 4 rows x 4 pieces of 4 elements and get the 16 columns
+            const int i = lane & 15, col = col0 + (r & ~15) + 4 * (i & 3), row = row0 + 4 * g + (i >> 2);
+            i16x4 v[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const char* p = tile + at(row + CHUNK<R> / 2 * u, col >> 3) + 8 * (i & 1);
+                v[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(p));
+            }
+            return __builtin_bit_cast(Frag<T>, __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7));
+        } else {
+            Frag<T> f;
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {
+                    const int row = row0 + CHUNK<R> / 2 * u + 4 * g + y;
+                    f[4 * u + y] = *reinterpret_cast<const float*>(tile + at(row, (col0 + r) >> 2) + 4 * (r & 3));
+                }
+            return f;
+        }
+    }
+};
+
+// 16 bytes of a row of `dim` elements, zeros behind them; `wide`: rows are 16-byte aligned and dim a multiple of the unit
+template <typename T>
+__device__ __forceinline__ u32x4 load_unit(const T* row, int unit, int dim, bool wide) {
+    constexpr int PER = 16 / (int)sizeof(T);
+    u32x4 v = {0, 0, 0, 0};
+    const int c = unit * PER;
+    if (wide) {
+        if (c < dim) v = *reinterpret_cast<const u32x4*>(row + c);
+    } else {
+        T e[PER] = {};
+#pragma unroll
+        for (int x = 0; x < PER; ++x)
+            if (c + x < dim) e[x] = row[c + x];
+        v = *reinterpret_cast<const u32x4*>(e);
+    }
+    return v;
+}
+
+// fragment of a row straight from global memory (elements 8 c8 ..)
+template <typename T>
+__device__ __forceinline__ Frag<T> load_frag(const T* row, int c8, int dim, bool wide) {
+    if constexpr (sizeof(T) == 2) {
+        return __builtin_bit_cast(Frag<T>, load_unit<T>(row, c8, dim, wide));
+    } else {
+        const f32x4 lo = __builtin_bit_cast(f32x4, load_unit<T>(row, 2 * c8, dim, wide)), hi = __builtin_bit_cast(f32x4, load_unit<T>(row, 2 * c8 + 1, dim, wide));
+        return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+}
+
+// A tile's way from global memory to LDS through the registers of THREADS threads
+template <typename T, int DP, int ROWS, int THREADS> struct Stage {
+    typedef Tile<T, DP> L;
+    static constexpr int N = ROWS * L::UNITS / THREADS;
+    static_assert(ROWS * L::UNITS % THREADS == 0, "every thread moves the same number of units");
+    u32x4 v[N];
+    // rows row0 .. row0 + ROWS - 1 of a matrix; rows from `end` on are zero and not read
+    __device__ __forceinline__ void load(const T* base, int64_t stride, int row0, int end, int dim, bool wide) {
+#pragma unroll
+        for (int x = 0; x < N; ++x) {
+            const int u = threadIdx.x + x * THREADS, row = u / L::UNITS, unit = u % L::UNITS;
+            v[x] = u32x4{0, 0, 0, 0};
+            if (row0 + row < end) v[x] = load_unit<T>(base + (int64_t)(row0 + row) * stride, unit, dim, wide);
+        }
+    }
+    __device__ __forceinline__ void store(char* tile) const {
+#pragma unroll
+        for (int x = 0; x < N; ++x) {
+            const int u = threadIdx.x + x * THREADS;
+            *reinterpret_cast<u32x4*>(tile + L::at(u / L::UNITS, u % L::UNITS)) = v[x];
+        }
+    }
+};
+
+// the values of lanes l % 32 and l % 32 + 32: v_permlane32_swap exchanges the halves of two registers
+__device__ __forceinline__ void both_halves(float v, float& lo, float& hi) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, v);
+    const auto a = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    const uint32_t x = a[0], y = a[1];
+    lo = __builtin_bit_cast(float, x);
+    hi = __builtin_bit_cast(float, y);
+}
+// maximum / sum over the lanes that hold one column (the groups g)
+template <int R> __device__ __forceinline__ float column_max(float v) {
+    float lo, hi;
+    both_halves(v, lo, hi);
+    v = fmaxf(lo, hi);
+    if constexpr (R == 16) v = fmaxf(v, __shfl_xor(v, 16));
+    return v;
+}
+template <int R> __device__ __forceinline__ float column_sum(float v) {
+    float lo, hi;
+    both_halves(v, lo, hi);
+    v = lo + hi;
+    if constexpr (R == 16) v = v + __shfl_xor(v, 16);
+    return v;
+}
+
+// ---- what a query sees, and its scores ---------------------------------------------------------
+
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+
+// tanh: 1 - 2 / (e^2y + 1) from one hardware exponential and reciprocal (2^-21 off at most) for 16-bit operands, the library's for float32
+template <typename T> __device__ __forceinline__ float cap_tanh(float y) {
+    if constexpr (sizeof(T) == 4) return tanhf(y);
+    return 1.0f - 2.0f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(y * (2.0f * LOG2E)) + 1.0f);
+}
+
+// Sequence b of a call.  Places and limits fit 32 bits: tokens are at most 2^30.
+struct Sequence {
+    int real;          // queries that are real
+    int end;           // keys that exist
+    int shift;         // place of query 0 among the keys
+    int prefix;
+    bool causal;
+    // query i sees keys j < limit(i)
+    __device__ __forceinline__ int limit(int i) const {
+        int v = end;
+        if (causal) {
+            const int p = i + shift + 1, q = p > prefix ? p : prefix;
+            v = q < end ? q : end;
+        }
+        return v < 0 ? 0 : v;
+    }
+};
+
+template <bool CACHED>
+__device__ __forceinline__ Sequence sequence_of(const tvl_attention_args& a, int b, bool& lost) {
+    Sequence s;
+    const int64_t p = a.prefix ? a.prefix[b] : a.prefix_value;
+    s.prefix = (int)(p < 0 ? 0 : (p < a.keys ? p : a.keys));
+    lost = false;
+    if constexpr (CACHED) {
+        const int64_t before = a.cache_len ? a.cache_len[b * a.cache_len_stride] : a.cache_len_value;
+        const int64_t n = a.count ? a.count[b] : a.queries;
+        s.real = (int)(n < 0 ? 0 : (n < a.queries ? n : a.queries));
+        s.causal = true;
+        lost = before < 0 || before >= a.keys;                   // no query of this sequence has a slot
+        s.shift = lost ? (int)a.keys : (int)before;              // query i's slot is shift + i: outside from a.keys on
+        const int64_t e = (int64_t)s.shift + s.real;
+        s.end = lost ? 0 : (int)(e < a.keys ? e : a.keys);
+    } else {
+        s.real = (int)a.queries;
+        s.causal = a.causal != 0;
+        s.shift = (int)(a.keys - a.queries);
+        s.end = (int)a.keys;
+    }
+    return s;
+}
+
+// first and last document of every block of 64 tokens: blocks that cannot meet are skipped, blocks of one document need no test
+struct DocumentSpan { int64_t lo, hi; };
+constexpr int SPAN = 64;
+
+// Sequence and head of a workgroup.  Workgroups with equal blockIdx % 8 share an L2 (8 XCDs): where the (sequence, key head) pairs divide by 8,
+// each pair's query tiles and heads stay on one of them, so its keys and values are fetched into one L2.  Tiles come last first: with a
+// causal mask those are the long ones.
+struct Place { int pair, head, tile; };
+__device__ __forceinline__ Place place_of(uint32_t id, int pairs, int group, int tiles) {
+    const uint32_t per = (uint32_t)group * tiles;
+    uint32_t pair, rest;
+    if (pairs % 8 == 0) {
+        const uint32_t local = id >> 3;
+        pair = (local / per) * 8 + (id & 7);
+        rest = local % per;
+    } else {
+        pair = id / per;
+        rest = id % per;
+    }
+    return Place{(int)pair, (int)(rest % group), tiles - 1 - (int)(rest / group)};
+}
+
+// host side
+static inline bool wide_rows(const void* p, int64_t dim, int64_t s0, int64_t s1, int64_t s2, size_t z) {
+    const int64_t per = (int64_t)(16 / z);
+    return aligned(p, 16) && dim % per == 0 && s0 % per == 0 && s1 % per == 0 && s2 % per == 0;
+}
+
+int launch_attention_forward(const tvl_attention_args& a, bool cached, const DocumentSpan* spans, hipStream_t st);
+int launch_attention_backward(const tvl_attention_args& a, const tvl_attention_grads& g, const DocumentSpan* spans, float* delta, float* maxima, hipStream_t st);
+int launch_document_spans(const tvl_attention_args& a, DocumentSpan* spans, hipStream_t st);
+
+}  // namespace tvl

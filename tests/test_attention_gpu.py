@@ -382,6 +382,38 @@ def test_attention_refusals(tv, dev):
             pytest.fail(f"case {n} was not refused")
 
 
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("documents", [False, True])
+def test_calls_stay_inside_the_workspace_they_ask_for(tv, dev, kind, documents, monkeypatch):
+    """Every workspace is handed out with a margin of known bytes on both sides, which have to be there afterwards."""
+    A = tv.attention_ops
+    given = []
+
+    def workspace(need, device):
+        if need == 0:
+            return None, 0
+        ws = torch.full((need + 2 * 65536,), 0xA5, dtype=torch.uint8, device=device)
+        given.append((ws, need))
+        return ws, ws.data_ptr() + 65536
+
+    monkeypatch.setattr(A, "_workspace", workspace)
+    dt = TYPES[kind]
+    for b, t, h, hk, d in ((3, 130, 4, 2, 64), (1, 1, 1, 1, 64), (2, 700, 2, 1, 128)):
+        leaves = [torch.randn(b, t, n, d, device=dev, dtype=dt, requires_grad=True) for n in (h, hk, hk)]
+        ids = (torch.arange(t, device=dev) // 50)[None].repeat(b, 1) if documents else None
+        out = tv.attention(*leaves, causal=True, documents=ids)
+        torch.autograd.grad(out, leaves, torch.randn_like(out))
+        with torch.no_grad():
+            for n in (1, min(t, 4), t):
+                tv.cached_attention(leaves[0][:, :n].detach(), leaves[1].detach().transpose(1, 2), leaves[2].detach().transpose(1, 2), t - n)
+                long = torch.randn(2, hk, 9000, d, device=dev, dtype=dt)
+                tv.cached_attention(torch.randn(2, n, h, d, device=dev, dtype=dt), long, long, 8000)
+    torch.cuda.synchronize()
+    assert given
+    for ws, need in given:
+        assert bool((ws[:65536] == 0xA5).all()) and bool((ws[65536 + need:] == 0xA5).all()), need
+
+
 def test_attention_empty_calls(tv, dev):
     z = lambda *s: torch.randn(*s, device=dev, requires_grad=True)
     for b, tq, tk in ((0, 4, 4), (2, 0, 4), (2, 4, 0), (2, 0, 0)):
