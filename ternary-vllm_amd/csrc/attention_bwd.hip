@@ -3,6 +3,8 @@
 // the registers of one workgroup, in a fixed order, without atomics.
 #include "attention_tiles.h"
 
+#include <type_traits>
+
 namespace tvl {
 
 constexpr int GT = 64;    // rows of a staged tile
@@ -18,8 +20,8 @@ __device__ __forceinline__ int range_exponent(float top) {
 __device__ __forceinline__ float power_of_two(int e) { return __builtin_bit_cast(float, (uint32_t)(e + 127) << 23); }
 
 // delta[row] and, for float16, the largest finite |grad_out| of every 64 rows.  16 lanes per row, 16 bytes each: bound by HBM.
-template <typename T>
-__global__ void __launch_bounds__(256) attention_delta_kernel(tvl_attention_args a, tvl_attention_grads gr, float* __restrict__ delta, float* __restrict__ maxima, int blocks, bool wide) {
+template <typename T, bool WIDE>
+__global__ void __launch_bounds__(256) attention_delta_kernel(tvl_attention_args a, tvl_attention_grads gr, float* __restrict__ delta, float* __restrict__ maxima, int blocks) {
     constexpr int PER = 16 / (int)sizeof(T);
     const int bh = blockIdx.x / blocks, n = blockIdx.x % blocks, h = bh % (int)a.heads, b = bh / (int)a.heads;
     const int lane = threadIdx.x % 16, row = threadIdx.x / 16, dim = (int)a.dim, queries = (int)a.queries;
@@ -32,7 +34,7 @@ __global__ void __launch_bounds__(256) attention_delta_kernel(tvl_attention_args
             const T* op = (const T*)a.out + b * a.o_batch + (int64_t)i * a.o_token + h * a.o_head;
             const T* gp = (const T*)gr.grad_out + b * gr.g_batch + (int64_t)i * gr.g_token + h * gr.g_head;
             for (int u = lane; u * PER < dim; u += 16) {
-                const u32x4 x = load_unit<T>(op, u, dim, wide), y = load_unit<T>(gp, u, dim, wide);
+                const u32x4 x = load_unit<T, WIDE>(op, u, dim), y = load_unit<T, WIDE>(gp, u, dim);
                 const T *xe = reinterpret_cast<const T*>(&x), *ye = reinterpret_cast<const T*>(&y);
 #pragma unroll
                 for (int e = 0; e < PER; ++e) {
@@ -55,9 +57,10 @@ __global__ void __launch_bounds__(256) attention_delta_kernel(tvl_attention_args
 }
 
 // dq.  4 waves x 32 queries; per 32 keys: S^T = K Q^T, dP^T = V dO^T, dS^T = P (dP - delta) bend (a lane holds one query), dQ^T += K^T dS^T.
-template <typename T, int DP>
-__global__ void __launch_bounds__(256) attention_dq_kernel(tvl_attention_args a, tvl_attention_grads gr, const DocumentSpan* __restrict__ spans, const float* __restrict__ delta,
-                                                           int tiles, bool wide) {
+template <typename T, int DP, Form FORM>
+__global__ void __launch_bounds__(256, DP == 64 && sizeof(T) == 2 ? 2 : 1) attention_dq_kernel(tvl_attention_args a, tvl_attention_grads gr, const DocumentSpan* __restrict__ spans, const float* __restrict__ delta,
+                                                           int tiles) {
+    constexpr bool WIDE = FORM != ODD;
     constexpr int R = 32, QB = 128, CK = CHUNK<R>;
     typedef Tile<T, DP> L;
     typedef typename Operand<T>::elem E;
@@ -67,18 +70,19 @@ __global__ void __launch_bounds__(256) attention_dq_kernel(tvl_attention_args a,
     const int group = (int)(a.heads / a.kv_heads), pairs = (int)(a.batch * a.kv_heads);
     const Place at = place_of(blockIdx.x, pairs, group, tiles);
     const int b = at.pair / (int)a.kv_heads, hk = at.pair % (int)a.kv_heads, h = hk * group + at.head;
-    const int wave = threadIdx.x / 64, lane = threadIdx.x % 64, r = lane % R, g = lane / R;
+    const int wave = wave_number(), lane = threadIdx.x % 64, r = lane % R, g = lane / R;
     const int q0 = at.tile * QB, qw = q0 + wave * R, i = qw + r;
     const int dim = (int)a.dim, queries = (int)a.queries;
     bool lost;
     const Sequence seq = sequence_of<false>(a, b, lost);
     const int last = q0 + QB < queries ? q0 + QB : queries, reach = seq.limit(last - 1);
+    const int all = FORM != PLAIN && a.documents ? 0 : seq.limit(q0);      // keys every query of the block sees
     const int wlast = qw + R < queries ? qw + R : queries;
     const int wreach = wlast > qw ? seq.limit(wlast - 1) : 0, wall = wlast > qw ? seq.limit(qw) : 0;
     const int mine = i < queries ? seq.limit(i) : 0;
     const T* kp = (const T*)a.k + b * a.k_batch + hk * a.k_head;
     const T* vp = (const T*)a.v + b * a.v_batch + hk * a.v_head;
-    const int64_t* docs = a.documents;
+    const int64_t* docs = FORM == PLAIN ? nullptr : a.documents;
     int64_t doc = -1, dlo = 0, dhi = -1;
     if (docs) {
         docs += b * a.documents_batch;
@@ -94,8 +98,8 @@ __global__ void __launch_bounds__(256) attention_dq_kernel(tvl_attention_args a,
     for (int c = 0; c < DP / CK; ++c) {
         qf[c] = gf[c] = Frag<T>{};
         if (i < queries) {
-            qf[c] = load_frag<T>((const T*)a.q + b * a.q_batch + (int64_t)i * a.q_token + h * a.q_head, g + (64 / R) * c, dim, wide);
-            gf[c] = load_frag<T>((const T*)gr.grad_out + b * gr.g_batch + (int64_t)i * gr.g_token + h * gr.g_head, g + (64 / R) * c, dim, wide);
+            qf[c] = load_frag<T, WIDE>((const T*)a.q + b * a.q_batch + (int64_t)i * a.q_token + h * a.q_head, g + (64 / R) * c, dim);
+            gf[c] = load_frag<T, WIDE>((const T*)gr.grad_out + b * gr.g_batch + (int64_t)i * gr.g_token + h * gr.g_head, g + (64 / R) * c, dim);
         }
         if constexpr (__is_same(T, f16)) {
 #pragma unroll
@@ -114,8 +118,9 @@ __global__ void __launch_bounds__(256) attention_dq_kernel(tvl_attention_args a,
     const float fit = power_of_two(-e);
     dl *= fit;
     const float slope = a.slopes ? a.slopes[h] * LOG2E : 0.0f;
-    const bool capped = a.softcap > 0.0f, biased = a.slopes != nullptr;
+    const bool capped = FORM != PLAIN && a.softcap > 0.0f, biased = FORM != PLAIN && a.slopes != nullptr;
     const float to_log2 = a.scale * LOG2E, to_cap = capped ? a.scale / a.softcap : 0.0f, from_cap = a.softcap * LOG2E;
+    const float pre = capped ? 1.0f : to_log2, unit = capped || biased ? 1.0f : to_log2;
     Acc<R> acc[DP / R] = {};
 
     auto skip = [&](int j0) { return docs && (spans[j0 / SPAN].hi < dlo || spans[j0 / SPAN].lo > dhi || spans[j0 / SPAN].hi < 0); };
@@ -123,76 +128,84 @@ __global__ void __launch_bounds__(256) attention_dq_kernel(tvl_attention_args a,
         while (j0 < reach && skip(j0)) j0 += GT;
         return j0;
     };
-    Stage<T, DP, GT, 256> sk, sv;
+    Stage<T, DP, GT, 256, WIDE> sk, sv;
     int j0 = next(0), buf = 0;
     if (j0 < reach) {
-        sk.load(kp, a.k_token, j0, seq.end, dim, wide);
-        sv.load(vp, a.v_token, j0, seq.end, dim, wide);
+        sk.load(kp, a.k_token, j0, seq.end, dim);
+        sv.load(vp, a.v_token, j0, seq.end, dim);
         sk.store(lds);
         sv.store(lds + TILE);
     }
     __syncthreads();
-    while (j0 < reach) {
+    // MASKED: some query of the block does not see some key of the tile
+    auto step = [&](auto masked) __attribute__((always_inline)) {
+        constexpr bool MASKED = decltype(masked)::value;
         const int j1 = next(j0 + GT);
         if (j1 < reach) {
-            sk.load(kp, a.k_token, j1, seq.end, dim, wide);
-            sv.load(vp, a.v_token, j1, seq.end, dim, wide);
+            sk.load(kp, a.k_token, j1, seq.end, dim);
+            sv.load(vp, a.v_token, j1, seq.end, dim);
         }
         const char *kt = lds + buf * 2 * TILE, *vt = kt + TILE;
-        const bool one_document = !docs || (dlo == dhi && dlo >= 0 && spans[j0 / SPAN].lo == dlo && spans[j0 / SPAN].hi == dlo);
+        const bool one_document = !MASKED || !docs || (dlo == dhi && dlo >= 0 && spans[j0 / SPAN].lo == dlo && spans[j0 / SPAN].hi == dlo);
 #pragma unroll 1
         for (int t = 0; t < GT; t += R) {
             const int jt = j0 + t;
-            if (jt >= wreach) break;
+            if (MASKED && jt >= wreach) break;
             Acc<R> s = {}, dp = {};
 #pragma unroll
             for (int c = 0; c < DP / CK; ++c) {
                 s = mma(L::read(kt, t + r, g + (64 / R) * c), qf[c], s);
                 dp = mma(L::read(vt, t + r, g + (64 / R) * c), gf[c], dp);
             }
-            const bool masked = jt + R > wall || !one_document;
             Frag<T> df[R / CK];
+            if (capped) {
 #pragma unroll
-            for (int x = 0; x < REGS<R>; ++x) {
-                const int j = jt + result_row<R>(x, g);
-                float v = s[x], bend = 1.0f;
-                if (capped) {
-                    const float th = cap_tanh<T>(v * to_cap);
-                    v = from_cap * th;
-                    bend = 1.0f - th * th;
-                } else {
-                    v *= to_log2;
+                for (int x = 0; x < REGS<R>; ++x) {
+                    const float th = cap_tanh<T>(s[x] * to_cap);
+                    s[x] = from_cap * th;
+                    dp[x] = __builtin_fmaf(dp[x], fit, -dl) * (1.0f - th * th);
                 }
-                if (biased) {
-                    const int away = i + seq.shift - j;
-                    v -= slope * (float)(away < 0 ? -away : away);
-                }
-                float d = __builtin_amdgcn_exp2f(v - lse) * __builtin_fmaf(dp[x], fit, -dl) * bend;
-                if (masked) {
-                    bool sees = j < mine;
-                    if (!one_document) sees = sees && doc >= 0 && docs[j < seq.end ? j : 0] == doc;
-                    d = sees ? d : 0.0f;
-                }
-                // score gradients are rounded to the operands' type for the last product; its sum is float32
-                df[x / 8][x % 8] = (E)d;
+            } else {
+#pragma unroll
+                for (int x = 0; x < REGS<R>; ++x) dp[x] = __builtin_fmaf(dp[x], fit, -dl);
             }
-            bool guard = false;
-            if (!one_document || (jt + R > wall && wall < wreach)) {
-                bool bad = false;
+            if (biased) {
+                const int here = i + seq.shift - jt - 4 * g;
+#pragma unroll
+                for (int x = 0; x < REGS<R>; ++x) s[x] = __builtin_fmaf(-slope, fabsf((float)(here - result_row<R>(x, 0))), s[x] * pre);
+            }
+#pragma unroll
+            for (int x = 0; x < REGS<R>; ++x) dp[x] *= __builtin_amdgcn_exp2f(__builtin_fmaf(s[x], unit, -lse));
+            if (MASKED && (jt + R > wall || !one_document)) {
+                const int left = mine - jt - 4 * g;
+#pragma unroll
+                for (int x = 0; x < REGS<R>; ++x)
+                    if (result_row<R>(x, 0) >= left) dp[x] = 0.0f;
+                if (!one_document) {
+#pragma unroll
+                    for (int x = 0; x < REGS<R>; ++x) {
+                        const int j = jt + result_row<R>(x, g);
+                        if (doc < 0 || docs[j < seq.end ? j : 0] != doc) dp[x] = 0.0f;
+                    }
+                }
+            }
+            // score gradients are rounded to the operands' type for the last product; its sum is float32
+#pragma unroll
+            for (int x = 0; x < REGS<R>; ++x) df[x / 8][x % 8] = (E)dp[x];
+            if (MASKED && (!one_document || (jt + R > wall && wall < wreach)) && holds_not_finite<T, DP, R>(kt + t * L::ROW, lane)) {
 #pragma unroll
                 for (int c = 0; c < R / CK; ++c)
 #pragma unroll
-                    for (int d = 0; d < DP / R; ++d) bad |= any_not_finite<T>(L::template read_across<R>(kt, t + c * CK, d * R, lane));
-                guard = __any(bad);
+                    for (int d = 0; d < DP / R; ++d) acc[d] = mma(finite_part<T>(L::template read_across<R>(kt, t + c * CK, d * R, lane)), df[c], acc[d]);
+#pragma unroll 1
+                for (int row = 0; row < R && jt + row < reach; ++row)
+                    add_not_finite<T, DP, R>(kt, t + row, jt + row < mine && (one_document || (doc >= 0 && docs[jt + row] == doc)), true, g, acc);
+            } else {
+#pragma unroll
+                for (int c = 0; c < R / CK; ++c)
+#pragma unroll
+                    for (int d = 0; d < DP / R; ++d) acc[d] = mma(L::template read_across<R>(kt, t + c * CK, d * R, lane), df[c], acc[d]);
             }
-#pragma unroll
-            for (int c = 0; c < R / CK; ++c)
-#pragma unroll
-                for (int d = 0; d < DP / R; ++d) {
-                    const Frag<T> kf = L::template read_across<R>(kt, t + c * CK, d * R, lane);
-                    if (!guard) acc[d] = mma(kf, df[c], acc[d]);
-                    else acc[d] = mma_behind_mask<T, R, true>(kf, df[c], acc[d]);
-                }
         }
         if (j1 < reach) {
             sk.store(lds + (buf ^ 1) * 2 * TILE);
@@ -201,7 +214,9 @@ __global__ void __launch_bounds__(256) attention_dq_kernel(tvl_attention_args a,
         __syncthreads();
         buf ^= 1;
         j0 = j1;
-    }
+    };
+    while (j0 < reach && j0 + GT <= all) step(std::false_type{});
+    while (j0 < reach) step(std::true_type{});
     if (i >= queries) return;
     const float back = a.scale * power_of_two(e);
     T* op = (T*)gr.dq + (((int64_t)b * queries + i) * a.heads + h) * dim;
@@ -216,9 +231,10 @@ __global__ void __launch_bounds__(256) attention_dq_kernel(tvl_attention_args a,
 
 // dk, dv.  4 waves x 32 keys; over the heads that share them and tiles of 64 queries: S = Q K^T, dP = dO V^T (a lane holds one key, K and V stay in
 // registers), dV^T += dO^T P, dK^T += Q^T dS.
-template <typename T, int DP>
-__global__ void __launch_bounds__(256) attention_dkv_kernel(tvl_attention_args a, tvl_attention_grads gr, const DocumentSpan* __restrict__ spans, const float* __restrict__ delta,
-                                                            const float* __restrict__ maxima, int tiles, bool wide) {
+template <typename T, int DP, Form FORM>
+__global__ void __launch_bounds__(256, DP == 64 && sizeof(T) == 2 ? 2 : 1) attention_dkv_kernel(tvl_attention_args a, tvl_attention_grads gr, const DocumentSpan* __restrict__ spans, const float* __restrict__ delta,
+                                                            const float* __restrict__ maxima, int tiles) {
+    constexpr bool WIDE = FORM != ODD;
     constexpr int R = 32, KB = 128, CK = CHUNK<R>;
     typedef Tile<T, DP> L;
     typedef typename Operand<T>::elem E;
@@ -228,12 +244,12 @@ __global__ void __launch_bounds__(256) attention_dkv_kernel(tvl_attention_args a
     const int group = (int)(a.heads / a.kv_heads), pairs = (int)(a.batch * a.kv_heads);
     const Place at = place_of(blockIdx.x, pairs, 1, tiles);
     const int b = at.pair / (int)a.kv_heads, hk = at.pair % (int)a.kv_heads;
-    const int wave = threadIdx.x / 64, lane = threadIdx.x % 64, r = lane % R, g = lane / R;
+    const int wave = wave_number(), lane = threadIdx.x % 64, r = lane % R, g = lane / R;
     const int k0 = (tiles - 1 - at.tile) * KB, kw = k0 + wave * R, j = kw + r;    // with a causal mask the first keys have the most queries
     const int dim = (int)a.dim, queries = (int)a.queries, keys = (int)a.keys;
     bool lost;
     const Sequence seq = sequence_of<false>(a, b, lost);
-    const int64_t* docs = a.documents;
+    const int64_t* docs = FORM == PLAIN ? nullptr : a.documents;
     int64_t doc = -1, dlo = 0, dhi = -1;
     if (docs) {
         docs += b * a.documents_batch;
@@ -248,8 +264,8 @@ __global__ void __launch_bounds__(256) attention_dkv_kernel(tvl_attention_args a
     for (int c = 0; c < DP / CK; ++c) {
         kf[c] = vf[c] = Frag<T>{};
         if (j < keys) {
-            kf[c] = load_frag<T>((const T*)a.k + b * a.k_batch + (int64_t)j * a.k_token + hk * a.k_head, g + (64 / R) * c, dim, wide);
-            vf[c] = load_frag<T>((const T*)a.v + b * a.v_batch + (int64_t)j * a.v_token + hk * a.v_head, g + (64 / R) * c, dim, wide);
+            kf[c] = load_frag<T, WIDE>((const T*)a.k + b * a.k_batch + (int64_t)j * a.k_token + hk * a.k_head, g + (64 / R) * c, dim);
+            vf[c] = load_frag<T, WIDE>((const T*)a.v + b * a.v_batch + (int64_t)j * a.v_token + hk * a.v_head, g + (64 / R) * c, dim);
         }
     }
     // float16: one power of two for all that this workgroup adds up
@@ -263,8 +279,9 @@ __global__ void __launch_bounds__(256) attention_dkv_kernel(tvl_attention_args a
         e = range_exponent(top);
     }
     const float fit = power_of_two(-e);
-    const bool capped = a.softcap > 0.0f, biased = a.slopes != nullptr;
+    const bool capped = FORM != PLAIN && a.softcap > 0.0f, biased = FORM != PLAIN && a.slopes != nullptr;
     const float to_log2 = a.scale * LOG2E, to_cap = capped ? a.scale / a.softcap : 0.0f, from_cap = a.softcap * LOG2E;
+    const float pre = capped ? 1.0f : to_log2, unit = capped || biased ? 1.0f : to_log2;
     Acc<R> dk[DP / R] = {}, dv[DP / R] = {};
 
     // query i sees key j from i = j - shift on (all of them for keys in the prefix)
@@ -280,12 +297,12 @@ __global__ void __launch_bounds__(256) attention_dkv_kernel(tvl_attention_args a
         while (n < total && skip(n)) ++n;
         return n;
     };
-    Stage<T, DP, GT, 256> sq, sg;
+    Stage<T, DP, GT, 256, WIDE> sq, sg;
     float side = 0.0f;      // threads 0..63: a log-sum, 64..127: a delta
     auto fetch = [&](int n) {
         const int h = hk * group + n / steps, i0 = begin + (n % steps) * GT;
-        sq.load((const T*)a.q + b * a.q_batch + h * a.q_head, a.q_token, i0, queries, dim, wide);
-        sg.load((const T*)gr.grad_out + b * gr.g_batch + h * gr.g_head, gr.g_token, i0, queries, dim, wide);
+        sq.load((const T*)a.q + b * a.q_batch + h * a.q_head, a.q_token, i0, queries, dim);
+        sg.load((const T*)gr.grad_out + b * gr.g_batch + h * gr.g_head, gr.g_token, i0, queries, dim);
         const int i = i0 + (threadIdx.x & 63);
         const int64_t row = ((int64_t)b * a.heads + h) * queries + i;
         // a query behind the last gets weights exp(-inf) = 0
@@ -303,83 +320,105 @@ __global__ void __launch_bounds__(256) attention_dkv_kernel(tvl_attention_args a
         put(lds);
     }
     __syncthreads();
-    while (n < total) {
+    // MASKED: some query of the tile does not see some key of the block
+    auto step = [&](auto masks) __attribute__((always_inline)) {
+        constexpr bool MASKED = decltype(masks)::value;
         const int n1 = next(n + 1);
         if (n1 < total) fetch(n1);
         const char *qt = lds + buf * STEP, *gt = qt + TILE;
         const float *lses = reinterpret_cast<const float*>(qt + 2 * TILE), *deltas = lses + GT;
         const int h = hk * group + n / steps, i0 = begin + (n % steps) * GT;
         const float slope = biased ? a.slopes[h] * LOG2E : 0.0f;
-        const bool one_document = !docs || (dlo == dhi && dlo >= 0 && spans[i0 / SPAN].lo == dlo && spans[i0 / SPAN].hi == dlo);
+        const bool one_document = !MASKED || !docs || (dlo == dhi && dlo >= 0 && spans[i0 / SPAN].lo == dlo && spans[i0 / SPAN].hi == dlo);
 #pragma unroll 1
         for (int t = 0; t < GT; t += R) {
             const int it = i0 + t;
             const int ilast = it + R < queries ? it + R - 1 : queries - 1;
-            if (it >= queries || kw >= keys) break;
-            if (seq.limit(ilast) <= kw) continue;                              // none of these queries sees a key of the wave
+            if (it >= queries || (MASKED && kw >= keys)) break;
+            if (MASKED && seq.limit(ilast) <= kw) continue;                              // none of these queries sees a key of the wave
             Acc<R> s = {}, dp = {};
 #pragma unroll
             for (int c = 0; c < DP / CK; ++c) {
                 s = mma(L::read(qt, t + r, g + (64 / R) * c), kf[c], s);
                 dp = mma(L::read(gt, t + r, g + (64 / R) * c), vf[c], dp);
             }
-            const bool edge = seq.limit(it) < kw + R, masked = edge || !one_document;
+            const bool masked = MASKED && (seq.limit(it) < kw + R || !one_document);
             Frag<T> pf[R / CK], df[R / CK];
+            const float *ls = lses + t + 4 * g, *dl = deltas + t + 4 * g;
+            if (capped) {
+#pragma unroll
+                for (int x = 0; x < REGS<R>; ++x) {
+                    const float th = cap_tanh<T>(s[x] * to_cap);
+                    s[x] = from_cap * th;
+                    dp[x] = __builtin_fmaf(dp[x], fit, -dl[result_row<R>(x, 0)]) * (1.0f - th * th);
+                }
+            } else {
+#pragma unroll
+                for (int x = 0; x < REGS<R>; ++x) dp[x] = __builtin_fmaf(dp[x], fit, -dl[result_row<R>(x, 0)]);
+            }
+            if (biased) {
+                const int here = it + 4 * g + seq.shift - j;
+#pragma unroll
+                for (int x = 0; x < REGS<R>; ++x) s[x] = __builtin_fmaf(-slope, fabsf((float)(here + result_row<R>(x, 0))), s[x] * pre);
+            }
 #pragma unroll
             for (int x = 0; x < REGS<R>; ++x) {
-                const int row = t + result_row<R>(x, g), i = i0 + row;
-                float v = s[x], bend = 1.0f;
-                if (capped) {
-                    const float th = cap_tanh<T>(v * to_cap);
-                    v = from_cap * th;
-                    bend = 1.0f - th * th;
-                } else {
-                    v *= to_log2;
-                }
-                if (biased) {
-                    const int away = i + seq.shift - j;
-                    v -= slope * (float)(away < 0 ? -away : away);
-                }
-                float w = __builtin_amdgcn_exp2f(v - lses[row]);
-                float d = w * __builtin_fmaf(dp[x], fit, -deltas[row]) * bend;
-                if (masked) {
-                    bool sees = i < queries && j < seq.limit(i);
-                    if (!one_document) sees = sees && doc >= 0 && docs[i < queries ? i : 0] == doc;
-                    w = sees ? w : 0.0f;
-                    d = sees ? d : 0.0f;
-                }
-                // weights and score gradients are rounded to the operands' type for the last products; their sums are float32
-                pf[x / 8][x % 8] = (E)w;
-                df[x / 8][x % 8] = (E)d;
+                s[x] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x], unit, -ls[result_row<R>(x, 0)]));
+                dp[x] *= s[x];
             }
-            bool guard = false;
-            if (masked) {
-                bool bad = false;
+            if (MASKED && masked) {
+                // query i = it + 4 g + row sees key j if j is in its sequence's prefix or not behind its place
+                const int from = j >= seq.end ? R : (!seq.causal || j < seq.prefix ? -R : j - seq.shift - it - 4 * g);
+#pragma unroll
+                for (int x = 0; x < REGS<R>; ++x)
+                    if (result_row<R>(x, 0) < from) s[x] = dp[x] = 0.0f;
+                if (!one_document) {
+#pragma unroll
+                    for (int x = 0; x < REGS<R>; ++x) {
+                        const int i = it + result_row<R>(x, g);
+                        if (doc < 0 || docs[i < queries ? i : 0] != doc) s[x] = dp[x] = 0.0f;
+                    }
+                }
+            }
+            // weights and score gradients are rounded to the operands' type for the last products; their sums are float32
+#pragma unroll
+            for (int x = 0; x < REGS<R>; ++x) {
+                pf[x / 8][x % 8] = (E)s[x];
+                df[x / 8][x % 8] = (E)dp[x];
+            }
+            if (MASKED && masked && (holds_not_finite<T, DP, R>(gt + t * L::ROW, lane) || holds_not_finite<T, DP, R>(qt + t * L::ROW, lane))) {
 #pragma unroll
                 for (int c = 0; c < R / CK; ++c)
 #pragma unroll
-                    for (int d = 0; d < DP / R; ++d)
-                        bad |= any_not_finite<T>(L::template read_across<R>(gt, t + c * CK, d * R, lane)) | any_not_finite<T>(L::template read_across<R>(qt, t + c * CK, d * R, lane));
-                guard = __any(bad);
-            }
-#pragma unroll
-            for (int c = 0; c < R / CK; ++c)
-#pragma unroll
-                for (int d = 0; d < DP / R; ++d) {
-                    const Frag<T> gf = L::template read_across<R>(gt, t + c * CK, d * R, lane), qf = L::template read_across<R>(qt, t + c * CK, d * R, lane);
-                    if (!guard) {
-                        dv[d] = mma(gf, pf[c], dv[d]);
-                        dk[d] = mma(qf, df[c], dk[d]);
-                    } else {
-                        dv[d] = mma_behind_mask<T, R, false>(gf, pf[c], dv[d]);
-                        dk[d] = mma_behind_mask<T, R, true>(qf, df[c], dk[d]);
+                    for (int d = 0; d < DP / R; ++d) {
+                        dv[d] = mma(finite_part<T>(L::template read_across<R>(gt, t + c * CK, d * R, lane)), pf[c], dv[d]);
+                        dk[d] = mma(finite_part<T>(L::template read_across<R>(qt, t + c * CK, d * R, lane)), df[c], dk[d]);
                     }
+#pragma unroll 1
+                for (int row = 0; row < R && it + row < queries; ++row) {
+                    const bool sees = j < seq.limit(it + row) && (one_document || (doc >= 0 && docs[it + row] == doc));
+                    add_not_finite<T, DP, R>(gt, t + row, sees, false, g, dv);
+                    add_not_finite<T, DP, R>(qt, t + row, sees, true, g, dk);
                 }
+            } else {
+#pragma unroll
+                for (int c = 0; c < R / CK; ++c)
+#pragma unroll
+                    for (int d = 0; d < DP / R; ++d) {
+                        dv[d] = mma(L::template read_across<R>(gt, t + c * CK, d * R, lane), pf[c], dv[d]);
+                        dk[d] = mma(L::template read_across<R>(qt, t + c * CK, d * R, lane), df[c], dk[d]);
+                    }
+            }
         }
         if (n1 < total) put(lds + (buf ^ 1) * STEP);
         __syncthreads();
         buf ^= 1;
         n = n1;
+    };
+    auto unmasked = [&](int m) { return !docs && seq.limit(begin + (m % steps) * GT) >= k0 + KB; };
+    while (n < total) {
+        while (n < total && !unmasked(n)) step(std::true_type{});
+        while (n < total && unmasked(n)) step(std::false_type{});
     }
     if (j >= keys) return;
     const float back = a.scale * power_of_two(e);
@@ -396,40 +435,47 @@ __global__ void __launch_bounds__(256) attention_dkv_kernel(tvl_attention_args a
         }
 }
 
-template <typename T, int DP>
-static int launch_backward(const tvl_attention_args& a, const tvl_attention_grads& g, const DocumentSpan* spans, float* delta, float* maxima, hipStream_t st) {
-    const size_t z = sizeof(T);
-    const int blocks = (int)ceil_div(a.queries, GT);
-    const bool grad = wide_rows(g.grad_out, a.dim, g.g_batch, g.g_token, g.g_head, z);
-    const bool wide = grad && wide_rows(a.q, a.dim, a.q_batch, a.q_token, a.q_head, z) && wide_rows(a.k, a.dim, a.k_batch, a.k_token, a.k_head, z) &&
-                      wide_rows(a.v, a.dim, a.v_batch, a.v_token, a.v_head, z);
-    if (a.queries > 0) {
-        hipLaunchKernelGGL((attention_delta_kernel<T>), dim3((unsigned)(a.batch * a.heads * blocks)), dim3(256), 0, st, a, g, delta, maxima, blocks,
-                           grad && wide_rows(a.out, a.dim, a.o_batch, a.o_token, a.o_head, z));
-        TVL_LAUNCH_CHECK();
-    }
+template <typename T, int DP, Form FORM>
+static int launch_gradients(const tvl_attention_args& a, const tvl_attention_grads& g, const DocumentSpan* spans, const float* delta, const float* maxima, hipStream_t st) {
     if (g.dq && a.queries > 0) {
         const int tiles = (int)ceil_div(a.queries, 128);
         const size_t bytes = 4 * GT * (size_t)Tile<T, DP>::ROW;
-        if (bytes > 65536) TVL_HIP_CHECK(hipFuncSetAttribute((const void*)attention_dq_kernel<T, DP>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
-        hipLaunchKernelGGL((attention_dq_kernel<T, DP>), dim3((unsigned)(a.batch * a.heads * tiles)), dim3(256), bytes, st, a, g, spans, delta, tiles, wide);
+        if (bytes > 65536) TVL_HIP_CHECK(hipFuncSetAttribute((const void*)attention_dq_kernel<T, DP, FORM>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+        hipLaunchKernelGGL((attention_dq_kernel<T, DP, FORM>), dim3((unsigned)(a.batch * a.heads * tiles)), dim3(256), bytes, st, a, g, spans, delta, tiles);
         TVL_LAUNCH_CHECK();
     }
     if (g.dk && a.keys > 0) {
         const int tiles = (int)ceil_div(a.keys, 128);
         const size_t bytes = 2 * (2 * GT * (size_t)Tile<T, DP>::ROW + 2 * GT * 4);
-        if (bytes > 65536) TVL_HIP_CHECK(hipFuncSetAttribute((const void*)attention_dkv_kernel<T, DP>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
-        hipLaunchKernelGGL((attention_dkv_kernel<T, DP>), dim3((unsigned)(a.batch * a.kv_heads * tiles)), dim3(256), bytes, st, a, g, spans, delta, maxima, tiles, wide);
+        if (bytes > 65536) TVL_HIP_CHECK(hipFuncSetAttribute((const void*)attention_dkv_kernel<T, DP, FORM>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+        hipLaunchKernelGGL((attention_dkv_kernel<T, DP, FORM>), dim3((unsigned)(a.batch * a.kv_heads * tiles)), dim3(256), bytes, st, a, g, spans, delta, maxima, tiles);
         TVL_LAUNCH_CHECK();
     }
     return TVL_OK;
 }
 
+template <typename T>
+static int launch_backward(const tvl_attention_args& a, const tvl_attention_grads& g, const DocumentSpan* spans, float* delta, float* maxima, hipStream_t st) {
+    const size_t z = sizeof(T);
+    const bool grad = wide_rows(g.grad_out, a.dim, g.g_batch, g.g_token, g.g_head, z);
+    const bool wide = grad && wide_rows(a.q, a.dim, a.q_batch, a.q_token, a.q_head, z) && wide_rows(a.k, a.dim, a.k_batch, a.k_token, a.k_head, z) &&
+                      wide_rows(a.v, a.dim, a.v_batch, a.v_token, a.v_head, z);
+    if (a.queries > 0) {
+        const int blocks = (int)ceil_div(a.queries, GT);
+        const unsigned n = (unsigned)(a.batch * a.heads * blocks);
+        if (grad && wide_rows(a.out, a.dim, a.o_batch, a.o_token, a.o_head, z)) hipLaunchKernelGGL((attention_delta_kernel<T, true>), dim3(n), dim3(256), 0, st, a, g, delta, maxima, blocks);
+        else hipLaunchKernelGGL((attention_delta_kernel<T, false>), dim3(n), dim3(256), 0, st, a, g, delta, maxima, blocks);
+        TVL_LAUNCH_CHECK();
+    }
+    if (!wide) return launch_gradients<T, 128, ODD>(a, g, spans, delta, maxima, st);
+    if (a.dim <= 64) return featureless(a) ? launch_gradients<T, 64, PLAIN>(a, g, spans, delta, maxima, st) : launch_gradients<T, 64, GENERAL>(a, g, spans, delta, maxima, st);
+    return featureless(a) ? launch_gradients<T, 128, PLAIN>(a, g, spans, delta, maxima, st) : launch_gradients<T, 128, GENERAL>(a, g, spans, delta, maxima, st);
+}
+
 int launch_attention_backward(const tvl_attention_args& a, const tvl_attention_grads& g, const DocumentSpan* spans, float* delta, float* maxima, hipStream_t st) {
-    const bool small = a.dim <= 64;
-    if (a.dtype == TVL_F32) return small ? launch_backward<float, 64>(a, g, spans, delta, maxima, st) : launch_backward<float, 128>(a, g, spans, delta, maxima, st);
-    if (a.dtype == TVL_F16) return small ? launch_backward<f16, 64>(a, g, spans, delta, maxima, st) : launch_backward<f16, 128>(a, g, spans, delta, maxima, st);
-    return small ? launch_backward<bf16_t, 64>(a, g, spans, delta, maxima, st) : launch_backward<bf16_t, 128>(a, g, spans, delta, maxima, st);
+    if (a.dtype == TVL_F32) return launch_backward<float>(a, g, spans, delta, maxima, st);
+    if (a.dtype == TVL_F16) return launch_backward<f16>(a, g, spans, delta, maxima, st);
+    return launch_backward<bf16_t>(a, g, spans, delta, maxima, st);
 }
 
 }  // namespace tvl

@@ -1,6 +1,8 @@
 // Forward attention over tiles: tvl_attention, and tvl_cached_attention for chunks of many tokens.
 #include "attention_tiles.h"
 
+#include <type_traits>
+
 namespace tvl {
 
 // One workgroup: 4 waves x 32 queries of one head; keys and values come in tiles of 64 through LDS, two buffers, the next tile's loads in
@@ -8,8 +10,9 @@ namespace tvl {
 // over its registers plus one exchange with the other half), weights 2^(s - m) rounded to the operands' type as the second product's operand,
 // O^T += V^T P^T.  m is kept until a score exceeds it by 8 (in powers of two): the weights stay below 2^8, exact in float32 sums, and the
 // accumulator is almost never rescaled.
-template <typename T, int DP, bool CACHED>
-__global__ void __launch_bounds__(256) attention_forward_kernel(tvl_attention_args a, const DocumentSpan* __restrict__ spans, int tiles, bool wide) {
+template <typename T, int DP, bool CACHED, Form FORM>
+__global__ void __launch_bounds__(256, DP == 64 && sizeof(T) == 2 ? 2 : 1) attention_forward_kernel(tvl_attention_args a, const DocumentSpan* __restrict__ spans, int tiles) {
+    constexpr bool WIDE = FORM != ODD;
     constexpr int R = 32, KT = 64, QB = 128, CK = CHUNK<R>;
     typedef Tile<T, DP> L;
     extern __shared__ __align__(16) char lds[];
@@ -18,7 +21,7 @@ __global__ void __launch_bounds__(256) attention_forward_kernel(tvl_attention_ar
     const int group = (int)(a.heads / a.kv_heads), pairs = (int)(a.batch * a.kv_heads);
     const Place at = place_of(blockIdx.x, pairs, group, tiles);
     const int b = at.pair / (int)a.kv_heads, hk = at.pair % (int)a.kv_heads, h = hk * group + at.head;
-    const int wave = threadIdx.x / 64, lane = threadIdx.x % 64, r = lane % R, g = lane / R;
+    const int wave = wave_number(), lane = threadIdx.x % 64, r = lane % R, g = lane / R;
     const int q0 = at.tile * QB, qw = q0 + wave * R, i = qw + r;
     const int dim = (int)a.dim, queries = (int)a.queries;
 
@@ -26,6 +29,7 @@ __global__ void __launch_bounds__(256) attention_forward_kernel(tvl_attention_ar
     const Sequence seq = sequence_of<CACHED>(a, b, lost);
     const int last = q0 + QB < seq.real ? q0 + QB : seq.real;                  // real queries of this block end here
     const int reach = last > q0 ? seq.limit(last - 1) : 0;                      // limits grow with the query
+    const int all = last > q0 && !(FORM != PLAIN && !CACHED && a.documents) ? seq.limit(q0) : 0;      // keys every real query of the block sees
     const int wlast = qw + R < seq.real ? qw + R : seq.real;
     const int wreach = wlast > qw ? seq.limit(wlast - 1) : 0, wall = wlast > qw ? seq.limit(qw) : 0;   // keys some / every query of the wave sees
     const int mine = i < seq.real ? seq.limit(i) : 0;
@@ -33,7 +37,7 @@ __global__ void __launch_bounds__(256) attention_forward_kernel(tvl_attention_ar
     const T* kp = (const T*)a.k + b * a.k_batch + hk * a.k_head;
     const T* vp = (const T*)a.v + b * a.v_batch + hk * a.v_head;
     const T* qp = (const T*)a.q + b * a.q_batch + h * a.q_head + (int64_t)i * a.q_token;
-    const int64_t* docs = CACHED ? nullptr : a.documents;
+    const int64_t* docs = CACHED || FORM == PLAIN ? nullptr : a.documents;
     int64_t doc = -1, dlo = 0, dhi = -1;
     if (docs) {
         docs += b * a.documents_batch;
@@ -50,12 +54,14 @@ __global__ void __launch_bounds__(256) attention_forward_kernel(tvl_attention_ar
 #pragma unroll
     for (int c = 0; c < DP / CK; ++c) {
         qf[c] = Frag<T>{};
-        if (i < seq.real) qf[c] = load_frag<T>(qp, g + (64 / R) * c, dim, wide);
+        if (i < seq.real) qf[c] = load_frag<T, WIDE>(qp, g + (64 / R) * c, dim);
         if (a.scale < 0.0f) qf[c] = -qf[c];
     }
     const float slope = a.slopes ? a.slopes[h] * LOG2E : 0.0f;
-    const bool capped = a.softcap > 0.0f, biased = a.slopes != nullptr;
+    const bool capped = FORM != PLAIN && a.softcap > 0.0f, biased = FORM != PLAIN && (a.slopes != nullptr || a.scale == 0.0f);
     const float to_log2 = scale * LOG2E, to_cap = capped ? scale / a.softcap : 0.0f, from_cap = a.softcap * LOG2E;
+    // without cap and bias the scaling is part of the exponential's argument (a zero scale would make NaN of -infinity there)
+    const float pre = capped ? 1.0f : to_log2, unit = capped || biased ? 1.0f : to_log2;
 
     Acc<R> acc[DP / R] = {};
     float m = -__builtin_inff(), base = 0.0f, sum = 0.0f;
@@ -66,23 +72,25 @@ __global__ void __launch_bounds__(256) attention_forward_kernel(tvl_attention_ar
         while (j0 < reach && skip(j0)) j0 += KT;
         return j0;
     };
-    Stage<T, DP, KT, 256> sk, sv;
+    Stage<T, DP, KT, 256, WIDE> sk, sv;
     int j0 = next(0), buf = 0;
     if (j0 < reach) {
-        sk.load(kp, a.k_token, j0, seq.end, dim, wide);
-        sv.load(vp, a.v_token, j0, seq.end, dim, wide);
+        sk.load(kp, a.k_token, j0, seq.end, dim);
+        sv.load(vp, a.v_token, j0, seq.end, dim);
         sk.store(lds);
         sv.store(lds + TILE);
     }
     __syncthreads();
-    while (j0 < reach) {
+    // MASKED: some query of the block does not see some key of the tile
+    auto step = [&](auto masked) __attribute__((always_inline)) {
+        constexpr bool MASKED = decltype(masked)::value;
         const int j1 = next(j0 + KT);
         if (j1 < reach) {
-            sk.load(kp, a.k_token, j1, seq.end, dim, wide);
-            sv.load(vp, a.v_token, j1, seq.end, dim, wide);
+            sk.load(kp, a.k_token, j1, seq.end, dim);
+            sv.load(vp, a.v_token, j1, seq.end, dim);
         }
         const char *kt = lds + buf * 2 * TILE, *vt = kt + TILE;
-        if (j0 < wreach) {
+        if (!MASKED || j0 < wreach) {
             Acc<R> s[KT / R];
 #pragma unroll
             for (int t = 0; t < KT / R; ++t) {
@@ -90,33 +98,47 @@ __global__ void __launch_bounds__(256) attention_forward_kernel(tvl_attention_ar
 #pragma unroll
                 for (int c = 0; c < DP / CK; ++c) s[t] = mma(L::read(kt, t * R + r, g + (64 / R) * c), qf[c], s[t]);
             }
-            // scores in powers of two
-            const bool one_document = !docs || (dlo == dhi && dlo >= 0 && spans[j0 / SPAN].lo == dlo && spans[j0 / SPAN].hi == dlo);
-            const bool masked = j0 + KT > wall || !one_document;
+            // scores: units of `unit` powers of two
+            const bool one_document = !MASKED || !docs || (dlo == dhi && dlo >= 0 && spans[j0 / SPAN].lo == dlo && spans[j0 / SPAN].hi == dlo);
+            if (capped) {
 #pragma unroll
-            for (int t = 0; t < KT / R; ++t)
+                for (int t = 0; t < KT / R; ++t)
 #pragma unroll
-                for (int x = 0; x < REGS<R>; ++x) {
-                    float v = s[t][x];
-                    const int j = j0 + t * R + result_row<R>(x, g);
-                    v = capped ? from_cap * cap_tanh<T>(v * to_cap) : v * to_log2;
-                    if (biased) {
-                        const int away = i + seq.shift - j;
-                        v -= slope * (float)(away < 0 ? -away : away);
+                    for (int x = 0; x < REGS<R>; ++x) s[t][x] = from_cap * cap_tanh<T>(s[t][x] * to_cap);
+            }
+            if (biased) {
+                const int here = i + seq.shift - j0 - 4 * g;
+#pragma unroll
+                for (int t = 0; t < KT / R; ++t)
+#pragma unroll
+                    for (int x = 0; x < REGS<R>; ++x) {
+                        const float away = fabsf((float)(here - (t * R + result_row<R>(x, 0))));
+                        s[t][x] = __builtin_fmaf(-slope, away, s[t][x] * pre);
                     }
-                    if (masked) {
-                        bool sees = j < mine;
-                        if (!one_document) sees = sees && doc >= 0 && docs[j < seq.end ? j : 0] == doc;
-                        v = sees ? v : -__builtin_inff();
-                    }
-                    s[t][x] = v;
+            }
+            if (MASKED && (j0 + KT > wall || !one_document)) {
+                const int left = mine - j0 - 4 * g;
+#pragma unroll
+                for (int t = 0; t < KT / R; ++t)
+#pragma unroll
+                    for (int x = 0; x < REGS<R>; ++x)
+                        if (t * R + result_row<R>(x, 0) >= left) s[t][x] = -__builtin_inff();
+                if (!one_document) {
+#pragma unroll
+                    for (int t = 0; t < KT / R; ++t)
+#pragma unroll
+                        for (int x = 0; x < REGS<R>; ++x) {
+                            const int j = j0 + t * R + result_row<R>(x, g);
+                            if (doc < 0 || docs[j < seq.end ? j : 0] != doc) s[t][x] = -__builtin_inff();
+                        }
                 }
+            }
             float top = s[0][0];
 #pragma unroll
             for (int t = 0; t < KT / R; ++t)
 #pragma unroll
                 for (int x = 0; x < REGS<R>; ++x) top = fmaxf(top, s[t][x]);
-            top = column_max<R>(top);
+            top = column_max<R>(top) * unit;
             const bool grow = top > m + 8.0f;
             if (__any(grow)) {
                 const float now = grow ? top : m, shrink = grow ? __builtin_amdgcn_exp2f(m - now) : 1.0f;
@@ -131,32 +153,25 @@ __global__ void __launch_bounds__(256) attention_forward_kernel(tvl_attention_ar
             for (int t = 0; t < KT / R; ++t)
 #pragma unroll
                 for (int x = 0; x < REGS<R>; ++x) {
-                    const float w = __builtin_amdgcn_exp2f(s[t][x] - base);
+                    const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][x], unit, -base));
                     sum += w;
                     // weights are rounded to the operands' type for the second product (relative 2^-11 / 2^-8 each, the sum stays float32)
                     pf[(t * REGS<R> + x) / 8][x % 8] = (typename Operand<T>::elem)w;
                 }
             // queries of the wave that see different keys of this tile: an infinity or NaN in a value must not reach the others
-            bool guard = false;
-            if (!one_document || (j0 + KT > wall && wall < wreach)) {
-                bool bad = false;
+            if (MASKED && (!one_document || (j0 + KT > wall && wall < wreach)) && holds_not_finite<T, DP, KT>(vt, lane)) {
 #pragma unroll
                 for (int c = 0; c < KT / CK; ++c)
 #pragma unroll
-                    for (int d = 0; d < DP / R; ++d) bad |= any_not_finite<T>(L::template read_across<R>(vt, c * CK, d * R, lane));
-                guard = __any(bad);
-            }
-            if (!guard) {
-#pragma unroll
-                for (int c = 0; c < KT / CK; ++c)
-#pragma unroll
-                    for (int d = 0; d < DP / R; ++d) acc[d] = mma(L::template read_across<R>(vt, c * CK, d * R, lane), pf[c], acc[d]);
+                    for (int d = 0; d < DP / R; ++d) acc[d] = mma(finite_part<T>(L::template read_across<R>(vt, c * CK, d * R, lane)), pf[c], acc[d]);
+#pragma unroll 1
+                for (int row = 0; row < KT && j0 + row < reach; ++row)
+                    add_not_finite<T, DP, R>(vt, row, j0 + row < mine && (one_document || (doc >= 0 && docs[j0 + row] == doc)), false, g, acc);
             } else {
 #pragma unroll
                 for (int c = 0; c < KT / CK; ++c)
 #pragma unroll
-                    for (int d = 0; d < DP / R; ++d)
-                        acc[d] = mma_behind_mask<T, R, false>(L::template read_across<R>(vt, c * CK, d * R, lane), pf[c], acc[d]);
+                    for (int d = 0; d < DP / R; ++d) acc[d] = mma(L::template read_across<R>(vt, c * CK, d * R, lane), pf[c], acc[d]);
             }
         }
         if (j1 < reach) {
@@ -166,7 +181,9 @@ __global__ void __launch_bounds__(256) attention_forward_kernel(tvl_attention_ar
         __syncthreads();
         buf ^= 1;
         j0 = j1;
-    }
+    };
+    while (j0 < reach && j0 + KT <= all) step(std::false_type{});
+    while (j0 < reach) step(std::true_type{});
 
     sum = column_sum<R>(sum);
     if (i >= queries) return;
@@ -182,7 +199,7 @@ __global__ void __launch_bounds__(256) attention_forward_kernel(tvl_attention_ar
             T v[4];
 #pragma unroll
             for (int y = 0; y < 4; ++y) v[y] = from_float<T>(nan ? __builtin_nanf("") : (empty ? 0.0f : acc[d][x + y] * inv));
-            if (wide) {
+            if constexpr (WIDE) {
                 typedef uint32_t quad __attribute__((ext_vector_type(sizeof(T))));
                 if (col < dim) *reinterpret_cast<quad*>(op + col) = *reinterpret_cast<const quad*>(v);
             } else {
@@ -213,28 +230,30 @@ int launch_document_spans(const tvl_attention_args& a, DocumentSpan* spans, hipS
     return TVL_OK;
 }
 
-template <typename T, int DP, bool CACHED>
+template <typename T, int DP, bool CACHED, Form FORM>
 static int launch_forward(const tvl_attention_args& a, const DocumentSpan* spans, hipStream_t st) {
     const int tiles = (int)ceil_div(a.queries, 128);
-    const size_t z = sizeof(T), bytes = 4 * 64 * (size_t)Tile<T, DP>::ROW;
-    const bool wide = wide_rows(a.q, a.dim, a.q_batch, a.q_token, a.q_head, z) && wide_rows(a.k, a.dim, a.k_batch, a.k_token, a.k_head, z) &&
-                      wide_rows(a.v, a.dim, a.v_batch, a.v_token, a.v_head, z) && wide_rows(a.out, a.dim, a.o_batch, a.o_token, a.o_head, z);
-    if (bytes > 65536) TVL_HIP_CHECK(hipFuncSetAttribute((const void*)attention_forward_kernel<T, DP, CACHED>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
-    hipLaunchKernelGGL((attention_forward_kernel<T, DP, CACHED>), dim3((unsigned)(a.batch * a.heads * tiles)), dim3(256), bytes, st, a, spans, tiles, wide);
+    const size_t bytes = 4 * 64 * (size_t)Tile<T, DP>::ROW;
+    if (bytes > 65536) TVL_HIP_CHECK(hipFuncSetAttribute((const void*)attention_forward_kernel<T, DP, CACHED, FORM>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+    hipLaunchKernelGGL((attention_forward_kernel<T, DP, CACHED, FORM>), dim3((unsigned)(a.batch * a.heads * tiles)), dim3(256), bytes, st, a, spans, tiles);
     TVL_LAUNCH_CHECK();
     return TVL_OK;
 }
 
-template <typename T>
-static int launch_forward_t(const tvl_attention_args& a, bool cached, const DocumentSpan* spans, hipStream_t st) {
-    if (a.dim <= 64) return cached ? launch_forward<T, 64, true>(a, spans, st) : launch_forward<T, 64, false>(a, spans, st);
-    return cached ? launch_forward<T, 128, true>(a, spans, st) : launch_forward<T, 128, false>(a, spans, st);
+template <typename T, bool CACHED>
+static int launch_forward_t(const tvl_attention_args& a, const DocumentSpan* spans, hipStream_t st) {
+    const size_t z = sizeof(T);
+    const bool wide = wide_rows(a.q, a.dim, a.q_batch, a.q_token, a.q_head, z) && wide_rows(a.k, a.dim, a.k_batch, a.k_token, a.k_head, z) &&
+                      wide_rows(a.v, a.dim, a.v_batch, a.v_token, a.v_head, z) && wide_rows(a.out, a.dim, a.o_batch, a.o_token, a.o_head, z);
+    if (!wide) return launch_forward<T, 128, CACHED, ODD>(a, spans, st);
+    if (a.dim <= 64) return featureless(a) ? launch_forward<T, 64, CACHED, PLAIN>(a, spans, st) : launch_forward<T, 64, CACHED, GENERAL>(a, spans, st);
+    return featureless(a) ? launch_forward<T, 128, CACHED, PLAIN>(a, spans, st) : launch_forward<T, 128, CACHED, GENERAL>(a, spans, st);
 }
 
 int launch_attention_forward(const tvl_attention_args& a, bool cached, const DocumentSpan* spans, hipStream_t st) {
-    if (a.dtype == TVL_F32) return launch_forward_t<float>(a, cached, spans, st);
-    if (a.dtype == TVL_F16) return launch_forward_t<f16>(a, cached, spans, st);
-    return launch_forward_t<bf16_t>(a, cached, spans, st);
+    if (a.dtype == TVL_F32) return cached ? launch_forward_t<float, true>(a, spans, st) : launch_forward_t<float, false>(a, spans, st);
+    if (a.dtype == TVL_F16) return cached ? launch_forward_t<f16, true>(a, spans, st) : launch_forward_t<f16, false>(a, spans, st);
+    return cached ? launch_forward_t<bf16_t, true>(a, spans, st) : launch_forward_t<bf16_t, false>(a, spans, st);
 }
 
 }  // namespace tvl

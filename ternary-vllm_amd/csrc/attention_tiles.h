@@ -55,39 +55,12 @@ template <int R> __device__ __forceinline__ constexpr int result_row(int x, int 
 
 __device__ __forceinline__ bool not_finite(float v) { return (__builtin_bit_cast(uint32_t, v) & 0x7F800000u) == 0x7F800000u; }
 
-// some element of the fragment is an infinity or NaN (fragments of small tiles only: not on the main path)
-template <typename T> __device__ __forceinline__ bool any_not_finite(Frag<T> a) {
-    bool bad = false;
+// the fragment with zeros in place of infinities and NaN
+template <typename T> __device__ __forceinline__ Frag<T> finite_part(Frag<T> a) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) bad |= not_finite((float)a[e]);
-    return bad;
-}
-
-// acc += a * w where a holds infinities or NaN: pairs whose weight is zero add nothing, whatever a holds; the others add what they must
-// (an infinity of the element's sign for weights that cannot be negative, else NaN)
-template <typename T, int R, bool SIGNED>
-__device__ __forceinline__ Acc<R> mma_behind_mask(Frag<T> a, Frag<T> w, Acc<R> acc) {
-    Frag<T> clean, up, down, none, seen;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const float v = (float)a[e];
-        const bool bad = not_finite(v), nan = v != v;
-        clean[e] = bad ? (typename Operand<T>::elem)0.0f : a[e];
-        up[e] = (typename Operand<T>::elem)(bad && !nan && v > 0.0f ? 1.0f : 0.0f);
-        down[e] = (typename Operand<T>::elem)(bad && !nan && v < 0.0f ? 1.0f : 0.0f);
-        none[e] = (typename Operand<T>::elem)(nan ? 1.0f : 0.0f);
-        seen[e] = (typename Operand<T>::elem)((float)w[e] != 0.0f ? 1.0f : 0.0f);   // a NaN weight is not zero
-    }
-    acc = mma(clean, w, acc);
-    Acc<R> zero = {};
-    const Acc<R> ups = mma(up, seen, zero), downs = mma(down, seen, zero), nones = mma(none, seen, zero);
-#pragma unroll
-    for (int x = 0; x < REGS<R>; ++x) {
-        if (SIGNED ? ups[x] + downs[x] + nones[x] > 0.0f : nones[x] > 0.0f) acc[x] += __builtin_nanf("");
-        if (!SIGNED && ups[x] > 0.0f) acc[x] += __builtin_inff();
-        if (!SIGNED && downs[x] > 0.0f) acc[x] -= __builtin_inff();
-    }
-    return acc;
+    for (int e = 0; e < 8; ++e)
+        if (not_finite((float)a[e])) a[e] = (typename Operand<T>::elem)0.0f;
+    return a;
 }
 
 // ---- tiles in LDS ------------------------------------------------------------------------------
@@ -138,13 +111,48 @@ template <typename T, int DP> struct Tile {
     }
 };
 
-// 16 bytes of a row of `dim` elements, zeros behind them; `wide`: rows are 16-byte aligned and dim a multiple of the unit
-template <typename T>
-__device__ __forceinline__ u32x4 load_unit(const T* row, int unit, int dim, bool wide) {
+// A masked weight is zero, and zero times an infinity or NaN is NaN: where rows of a tile are seen by some columns of a wave's product and not by
+// others, the wave looks for such rows first.  If there are any it multiplies the finite part of the tile and adds what is not finite to
+// the columns that see it.
+template <typename T, int DP, int ROWS> __device__ __forceinline__ bool holds_not_finite(const char* tile, int lane) {
+    bool bad = false;
+#pragma unroll
+    for (int u = lane; u < ROWS * Tile<T, DP>::UNITS; u += 64) {
+        const u32x4 v = *reinterpret_cast<const u32x4*>(tile + 16 * u);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const uint32_t w = v[e];
+            if constexpr (sizeof(T) == 4) {
+                bad |= (w & 0x7F800000u) == 0x7F800000u;
+            } else {
+                constexpr uint32_t EXP = __is_same(T, f16) ? 0x7C00u : 0x7F80u;
+                bad |= (w & EXP) == EXP || (w & (EXP << 16)) == (EXP << 16);
+            }
+        }
+    }
+    return __any(bad);
+}
+// acc += the infinities and NaN of row `row`, where the lane's column sees it (`spoil`: NaN whatever the element is)
+template <typename T, int DP, int R>
+__device__ __forceinline__ void add_not_finite(const char* tile, int row, bool sees, bool spoil, int g, Acc<R>* acc) {
+#pragma unroll
+    for (int d = 0; d < DP / R; ++d)
+#pragma unroll
+        for (int x = 0; x < REGS<R>; ++x) {
+            const int col = d * R + result_row<R>(x, g);
+            constexpr int PER = Tile<T, DP>::PER;
+            const float v = to_float(*reinterpret_cast<const T*>(tile + Tile<T, DP>::at(row, col / PER) + (int)sizeof(T) * (col % PER)));
+            if (sees && not_finite(v)) acc[d][x] += spoil ? __builtin_nanf("") : v;
+        }
+}
+
+// 16 bytes of a row of `dim` elements, zeros behind them; WIDE: rows are 16-byte aligned and dim a multiple of the unit
+template <typename T, bool WIDE>
+__device__ __forceinline__ u32x4 load_unit(const T* row, int unit, int dim) {
     constexpr int PER = 16 / (int)sizeof(T);
     u32x4 v = {0, 0, 0, 0};
     const int c = unit * PER;
-    if (wide) {
+    if constexpr (WIDE) {
         if (c < dim) v = *reinterpret_cast<const u32x4*>(row + c);
     } else {
         T e[PER] = {};
@@ -157,29 +165,29 @@ __device__ __forceinline__ u32x4 load_unit(const T* row, int unit, int dim, bool
 }
 
 // fragment of a row straight from global memory (elements 8 c8 ..)
-template <typename T>
-__device__ __forceinline__ Frag<T> load_frag(const T* row, int c8, int dim, bool wide) {
+template <typename T, bool WIDE>
+__device__ __forceinline__ Frag<T> load_frag(const T* row, int c8, int dim) {
     if constexpr (sizeof(T) == 2) {
-        return __builtin_bit_cast(Frag<T>, load_unit<T>(row, c8, dim, wide));
+        return __builtin_bit_cast(Frag<T>, load_unit<T, WIDE>(row, c8, dim));
     } else {
-        const f32x4 lo = __builtin_bit_cast(f32x4, load_unit<T>(row, 2 * c8, dim, wide)), hi = __builtin_bit_cast(f32x4, load_unit<T>(row, 2 * c8 + 1, dim, wide));
+        const f32x4 lo = __builtin_bit_cast(f32x4, load_unit<T, WIDE>(row, 2 * c8, dim)), hi = __builtin_bit_cast(f32x4, load_unit<T, WIDE>(row, 2 * c8 + 1, dim));
         return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     }
 }
 
 // A tile's way from global memory to LDS through the registers of THREADS threads
-template <typename T, int DP, int ROWS, int THREADS> struct Stage {
+template <typename T, int DP, int ROWS, int THREADS, bool WIDE> struct Stage {
     typedef Tile<T, DP> L;
     static constexpr int N = ROWS * L::UNITS / THREADS;
     static_assert(ROWS * L::UNITS % THREADS == 0, "every thread moves the same number of units");
     u32x4 v[N];
     // rows row0 .. row0 + ROWS - 1 of a matrix; rows from `end` on are zero and not read
-    __device__ __forceinline__ void load(const T* base, int64_t stride, int row0, int end, int dim, bool wide) {
+    __device__ __forceinline__ void load(const T* base, int64_t stride, int row0, int end, int dim) {
 #pragma unroll
         for (int x = 0; x < N; ++x) {
             const int u = threadIdx.x + x * THREADS, row = u / L::UNITS, unit = u % L::UNITS;
             v[x] = u32x4{0, 0, 0, 0};
-            if (row0 + row < end) v[x] = load_unit<T>(base + (int64_t)(row0 + row) * stride, unit, dim, wide);
+            if (row0 + row < end) v[x] = load_unit<T, WIDE>(base + (int64_t)(row0 + row) * stride, unit, dim);
         }
     }
     __device__ __forceinline__ void store(char* tile) const {
@@ -199,6 +207,9 @@ __device__ __forceinline__ void both_halves(float v, float& lo, float& hi) {
     lo = __builtin_bit_cast(float, x);
     hi = __builtin_bit_cast(float, y);
 }
+// the wave's number in its workgroup, known to be the same for all its lanes
+__device__ __forceinline__ int wave_number() { return __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64); }
+
 // maximum / sum over the lanes that hold one column (the groups g)
 template <int R> __device__ __forceinline__ float column_max(float v) {
     float lo, hi;
@@ -289,7 +300,11 @@ __device__ __forceinline__ Place place_of(uint32_t id, int pairs, int group, int
     return Place{(int)pair, (int)(rest % group), tiles - 1 - (int)(rest / group)};
 }
 
+// Forms of a kernel.  PLAIN: wide rows, no cap, no bias, no documents.  GENERAL: wide rows, all of them.  ODD: any rows.
+enum Form { PLAIN, GENERAL, ODD };
+
 // host side
+static inline bool featureless(const tvl_attention_args& a) { return a.softcap == 0.0f && a.slopes == nullptr && a.documents == nullptr && a.scale != 0.0f; }
 static inline bool wide_rows(const void* p, int64_t dim, int64_t s0, int64_t s1, int64_t s2, size_t z) {
     const int64_t per = (int64_t)(16 / z);
     return aligned(p, 16) && dim % per == 0 && s0 % per == 0 && s1 % per == 0 && s2 % per == 0;
