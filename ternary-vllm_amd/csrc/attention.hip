@@ -29,8 +29,9 @@ static int check(const tvl_attention_args* a, const char* who, bool cached) {
     TVL_REQUIRE(a->heads > 0 && a->kv_heads > 0 && a->heads % a->kv_heads == 0, "%s: heads=%lld must be a multiple of kv_heads=%lld", who, (long long)a->heads, (long long)a->kv_heads);
     TVL_REQUIRE(a->dim >= 1 && a->dim <= ATTENTION_MAX_DIM, "%s: head dim %lld outside [1, %d]", who, (long long)a->dim, ATTENTION_MAX_DIM);
     TVL_REQUIRE(a->heads <= (1 << 16) && a->batch <= (1 << 20) && a->queries <= (1 << 30) && a->keys <= (1 << 30), "%s: batch, heads or tokens too large", who);
-    // every launch stays under 2^24 workgroups (2^32 threads): the smallest work item is one tile of 64 rows
-    TVL_REQUIRE(a->batch * a->heads * ceil_div(cached || a->queries > a->keys ? a->queries : a->keys, 64) < ((int64_t)1 << 24), "%s: too many rows for one launch", who);
+    // every launch stays under 2^32 threads: at least 64 rows for each 256 of them, a cache's steps 16 rows for 512
+    const int64_t most = cached || a->queries > a->keys ? a->queries : a->keys;
+    TVL_REQUIRE(a->batch * a->heads * ceil_div(most, cached ? 16 : 64) < ((int64_t)1 << (cached ? 23 : 24)), "%s: too many rows for one launch", who);
     TVL_REQUIRE(a->scale == a->scale && a->scale - a->scale == 0.0f, "%s: scale must be finite", who);
     TVL_REQUIRE(a->softcap >= 0.0f && a->softcap - a->softcap == 0.0f, "%s: softcap must be finite and not negative", who);
     TVL_REQUIRE(cached || a->documents == nullptr || a->queries == a->keys, "%s: documents need as many queries as keys", who);
@@ -100,13 +101,16 @@ int tvl_attention_backward(const tvl_attention_args* a, const tvl_attention_grad
     return launch_attention_backward(*a, *g, spans, delta, maxima, st);
 }
 
-size_t tvl_cached_attention_workspace_bytes(const tvl_attention_args* a) { (void)a; return 0; }
+size_t tvl_cached_attention_workspace_bytes(const tvl_attention_args* a) {
+    return a && any_rows(*a) && a->kv_heads > 0 && attention_step_serves(*a) ? round256(attention_step_bytes(*a)) : 0;
+}
 
 int tvl_cached_attention(const tvl_attention_args* a, void* workspace, size_t workspace_bytes, void* stream) {
     if (const int rc = check(a, "cached_attention", true); rc != TVL_OK) return rc;
     if (a->batch == 0 || a->queries == 0) return TVL_OK;
-    (void)workspace; (void)workspace_bytes;
-    return launch_attention_forward(*a, true, nullptr, (hipStream_t)stream);
+    if (const int rc = check_workspace("cached_attention", tvl_cached_attention_workspace_bytes(a), workspace, workspace_bytes); rc != TVL_OK) return rc;
+    hipStream_t st = (hipStream_t)stream;
+    return attention_step_serves(*a) ? launch_attention_step(*a, static_cast<float*>(workspace), st) : launch_attention_forward(*a, true, nullptr, st);
 }
 
 }  // extern "C"

@@ -312,6 +312,9 @@ static inline bool wide_rows(const void* p, int64_t dim, int64_t s0, int64_t s1,
 
 int launch_attention_forward(const tvl_attention_args& a, bool cached, const DocumentSpan* spans, hipStream_t st);
 int launch_attention_backward(const tvl_attention_args& a, const tvl_attention_grads& g, const DocumentSpan* spans, float* delta, float* maxima, hipStream_t st);
+bool attention_step_serves(const tvl_attention_args& a);
+size_t attention_step_bytes(const tvl_attention_args& a);
+int launch_attention_step(const tvl_attention_args& a, float* parts, hipStream_t st);
 int launch_document_spans(const tvl_attention_args& a, DocumentSpan* spans, hipStream_t st);
 
 }  // namespace tvl
