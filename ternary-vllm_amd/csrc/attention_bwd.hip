@@ -65,7 +65,7 @@ __global__ void __launch_bounds__(256, DP == 64 && sizeof(T) == 2 ? 2 : 1) atten
     typedef Tile<T, DP> L;
     typedef typename Operand<T>::elem E;
     extern __shared__ __align__(16) char lds[];
-    constexpr int TILE = GT * L::ROW;
+    constexpr int TILE = GT * L::ROW, BUFFER = 2 * TILE + (FORM == PLAIN ? 0 : GT * 8);     // keys, values, documents
 
     const int group = (int)(a.heads / a.kv_heads), pairs = (int)(a.batch * a.kv_heads);
     const Place at = place_of(blockIdx.x, pairs, group, tiles);
@@ -76,21 +76,19 @@ __global__ void __launch_bounds__(256, DP == 64 && sizeof(T) == 2 ? 2 : 1) atten
     bool lost;
     const Sequence seq = sequence_of<false>(a, b, lost);
     const int last = q0 + QB < queries ? q0 + QB : queries, reach = seq.limit(last - 1);
-    const int all = FORM != PLAIN && a.documents ? 0 : seq.limit(q0);      // keys every query of the block sees
+    const int all = seq.limit(q0);      // keys every query of the block sees
     const int wlast = qw + R < queries ? qw + R : queries;
     const int wreach = wlast > qw ? seq.limit(wlast - 1) : 0, wall = wlast > qw ? seq.limit(qw) : 0;
     const int mine = i < queries ? seq.limit(i) : 0;
     const T* kp = (const T*)a.k + b * a.k_batch + hk * a.k_head;
     const T* vp = (const T*)a.v + b * a.v_batch + hk * a.v_head;
     const int64_t* docs = FORM == PLAIN ? nullptr : a.documents;
-    int64_t doc = -1, dlo = 0, dhi = -1;
+    int64_t doc = -1;
+    DocumentWindow docw;
     if (docs) {
         docs += b * a.documents_batch;
-        spans += (int64_t)b * ((queries + SPAN - 1) / SPAN);
         if (i < queries) doc = docs[i];
-        const DocumentSpan s0 = spans[q0 / SPAN], s1 = q0 + SPAN < queries ? spans[q0 / SPAN + 1] : s0;
-        dlo = s0.lo < s1.lo ? s0.lo : s1.lo;
-        dhi = s0.hi > s1.hi ? s0.hi : s1.hi;
+        docw.start(spans + (int64_t)b * ((queries + SPAN - 1) / SPAN), queries, q0, QB);
     }
     Frag<T> qf[DP / CK], gf[DP / CK];
     float lse = 0.0f, dl = 0.0f, top = 0.0f;
@@ -123,30 +121,33 @@ __global__ void __launch_bounds__(256, DP == 64 && sizeof(T) == 2 ? 2 : 1) atten
     const float pre = capped ? 1.0f : to_log2, unit = capped || biased ? 1.0f : to_log2;
     Acc<R> acc[DP / R] = {};
 
-    auto skip = [&](int j0) { return docs && (spans[j0 / SPAN].hi < dlo || spans[j0 / SPAN].lo > dhi || spans[j0 / SPAN].hi < 0); };
-    auto next = [&](int j0) {
-        while (j0 < reach && skip(j0)) j0 += GT;
-        return j0;
-    };
+    auto next = [&](int j) { return docs && j < reach ? docw.next(j / SPAN, (reach + SPAN - 1) / SPAN, lane) * SPAN : j; };
     Stage<T, DP, GT, 256, WIDE> sk, sv;
+    int64_t side = -1;
+    auto fetch = [&](int j) {
+        sk.load(kp, a.k_token, j, seq.end, dim);
+        sv.load(vp, a.v_token, j, seq.end, dim);
+        if (docs && threadIdx.x < GT) side = j + (int)threadIdx.x < seq.end ? docs[j + threadIdx.x] : -1;
+    };
+    auto put = [&](char* to) {
+        sk.store(to);
+        sv.store(to + TILE);
+        if (docs && threadIdx.x < GT) reinterpret_cast<int64_t*>(to + 2 * TILE)[threadIdx.x] = side;
+    };
     int j0 = next(0), buf = 0;
     if (j0 < reach) {
-        sk.load(kp, a.k_token, j0, seq.end, dim);
-        sv.load(vp, a.v_token, j0, seq.end, dim);
-        sk.store(lds);
-        sv.store(lds + TILE);
+        fetch(j0);
+        put(lds);
     }
     __syncthreads();
     // MASKED: some query of the block does not see some key of the tile
     auto step = [&](auto masked) __attribute__((always_inline)) {
         constexpr bool MASKED = decltype(masked)::value;
         const int j1 = next(j0 + GT);
-        if (j1 < reach) {
-            sk.load(kp, a.k_token, j1, seq.end, dim);
-            sv.load(vp, a.v_token, j1, seq.end, dim);
-        }
-        const char *kt = lds + buf * 2 * TILE, *vt = kt + TILE;
-        const bool one_document = !MASKED || !docs || (dlo == dhi && dlo >= 0 && spans[j0 / SPAN].lo == dlo && spans[j0 / SPAN].hi == dlo);
+        if (j1 < reach) fetch(j1);
+        const char *kt = lds + buf * BUFFER, *vt = kt + TILE;
+        const int64_t* kdocs = reinterpret_cast<const int64_t*>(kt + 2 * TILE);
+        const bool one_document = !MASKED || !docs || docw.one(j0 / SPAN, lane);
 #pragma unroll 1
         for (int t = 0; t < GT; t += R) {
             const int jt = j0 + t;
@@ -183,10 +184,8 @@ __global__ void __launch_bounds__(256, DP == 64 && sizeof(T) == 2 ? 2 : 1) atten
                     if (result_row<R>(x, 0) >= left) dp[x] = 0.0f;
                 if (!one_document) {
 #pragma unroll
-                    for (int x = 0; x < REGS<R>; ++x) {
-                        const int j = jt + result_row<R>(x, g);
-                        if (doc < 0 || docs[j < seq.end ? j : 0] != doc) dp[x] = 0.0f;
-                    }
+                    for (int x = 0; x < REGS<R>; ++x)
+                        if (!same_document<R>(kdocs + t + 4 * g, x, doc)) dp[x] = 0.0f;
                 }
             }
             // score gradients are rounded to the operands' type for the last product; its sum is float32
@@ -199,7 +198,7 @@ __global__ void __launch_bounds__(256, DP == 64 && sizeof(T) == 2 ? 2 : 1) atten
                     for (int d = 0; d < DP / R; ++d) acc[d] = mma(finite_part<T>(L::template read_across<R>(kt, t + c * CK, d * R, lane)), df[c], acc[d]);
 #pragma unroll 1
                 for (int row = 0; row < R && jt + row < reach; ++row)
-                    add_not_finite<T, DP, R>(kt, t + row, jt + row < mine && (one_document || (doc >= 0 && docs[jt + row] == doc)), true, g, acc);
+                    add_not_finite<T, DP, R>(kt, t + row, jt + row < mine && (one_document || (doc >= 0 && kdocs[t + row] == doc)), true, g, acc);
             } else {
 #pragma unroll
                 for (int c = 0; c < R / CK; ++c)
@@ -207,16 +206,16 @@ __global__ void __launch_bounds__(256, DP == 64 && sizeof(T) == 2 ? 2 : 1) atten
                     for (int d = 0; d < DP / R; ++d) acc[d] = mma(L::template read_across<R>(kt, t + c * CK, d * R, lane), df[c], acc[d]);
             }
         }
-        if (j1 < reach) {
-            sk.store(lds + (buf ^ 1) * 2 * TILE);
-            sv.store(lds + (buf ^ 1) * 2 * TILE + TILE);
-        }
+        if (j1 < reach) put(lds + (buf ^ 1) * BUFFER);
         __syncthreads();
         buf ^= 1;
         j0 = j1;
     };
-    while (j0 < reach && j0 + GT <= all) step(std::false_type{});
-    while (j0 < reach) step(std::true_type{});
+    auto clean = [&](int j) { return j + GT <= all && (!docs || docw.one(j / SPAN, lane)); };
+    while (j0 < reach) {
+        while (j0 < reach && clean(j0)) step(std::false_type{});
+        while (j0 < reach && !clean(j0)) step(std::true_type{});
+    }
     if (i >= queries) return;
     const float back = a.scale * power_of_two(e);
     T* op = (T*)gr.dq + (((int64_t)b * queries + i) * a.heads + h) * dim;
@@ -239,7 +238,7 @@ __global__ void __launch_bounds__(256, DP == 64 && sizeof(T) == 2 ? 2 : 1) atten
     typedef Tile<T, DP> L;
     typedef typename Operand<T>::elem E;
     extern __shared__ __align__(16) char lds[];
-    constexpr int TILE = GT * L::ROW, STEP = 2 * TILE + 2 * GT * 4;     // q, grad_out, log-sums, deltas
+    constexpr int TILE = GT * L::ROW, STEP = 2 * TILE + 2 * GT * 4 + (FORM == PLAIN ? 0 : GT * 8);     // q, grad_out, log-sums, deltas, documents
 
     const int group = (int)(a.heads / a.kv_heads), pairs = (int)(a.batch * a.kv_heads);
     const Place at = place_of(blockIdx.x, pairs, 1, tiles);
@@ -250,14 +249,12 @@ __global__ void __launch_bounds__(256, DP == 64 && sizeof(T) == 2 ? 2 : 1) atten
     bool lost;
     const Sequence seq = sequence_of<false>(a, b, lost);
     const int64_t* docs = FORM == PLAIN ? nullptr : a.documents;
-    int64_t doc = -1, dlo = 0, dhi = -1;
+    int64_t doc = -1;
+    DocumentWindow docw;
     if (docs) {
         docs += b * a.documents_batch;
-        spans += (int64_t)b * ((queries + SPAN - 1) / SPAN);
         if (j < keys) doc = docs[j];
-        const DocumentSpan s0 = spans[k0 / SPAN], s1 = k0 + SPAN < keys ? spans[k0 / SPAN + 1] : s0;
-        dlo = s0.lo < s1.lo ? s0.lo : s1.lo;
-        dhi = s0.hi > s1.hi ? s0.hi : s1.hi;
+        docw.start(spans + (int64_t)b * ((queries + SPAN - 1) / SPAN), queries, k0, KB);
     }
     Frag<T> kf[DP / CK], vf[DP / CK];
 #pragma unroll
@@ -288,17 +285,19 @@ __global__ void __launch_bounds__(256, DP == 64 && sizeof(T) == 2 ? 2 : 1) atten
     int begin = seq.causal && k0 >= seq.prefix ? k0 - seq.shift : 0;
     begin = begin < 0 ? 0 : begin / GT * GT;
     const int steps = begin < queries ? (queries - begin + GT - 1) / GT : 0, total = steps * group;
-    auto skip = [&](int n) {
-        if (!docs) return false;
-        const DocumentSpan s = spans[(begin + (n % steps) * GT) / SPAN];
-        return s.hi < dlo || s.lo > dhi || s.hi < 0;
-    };
+    // steps in order: tiles of the first head, then of the next; tiles without a document of the block's are skipped
     auto next = [&](int n) {
-        while (n < total && skip(n)) ++n;
+        if (!docs) return n;
+        while (n < total) {
+            const int from = n / steps * steps, at = begin / SPAN, m = docw.next(at + n - from, at + steps, lane) - at;
+            if (m < steps) return from + m;
+            n = from + steps;
+        }
         return n;
     };
     Stage<T, DP, GT, 256, WIDE> sq, sg;
     float side = 0.0f;      // threads 0..63: a log-sum, 64..127: a delta
+    int64_t qdoc = -1;      // threads 0..63
     auto fetch = [&](int n) {
         const int h = hk * group + n / steps, i0 = begin + (n % steps) * GT;
         sq.load((const T*)a.q + b * a.q_batch + h * a.q_head, a.q_token, i0, queries, dim);
@@ -308,11 +307,13 @@ __global__ void __launch_bounds__(256, DP == 64 && sizeof(T) == 2 ? 2 : 1) atten
         // a query behind the last gets weights exp(-inf) = 0
         if (threadIdx.x < 64) side = i < queries ? a.lse[row] * LOG2E : __builtin_inff();
         else if (threadIdx.x < 128) side = i < queries ? delta[row] * fit : 0.0f;
+        if (docs && threadIdx.x < GT) qdoc = i < queries ? docs[i] : -1;
     };
     auto put = [&](char* to) {
         sq.store(to);
         sg.store(to + TILE);
         if (threadIdx.x < 128) *reinterpret_cast<float*>(to + 2 * TILE + 4 * threadIdx.x) = side;
+        if (docs && threadIdx.x < GT) reinterpret_cast<int64_t*>(to + 2 * TILE + 2 * GT * 4)[threadIdx.x] = qdoc;
     };
     int n = next(0), buf = 0;
     if (n < total) {
@@ -327,9 +328,10 @@ __global__ void __launch_bounds__(256, DP == 64 && sizeof(T) == 2 ? 2 : 1) atten
         if (n1 < total) fetch(n1);
         const char *qt = lds + buf * STEP, *gt = qt + TILE;
         const float *lses = reinterpret_cast<const float*>(qt + 2 * TILE), *deltas = lses + GT;
+        const int64_t* qdocs = reinterpret_cast<const int64_t*>(deltas + GT);
         const int h = hk * group + n / steps, i0 = begin + (n % steps) * GT;
         const float slope = biased ? a.slopes[h] * LOG2E : 0.0f;
-        const bool one_document = !MASKED || !docs || (dlo == dhi && dlo >= 0 && spans[i0 / SPAN].lo == dlo && spans[i0 / SPAN].hi == dlo);
+        const bool one_document = !MASKED || !docs || docw.one(i0 / SPAN, lane);
 #pragma unroll 1
         for (int t = 0; t < GT; t += R) {
             const int it = i0 + t;
@@ -374,10 +376,8 @@ __global__ void __launch_bounds__(256, DP == 64 && sizeof(T) == 2 ? 2 : 1) atten
                     if (result_row<R>(x, 0) < from) s[x] = dp[x] = 0.0f;
                 if (!one_document) {
 #pragma unroll
-                    for (int x = 0; x < REGS<R>; ++x) {
-                        const int i = it + result_row<R>(x, g);
-                        if (doc < 0 || docs[i < queries ? i : 0] != doc) s[x] = dp[x] = 0.0f;
-                    }
+                    for (int x = 0; x < REGS<R>; ++x)
+                        if (!same_document<R>(qdocs + t + 4 * g, x, doc)) s[x] = dp[x] = 0.0f;
                 }
             }
             // weights and score gradients are rounded to the operands' type for the last products; their sums are float32
@@ -396,7 +396,7 @@ __global__ void __launch_bounds__(256, DP == 64 && sizeof(T) == 2 ? 2 : 1) atten
                     }
 #pragma unroll 1
                 for (int row = 0; row < R && it + row < queries; ++row) {
-                    const bool sees = j < seq.limit(it + row) && (one_document || (doc >= 0 && docs[it + row] == doc));
+                    const bool sees = j < seq.limit(it + row) && (one_document || (doc >= 0 && qdocs[t + row] == doc));
                     add_not_finite<T, DP, R>(gt, t + row, sees, false, g, dv);
                     add_not_finite<T, DP, R>(qt, t + row, sees, true, g, dk);
                 }
@@ -415,10 +415,13 @@ __global__ void __launch_bounds__(256, DP == 64 && sizeof(T) == 2 ? 2 : 1) atten
         buf ^= 1;
         n = n1;
     };
-    auto unmasked = [&](int m) { return !docs && seq.limit(begin + (m % steps) * GT) >= k0 + KB; };
+    auto clean = [&](int m) {
+        const int i0 = begin + (m % steps) * GT;
+        return seq.limit(i0) >= k0 + KB && (!docs || docw.one(i0 / SPAN, lane));
+    };
     while (n < total) {
-        while (n < total && !unmasked(n)) step(std::true_type{});
-        while (n < total && unmasked(n)) step(std::false_type{});
+        while (n < total && !clean(n)) step(std::true_type{});
+        while (n < total && clean(n)) step(std::false_type{});
     }
     if (j >= keys) return;
     const float back = a.scale * power_of_two(e);
@@ -439,14 +442,14 @@ template <typename T, int DP, Form FORM>
 static int launch_gradients(const tvl_attention_args& a, const tvl_attention_grads& g, const DocumentSpan* spans, const float* delta, const float* maxima, hipStream_t st) {
     if (g.dq && a.queries > 0) {
         const int tiles = (int)ceil_div(a.queries, 128);
-        const size_t bytes = 4 * GT * (size_t)Tile<T, DP>::ROW;
+        const size_t bytes = 4 * GT * (size_t)Tile<T, DP>::ROW + (FORM == PLAIN ? 0 : 2 * GT * 8);
         if (bytes > 65536) TVL_HIP_CHECK(hipFuncSetAttribute((const void*)attention_dq_kernel<T, DP, FORM>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
         hipLaunchKernelGGL((attention_dq_kernel<T, DP, FORM>), dim3((unsigned)(a.batch * a.heads * tiles)), dim3(256), bytes, st, a, g, spans, delta, tiles);
         TVL_LAUNCH_CHECK();
     }
     if (g.dk && a.keys > 0) {
         const int tiles = (int)ceil_div(a.keys, 128);
-        const size_t bytes = 2 * (2 * GT * (size_t)Tile<T, DP>::ROW + 2 * GT * 4);
+        const size_t bytes = 2 * (2 * GT * (size_t)Tile<T, DP>::ROW + 2 * GT * 4 + (FORM == PLAIN ? 0 : GT * 8));
         if (bytes > 65536) TVL_HIP_CHECK(hipFuncSetAttribute((const void*)attention_dkv_kernel<T, DP, FORM>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
         hipLaunchKernelGGL((attention_dkv_kernel<T, DP, FORM>), dim3((unsigned)(a.batch * a.kv_heads * tiles)), dim3(256), bytes, st, a, g, spans, delta, maxima, tiles);
         TVL_LAUNCH_CHECK();

@@ -16,7 +16,7 @@ __global__ void __launch_bounds__(256, DP == 64 && sizeof(T) == 2 ? 2 : 1) atten
     constexpr int R = 32, KT = 64, QB = 128, CK = CHUNK<R>;
     typedef Tile<T, DP> L;
     extern __shared__ __align__(16) char lds[];
-    constexpr int TILE = KT * L::ROW;
+    constexpr int TILE = KT * L::ROW, BUFFER = 2 * TILE + (FORM == PLAIN ? 0 : KT * 8);     // keys, values, documents
 
     const int group = (int)(a.heads / a.kv_heads), pairs = (int)(a.batch * a.kv_heads);
     const Place at = place_of(blockIdx.x, pairs, group, tiles);
@@ -29,7 +29,7 @@ __global__ void __launch_bounds__(256, DP == 64 && sizeof(T) == 2 ? 2 : 1) atten
     const Sequence seq = sequence_of<CACHED>(a, b, lost);
     const int last = q0 + QB < seq.real ? q0 + QB : seq.real;                  // real queries of this block end here
     const int reach = last > q0 ? seq.limit(last - 1) : 0;                      // limits grow with the query
-    const int all = last > q0 && !(FORM != PLAIN && !CACHED && a.documents) ? seq.limit(q0) : 0;      // keys every real query of the block sees
+    const int all = last > q0 ? seq.limit(q0) : 0;                              // keys every real query of the block sees
     const int wlast = qw + R < seq.real ? qw + R : seq.real;
     const int wreach = wlast > qw ? seq.limit(wlast - 1) : 0, wall = wlast > qw ? seq.limit(qw) : 0;   // keys some / every query of the wave sees
     const int mine = i < seq.real ? seq.limit(i) : 0;
@@ -38,14 +38,12 @@ __global__ void __launch_bounds__(256, DP == 64 && sizeof(T) == 2 ? 2 : 1) atten
     const T* vp = (const T*)a.v + b * a.v_batch + hk * a.v_head;
     const T* qp = (const T*)a.q + b * a.q_batch + h * a.q_head + (int64_t)i * a.q_token;
     const int64_t* docs = CACHED || FORM == PLAIN ? nullptr : a.documents;
-    int64_t doc = -1, dlo = 0, dhi = -1;
+    int64_t doc = -1;
+    DocumentWindow docw;
     if (docs) {
         docs += b * a.documents_batch;
-        spans += (int64_t)b * ((queries + SPAN - 1) / SPAN);
         if (i < queries) doc = docs[i];
-        const DocumentSpan s0 = spans[q0 / SPAN], s1 = q0 + SPAN < queries ? spans[q0 / SPAN + 1] : s0;
-        dlo = s0.lo < s1.lo ? s0.lo : s1.lo;
-        dhi = s0.hi > s1.hi ? s0.hi : s1.hi;
+        docw.start(spans + (int64_t)b * ((queries + SPAN - 1) / SPAN), queries, q0, QB);
     }
 
     // a negative scale goes into the queries' sign, so that the largest product is the largest score
@@ -66,30 +64,33 @@ __global__ void __launch_bounds__(256, DP == 64 && sizeof(T) == 2 ? 2 : 1) atten
     Acc<R> acc[DP / R] = {};
     float m = -__builtin_inff(), base = 0.0f, sum = 0.0f;
 
-    // tiles that no query of the block meets are skipped
-    auto skip = [&](int j0) { return docs && (spans[j0 / SPAN].hi < dlo || spans[j0 / SPAN].lo > dhi || spans[j0 / SPAN].hi < 0); };
-    auto next = [&](int j0) {
-        while (j0 < reach && skip(j0)) j0 += KT;
-        return j0;
-    };
+    // tiles whose documents no query of the block has are skipped
+    auto next = [&](int j) { return docs && j < reach ? docw.next(j / SPAN, (reach + SPAN - 1) / SPAN, lane) * SPAN : j; };
     Stage<T, DP, KT, 256, WIDE> sk, sv;
+    int64_t side = -1;
+    auto fetch = [&](int j) {
+        sk.load(kp, a.k_token, j, seq.end, dim);
+        sv.load(vp, a.v_token, j, seq.end, dim);
+        if (docs && threadIdx.x < KT) side = j + (int)threadIdx.x < seq.end ? docs[j + threadIdx.x] : -1;
+    };
+    auto put = [&](char* to) {
+        sk.store(to);
+        sv.store(to + TILE);
+        if (docs && threadIdx.x < KT) reinterpret_cast<int64_t*>(to + 2 * TILE)[threadIdx.x] = side;
+    };
     int j0 = next(0), buf = 0;
     if (j0 < reach) {
-        sk.load(kp, a.k_token, j0, seq.end, dim);
-        sv.load(vp, a.v_token, j0, seq.end, dim);
-        sk.store(lds);
-        sv.store(lds + TILE);
+        fetch(j0);
+        put(lds);
     }
     __syncthreads();
     // MASKED: some query of the block does not see some key of the tile
     auto step = [&](auto masked) __attribute__((always_inline)) {
         constexpr bool MASKED = decltype(masked)::value;
         const int j1 = next(j0 + KT);
-        if (j1 < reach) {
-            sk.load(kp, a.k_token, j1, seq.end, dim);
-            sv.load(vp, a.v_token, j1, seq.end, dim);
-        }
-        const char *kt = lds + buf * 2 * TILE, *vt = kt + TILE;
+        if (j1 < reach) fetch(j1);
+        const char *kt = lds + buf * BUFFER, *vt = kt + TILE;
+        const int64_t* kdocs = reinterpret_cast<const int64_t*>(kt + 2 * TILE);
         if (!MASKED || j0 < wreach) {
             Acc<R> s[KT / R];
 #pragma unroll
@@ -99,7 +100,7 @@ __global__ void __launch_bounds__(256, DP == 64 && sizeof(T) == 2 ? 2 : 1) atten
                 for (int c = 0; c < DP / CK; ++c) s[t] = mma(L::read(kt, t * R + r, g + (64 / R) * c), qf[c], s[t]);
             }
             // scores: units of `unit` powers of two
-            const bool one_document = !MASKED || !docs || (dlo == dhi && dlo >= 0 && spans[j0 / SPAN].lo == dlo && spans[j0 / SPAN].hi == dlo);
+            const bool one_document = !MASKED || !docs || docw.one(j0 / SPAN, lane);
             if (capped) {
 #pragma unroll
                 for (int t = 0; t < KT / R; ++t)
@@ -127,10 +128,8 @@ __global__ void __launch_bounds__(256, DP == 64 && sizeof(T) == 2 ? 2 : 1) atten
 #pragma unroll
                     for (int t = 0; t < KT / R; ++t)
 #pragma unroll
-                        for (int x = 0; x < REGS<R>; ++x) {
-                            const int j = j0 + t * R + result_row<R>(x, g);
-                            if (doc < 0 || docs[j < seq.end ? j : 0] != doc) s[t][x] = -__builtin_inff();
-                        }
+                        for (int x = 0; x < REGS<R>; ++x)
+                            if (!same_document<R>(kdocs + t * R + 4 * g, x, doc)) s[t][x] = -__builtin_inff();
                 }
             }
             float top = s[0][0];
@@ -166,7 +165,7 @@ __global__ void __launch_bounds__(256, DP == 64 && sizeof(T) == 2 ? 2 : 1) atten
                     for (int d = 0; d < DP / R; ++d) acc[d] = mma(finite_part<T>(L::template read_across<R>(vt, c * CK, d * R, lane)), pf[c], acc[d]);
 #pragma unroll 1
                 for (int row = 0; row < KT && j0 + row < reach; ++row)
-                    add_not_finite<T, DP, R>(vt, row, j0 + row < mine && (one_document || (doc >= 0 && docs[j0 + row] == doc)), false, g, acc);
+                    add_not_finite<T, DP, R>(vt, row, j0 + row < mine && (one_document || (doc >= 0 && kdocs[row] == doc)), false, g, acc);
             } else {
 #pragma unroll
                 for (int c = 0; c < KT / CK; ++c)
@@ -174,16 +173,16 @@ __global__ void __launch_bounds__(256, DP == 64 && sizeof(T) == 2 ? 2 : 1) atten
                     for (int d = 0; d < DP / R; ++d) acc[d] = mma(L::template read_across<R>(vt, c * CK, d * R, lane), pf[c], acc[d]);
             }
         }
-        if (j1 < reach) {
-            sk.store(lds + (buf ^ 1) * 2 * TILE);
-            sv.store(lds + (buf ^ 1) * 2 * TILE + TILE);
-        }
+        if (j1 < reach) put(lds + (buf ^ 1) * BUFFER);
         __syncthreads();
         buf ^= 1;
         j0 = j1;
     };
-    while (j0 < reach && j0 + KT <= all) step(std::false_type{});
-    while (j0 < reach) step(std::true_type{});
+    auto clean = [&](int j) { return j + KT <= all && (!docs || docw.one(j / SPAN, lane)); };
+    while (j0 < reach) {
+        while (j0 < reach && clean(j0)) step(std::false_type{});
+        while (j0 < reach && !clean(j0)) step(std::true_type{});
+    }
 
     sum = column_sum<R>(sum);
     if (i >= queries) return;
@@ -211,16 +210,18 @@ __global__ void __launch_bounds__(256, DP == 64 && sizeof(T) == 2 ? 2 : 1) atten
     if (!CACHED && a.lse && g == 0) a.lse[((int64_t)b * a.heads + h) * queries + i] = sum == 0.0f ? -__builtin_inff() : (base + __builtin_amdgcn_logf(sum)) * LN2;
 }
 
-// spans[b][n]: smallest and largest document of tokens 64 n .. 64 n + 63
+// spans[b][n] of tokens 64 n .. 64 n + 63
 __global__ void __launch_bounds__(64) document_spans_kernel(const int64_t* __restrict__ documents, int64_t stride, int tokens, int blocks, DocumentSpan* __restrict__ spans) {
     const int b = blockIdx.x / blocks, n = blockIdx.x % blocks, i = n * SPAN + threadIdx.x;
-    int64_t lo = documents[b * stride + (i < tokens ? i : n * SPAN)], hi = lo;
+    const int64_t doc = documents[b * stride + (i < tokens ? i : n * SPAN)];
+    int64_t lo = doc < 0 ? INT64_MAX : doc, hi = doc < 0 ? -1 : doc;
     for (int o = 32; o > 0; o >>= 1) {
         const int64_t l = __shfl_xor((long long)lo, o), u = __shfl_xor((long long)hi, o);
         lo = l < lo ? l : lo;
         hi = u > hi ? u : hi;
     }
-    if (threadIdx.x == 0) spans[blockIdx.x] = DocumentSpan{lo, hi};
+    const bool whole = __all(doc >= 0);
+    if (threadIdx.x == 0) spans[blockIdx.x] = DocumentSpan{lo, hi, whole};
 }
 
 int launch_document_spans(const tvl_attention_args& a, DocumentSpan* spans, hipStream_t st) {
@@ -233,7 +234,7 @@ int launch_document_spans(const tvl_attention_args& a, DocumentSpan* spans, hipS
 template <typename T, int DP, bool CACHED, Form FORM>
 static int launch_forward(const tvl_attention_args& a, const DocumentSpan* spans, hipStream_t st) {
     const int tiles = (int)ceil_div(a.queries, 128);
-    const size_t bytes = 4 * 64 * (size_t)Tile<T, DP>::ROW;
+    const size_t bytes = 4 * 64 * (size_t)Tile<T, DP>::ROW + (FORM == PLAIN ? 0 : 2 * 64 * 8);
     if (bytes > 65536) TVL_HIP_CHECK(hipFuncSetAttribute((const void*)attention_forward_kernel<T, DP, CACHED, FORM>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
     hipLaunchKernelGGL((attention_forward_kernel<T, DP, CACHED, FORM>), dim3((unsigned)(a.batch * a.heads * tiles)), dim3(256), bytes, st, a, spans, tiles);
     TVL_LAUNCH_CHECK();

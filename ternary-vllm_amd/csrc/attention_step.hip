@@ -198,35 +198,62 @@ __global__ void __launch_bounds__(64 * WAVES) attention_step_kernel(tvl_attentio
     }
 }
 
-// out of the parts of a long cache: one wave per row
+// out of the parts of a long cache: one workgroup per row; the parts' maxima and sums first, then every wave adds its share of the accumulators
+constexpr int MOST_PARTS = 512;
 template <typename T, int DP>
 __global__ void __launch_bounds__(256) attention_join_kernel(tvl_attention_args a, int splits, const float* __restrict__ parts) {
-    const int group = (int)(a.heads / a.kv_heads), rows = (int)a.queries * group, lane = threadIdx.x % 64;
-    const int64_t n = (int64_t)blockIdx.x * 4 + threadIdx.x / 64;
-    if (n >= a.batch * a.kv_heads * rows) return;
-    const int pair = (int)(n / rows), row = (int)(n % rows), i = row / group, b = pair / (int)a.kv_heads, h = pair % (int)a.kv_heads * group + row % group;
-    bool lost;
-    const Sequence seq = sequence_of<true>(a, b, lost);
+    __shared__ float factor[MOST_PARTS], side[4], sums[4][DP];
+    const int group = (int)(a.heads / a.kv_heads), rows = (int)a.queries * group, lane = threadIdx.x % 64, wave = wave_number();
+    const int pair = (int)(blockIdx.x / (unsigned)rows), row = (int)(blockIdx.x % (unsigned)rows), i = row / group, b = pair / (int)a.kv_heads, h = pair % (int)a.kv_heads * group + row % group;
     const float* part = parts + ((int64_t)pair * splits * rows + row) * (DP + 2);
     const int64_t stride = (int64_t)rows * (DP + 2);
-    float top = -__builtin_inff();
-    for (int s = lane; s < splits; s += 64) top = fmaxf(top, part[s * stride]);
-    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-    const float from = top == -__builtin_inff() ? 0.0f : top;
-    float total = 0.0f, acc[DP / 64] = {};
-    for (int s = 0; s < splits; ++s) {
-        const float m = part[s * stride], ws = part[s * stride + 1];
-        if (ws == 0.0f) continue;
-        const float f = __builtin_amdgcn_exp2f((m == -__builtin_inff() ? 0.0f : m) - from);
-        total += f * ws;
+    float m[MOST_PARTS / 256], ws[MOST_PARTS / 256], top = -__builtin_inff();
 #pragma unroll
-        for (int d = 0; d < DP / 64; ++d) acc[d] += f * part[s * stride + 2 + lane + 64 * d];
+    for (int x = 0; x < MOST_PARTS / 256; ++x) {
+        const int s = threadIdx.x + 256 * x;
+        m[x] = -__builtin_inff();
+        ws[x] = 0.0f;
+        if (s < splits) { m[x] = part[s * stride]; ws[x] = part[s * stride + 1]; }
+        top = fmaxf(top, m[x]);
     }
-    const bool empty = total == 0.0f || i >= seq.real, nan = i < seq.real && (lost || seq.shift + i >= (int)a.keys);
-    T* op = (T*)a.out + b * a.o_batch + (int64_t)i * a.o_token + h * a.o_head;
+    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+    if (lane == 0) side[wave] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(side[0], side[1]), fmaxf(side[2], side[3]));
+    const float from = top == -__builtin_inff() ? 0.0f : top;
+    float total = 0.0f;
 #pragma unroll
-    for (int d = 0; d < DP / 64; ++d)
-        if (lane + 64 * d < a.dim) op[lane + 64 * d] = from_float<T>(nan ? __builtin_nanf("") : (empty ? 0.0f : acc[d] / total));
+    for (int x = 0; x < MOST_PARTS / 256; ++x) {
+        // a part that saw nothing adds nothing
+        const float f = ws[x] == 0.0f ? 0.0f : __builtin_amdgcn_exp2f((m[x] == -__builtin_inff() ? 0.0f : m[x]) - from);
+        if (ws[x] != 0.0f) total += f * ws[x];
+        const int s = threadIdx.x + 256 * x;
+        if (s < splits) factor[s] = f;
+    }
+    for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o);
+    __syncthreads();
+    if (lane == 0) side[wave] = total;
+    float acc[DP / 64] = {};
+#pragma unroll 4
+    for (int s = wave; s < splits; s += 4) {
+        const float f = factor[s];
+#pragma unroll
+        for (int d = 0; d < DP / 64; ++d) {
+            const float v = part[s * stride + 2 + lane + 64 * d];
+            acc[d] += f == 0.0f ? 0.0f : f * v;
+        }
+    }
+#pragma unroll
+    for (int d = 0; d < DP / 64; ++d) sums[wave][lane + 64 * d] = acc[d];
+    __syncthreads();
+    bool lost;
+    const Sequence seq = sequence_of<true>(a, b, lost);
+    total = (side[0] + side[1]) + (side[2] + side[3]);
+    const int col = threadIdx.x;
+    if (col >= (int)a.dim) return;
+    const float o = (sums[0][col] + sums[1][col]) + (sums[2][col] + sums[3][col]);
+    const bool empty = total == 0.0f || i >= seq.real, nan = i < seq.real && (lost || seq.shift + i >= (int)a.keys);
+    ((T*)a.out)[b * a.o_batch + (int64_t)i * a.o_token + h * a.o_head + col] = from_float<T>(nan ? __builtin_nanf("") : (empty ? 0.0f : o / total));
 }
 
 static bool step_wide(const tvl_attention_args& a) {
@@ -239,11 +266,14 @@ bool attention_step_serves(const tvl_attention_args& a) {
     return rows <= 64;
 }
 
-// parts the keys are cut into: as many as fill the chip (512 workgroups), none shorter than one step of every wave
+// Parts the keys are cut into: enough for one workgroup per compute unit, none shorter than 512 keys; a cache of up to 1024 slots stays whole, its
+// second launch costs more than the parts gain.  Measured (us, us): 32 pairs x 745 of 1024 slots whole 8.3, 4 parts 9.3; 256 pairs x 745 whole 11.9,
+// 2 parts 17.3; 32 pairs x 28000 x 128 in 8 parts 89.6, 16 parts 92.6; one pair x 32000 in 62 parts 20.5, 31 parts 23.8, 125 parts 20.1.
 int attention_step_splits(const tvl_attention_args& a) {
     const int64_t work = a.batch * a.kv_heads * ceil_div(a.queries * (a.heads / a.kv_heads), ROWS);
-    const int64_t want = ceil_div(512, work), most = ceil_div(a.keys, WAVES * STEP);
-    const int64_t n = want < most ? want : most;
+    const int64_t want = ceil_div(256, work), most = a.keys <= 1024 ? 1 : ceil_div(a.keys, 512);
+    int64_t n = want < most ? want : most;
+    n = n < MOST_PARTS ? n : MOST_PARTS;
     return (int)(n < 1 ? 1 : n);
 }
 
@@ -262,7 +292,7 @@ static int launch_step(const tvl_attention_args& a, float* parts, hipStream_t st
     hipLaunchKernelGGL((attention_step_kernel<T, DP, FORM>), dim3((unsigned)(pairs * tiles * splits)), dim3(64 * WAVES), bytes, st, a, tiles, splits, parts);
     TVL_LAUNCH_CHECK();
     if (splits > 1) {
-        hipLaunchKernelGGL((attention_join_kernel<T, DP>), dim3((unsigned)ceil_div(pairs * rows, 4)), dim3(256), 0, st, a, splits, parts);
+        hipLaunchKernelGGL((attention_join_kernel<T, DP>), dim3((unsigned)(pairs * rows)), dim3(256), 0, st, a, splits, parts);
         TVL_LAUNCH_CHECK();
     }
     return TVL_OK;

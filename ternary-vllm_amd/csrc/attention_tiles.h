@@ -210,6 +210,9 @@ __device__ __forceinline__ void both_halves(float v, float& lo, float& hi) {
 // the wave's number in its workgroup, known to be the same for all its lanes
 __device__ __forceinline__ int wave_number() { return __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64); }
 
+// whether the row of result register x is of document `doc` (none if negative); `docs`: the documents of rows 4 g + .. of a tile, staged behind it in LDS
+template <int R> __device__ __forceinline__ bool same_document(const int64_t* docs, int x, int64_t doc) { return (docs[result_row<R>(x, 0)] == doc) & (doc >= 0); }
+
 // maximum / sum over the lanes that hold one column (the groups g)
 template <int R> __device__ __forceinline__ float column_max(float v) {
     float lo, hi;
@@ -278,9 +281,55 @@ __device__ __forceinline__ Sequence sequence_of(const tvl_attention_args& a, int
     return s;
 }
 
-// first and last document of every block of 64 tokens: blocks that cannot meet are skipped, blocks of one document need no test
-struct DocumentSpan { int64_t lo, hi; };
+// smallest and largest document of every block of 64 tokens, without the padding (lo > hi: nothing but padding), and whether there is none:
+// blocks that cannot meet are skipped, blocks of one document need no test
+struct DocumentSpan { int64_t lo, hi, whole; };
 constexpr int SPAN = 64;
+
+// The documents of 64 blocks of tokens against those of a workgroup's own tokens [lo, hi], as two bit masks that stay in scalar registers:
+// blocks that cannot meet them, and blocks that hold the one document they all are: one trip to memory per 4096 tokens.
+struct DocumentWindow {
+    const DocumentSpan* spans;
+    int blocks, window;
+    int64_t lo, hi;
+    bool whole;
+    uint64_t skip, single;
+    __device__ __forceinline__ void start(const DocumentSpan* s, int tokens, int first, int rows) {
+        spans = s;
+        blocks = (tokens + SPAN - 1) / SPAN;
+        window = -1;
+        lo = INT64_MAX;
+        hi = -1;
+        whole = true;
+        for (int i = first / SPAN; i < blocks && i * SPAN < first + rows; ++i) {
+            lo = s[i].lo < lo ? s[i].lo : lo;
+            hi = s[i].hi > hi ? s[i].hi : hi;
+            whole = whole && s[i].whole;
+        }
+    }
+    __device__ __forceinline__ void look(int block, int lane) {
+        if (block / 64 == window) return;
+        window = block / 64;
+        DocumentSpan s{INT64_MAX, -1, 0};
+        if (window * 64 + lane < blocks) s = spans[window * 64 + lane];
+        skip = __ballot(s.hi < lo || s.lo > hi);
+        single = __ballot(s.whole && whole && s.lo == s.hi && lo == hi && s.lo == lo);
+    }
+    // first block from `block` on, below `end`, that is not skipped
+    __device__ __forceinline__ int next(int block, int end, int lane) {
+        while (block < end) {
+            look(block, lane);
+            const uint64_t rest = ~skip >> (block & 63);
+            if (rest != 0) return block + __builtin_ctzll(rest);
+            block = (block / 64 + 1) * 64;
+        }
+        return block;
+    }
+    __device__ __forceinline__ bool one(int block, int lane) {
+        look(block, lane);
+        return (single >> (block & 63)) & 1;
+    }
+};
 
 // Sequence and head of a workgroup.  Workgroups with equal blockIdx % 8 share an L2 (8 XCDs): where the (sequence, key head) pairs divide by 8,
 // each pair's query tiles and heads stay on one of them, so its keys and values are fetched into one L2.  Tiles come last first: with a
