@@ -8,6 +8,9 @@
 namespace tvl {
 
 constexpr int GT = 64;    // rows of a staged tile
+#ifndef XB
+#define XB (DP == 128 && sizeof(T) == 2)
+#endif
 
 // power of two that brings float16 score gradients into the type's range: near the largest output gradient, in steps of 2^8 so that it
 // rarely moves; float32 and bfloat16 need none
@@ -62,6 +65,7 @@ __global__ void __launch_bounds__(256, DP == 64 && sizeof(T) == 2 ? 2 : 1) atten
                                                            int tiles) {
     constexpr bool WIDE = FORM != ODD;
     constexpr int R = 32, QB = 128, CK = CHUNK<R>;
+    constexpr bool BOTH = XB;
     typedef Tile<T, DP> L;
     typedef typename Operand<T>::elem E;
     extern __shared__ __align__(16) char lds[];
@@ -122,6 +126,7 @@ __global__ void __launch_bounds__(256, DP == 64 && sizeof(T) == 2 ? 2 : 1) atten
     Acc<R> acc[DP / R] = {};
 
     auto next = [&](int j) { return docs && j < reach ? docw.next(j / SPAN, (reach + SPAN - 1) / SPAN, lane) * SPAN : j; };
+    const int lane_row = L::template lane_row<R>(lane), lane_col = L::template lane_column<R>(lane);
     Stage<T, DP, GT, 256, WIDE> sk, sv;
     int64_t side = -1;
     auto fetch = [&](int j) {
@@ -148,15 +153,14 @@ __global__ void __launch_bounds__(256, DP == 64 && sizeof(T) == 2 ? 2 : 1) atten
         const char *kt = lds + buf * BUFFER, *vt = kt + TILE;
         const int64_t* kdocs = reinterpret_cast<const int64_t*>(kt + 2 * TILE);
         const bool one_document = !MASKED || !docs || docw.one(j0 / SPAN, lane);
-#pragma unroll 1
-        for (int t = 0; t < GT; t += R) {
+        auto piece = [&](int t) __attribute__((always_inline)) {
             const int jt = j0 + t;
-            if (MASKED && jt >= wreach) break;
+            if (MASKED && jt >= wreach) return;
             Acc<R> s = {}, dp = {};
 #pragma unroll
             for (int c = 0; c < DP / CK; ++c) {
-                s = mma(L::read(kt, t + r, g + (64 / R) * c), qf[c], s);
-                dp = mma(L::read(vt, t + r, g + (64 / R) * c), gf[c], dp);
+                s = mma(L::template read<R>(kt + t * L::ROW, lane_row, 0, c), qf[c], s);
+                dp = mma(L::template read<R>(vt + t * L::ROW, lane_row, 0, c), gf[c], dp);
             }
             Frag<T> df[R / CK];
             if (capped) {
@@ -195,7 +199,7 @@ __global__ void __launch_bounds__(256, DP == 64 && sizeof(T) == 2 ? 2 : 1) atten
 #pragma unroll
                 for (int c = 0; c < R / CK; ++c)
 #pragma unroll
-                    for (int d = 0; d < DP / R; ++d) acc[d] = mma(finite_part<T>(L::template read_across<R>(kt, t + c * CK, d * R, lane)), df[c], acc[d]);
+                    for (int d = 0; d < DP / R; ++d) acc[d] = mma(finite_part<T>(L::template read_across<R>(kt + t * L::ROW, lane_col, c * CK, d)), df[c], acc[d]);
 #pragma unroll 1
                 for (int row = 0; row < R && jt + row < reach; ++row)
                     add_not_finite<T, DP, R>(kt, t + row, jt + row < mine && (one_document || (doc >= 0 && kdocs[t + row] == doc)), true, g, acc);
@@ -203,8 +207,15 @@ __global__ void __launch_bounds__(256, DP == 64 && sizeof(T) == 2 ? 2 : 1) atten
 #pragma unroll
                 for (int c = 0; c < R / CK; ++c)
 #pragma unroll
-                    for (int d = 0; d < DP / R; ++d) acc[d] = mma(L::template read_across<R>(kt, t + c * CK, d * R, lane), df[c], acc[d]);
+                    for (int d = 0; d < DP / R; ++d) acc[d] = mma(L::template read_across<R>(kt + t * L::ROW, lane_col, c * CK, d), df[c], acc[d]);
             }
+        };
+        if constexpr (BOTH && !MASKED) {
+            piece(0);
+            piece(R);
+        } else {
+#pragma unroll 1
+            for (int t = 0; t < GT; t += R) piece(t);
         }
         if (j1 < reach) put(lds + (buf ^ 1) * BUFFER);
         __syncthreads();
@@ -235,6 +246,7 @@ __global__ void __launch_bounds__(256, DP == 64 && sizeof(T) == 2 ? 2 : 1) atten
                                                             const float* __restrict__ maxima, int tiles) {
     constexpr bool WIDE = FORM != ODD;
     constexpr int R = 32, KB = 128, CK = CHUNK<R>;
+    constexpr bool BOTH = XB;
     typedef Tile<T, DP> L;
     typedef typename Operand<T>::elem E;
     extern __shared__ __align__(16) char lds[];
@@ -295,6 +307,7 @@ __global__ void __launch_bounds__(256, DP == 64 && sizeof(T) == 2 ? 2 : 1) atten
         }
         return n;
     };
+    const int lane_row = L::template lane_row<R>(lane), lane_col = L::template lane_column<R>(lane);
     Stage<T, DP, GT, 256, WIDE> sq, sg;
     float side = 0.0f;      // threads 0..63: a log-sum, 64..127: a delta
     int64_t qdoc = -1;      // threads 0..63
@@ -332,17 +345,16 @@ __global__ void __launch_bounds__(256, DP == 64 && sizeof(T) == 2 ? 2 : 1) atten
         const int h = hk * group + n / steps, i0 = begin + (n % steps) * GT;
         const float slope = biased ? a.slopes[h] * LOG2E : 0.0f;
         const bool one_document = !MASKED || !docs || docw.one(i0 / SPAN, lane);
-#pragma unroll 1
-        for (int t = 0; t < GT; t += R) {
+        auto piece = [&](int t) __attribute__((always_inline)) {
             const int it = i0 + t;
             const int ilast = it + R < queries ? it + R - 1 : queries - 1;
-            if (it >= queries || (MASKED && kw >= keys)) break;
-            if (MASKED && seq.limit(ilast) <= kw) continue;                              // none of these queries sees a key of the wave
+            if (MASKED && (it >= queries || kw >= keys)) return;
+            if (MASKED && seq.limit(ilast) <= kw) return;                              // none of these queries sees a key of the wave
             Acc<R> s = {}, dp = {};
 #pragma unroll
             for (int c = 0; c < DP / CK; ++c) {
-                s = mma(L::read(qt, t + r, g + (64 / R) * c), kf[c], s);
-                dp = mma(L::read(gt, t + r, g + (64 / R) * c), vf[c], dp);
+                s = mma(L::template read<R>(qt + t * L::ROW, lane_row, 0, c), kf[c], s);
+                dp = mma(L::template read<R>(gt + t * L::ROW, lane_row, 0, c), vf[c], dp);
             }
             const bool masked = MASKED && (seq.limit(it) < kw + R || !one_document);
             Frag<T> pf[R / CK], df[R / CK];
@@ -391,8 +403,8 @@ __global__ void __launch_bounds__(256, DP == 64 && sizeof(T) == 2 ? 2 : 1) atten
                 for (int c = 0; c < R / CK; ++c)
 #pragma unroll
                     for (int d = 0; d < DP / R; ++d) {
-                        dv[d] = mma(finite_part<T>(L::template read_across<R>(gt, t + c * CK, d * R, lane)), pf[c], dv[d]);
-                        dk[d] = mma(finite_part<T>(L::template read_across<R>(qt, t + c * CK, d * R, lane)), df[c], dk[d]);
+                        dv[d] = mma(finite_part<T>(L::template read_across<R>(gt + t * L::ROW, lane_col, c * CK, d)), pf[c], dv[d]);
+                        dk[d] = mma(finite_part<T>(L::template read_across<R>(qt + t * L::ROW, lane_col, c * CK, d)), df[c], dk[d]);
                     }
 #pragma unroll 1
                 for (int row = 0; row < R && it + row < queries; ++row) {
@@ -405,10 +417,17 @@ __global__ void __launch_bounds__(256, DP == 64 && sizeof(T) == 2 ? 2 : 1) atten
                 for (int c = 0; c < R / CK; ++c)
 #pragma unroll
                     for (int d = 0; d < DP / R; ++d) {
-                        dv[d] = mma(L::template read_across<R>(gt, t + c * CK, d * R, lane), pf[c], dv[d]);
-                        dk[d] = mma(L::template read_across<R>(qt, t + c * CK, d * R, lane), df[c], dk[d]);
+                        dv[d] = mma(L::template read_across<R>(gt + t * L::ROW, lane_col, c * CK, d), pf[c], dv[d]);
+                        dk[d] = mma(L::template read_across<R>(qt + t * L::ROW, lane_col, c * CK, d), df[c], dk[d]);
                     }
             }
+        };
+        if constexpr (BOTH && !MASKED) {
+            piece(0);
+            piece(R);
+        } else {
+#pragma unroll 1
+            for (int t = 0; t < GT; t += R) piece(t);
         }
         if (n1 < total) put(lds + (buf ^ 1) * STEP);
         __syncthreads();

@@ -11,7 +11,7 @@ namespace tvl {
 // O^T += V^T P^T.  m is kept until a score exceeds it by 8 (in powers of two): the weights stay below 2^8, exact in float32 sums, and the
 // accumulator is almost never rescaled.
 template <typename T, int DP, bool CACHED, Form FORM>
-__global__ void __launch_bounds__(256, DP == 64 && sizeof(T) == 2 ? 2 : 1) attention_forward_kernel(tvl_attention_args a, const DocumentSpan* __restrict__ spans, int tiles) {
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attention_forward_kernel(tvl_attention_args a, const DocumentSpan* __restrict__ spans, int tiles) {
     constexpr bool WIDE = FORM != ODD;
     constexpr int R = 32, KT = 64, QB = 128, CK = CHUNK<R>;
     typedef Tile<T, DP> L;
@@ -66,39 +66,49 @@ __global__ void __launch_bounds__(256, DP == 64 && sizeof(T) == 2 ? 2 : 1) atten
 
     // tiles whose documents no query of the block has are skipped
     auto next = [&](int j) { return docs && j < reach ? docw.next(j / SPAN, (reach + SPAN - 1) / SPAN, lane) * SPAN : j; };
-    Stage<T, DP, KT, 256, WIDE> sk, sv;
+    // one set of staging registers: the next keys are on their way while the scores are formed, the next values during the rest
+    Stage<T, DP, KT, 256, WIDE> stage;
     int64_t side = -1;
-    auto fetch = [&](int j) {
-        sk.load(kp, a.k_token, j, seq.end, dim);
-        sv.load(vp, a.v_token, j, seq.end, dim);
+    auto fetch_keys = [&](int j) {
+        stage.load(kp, a.k_token, j, seq.end, dim);
         if (docs && threadIdx.x < KT) side = j + (int)threadIdx.x < seq.end ? docs[j + threadIdx.x] : -1;
     };
-    auto put = [&](char* to) {
-        sk.store(to);
-        sv.store(to + TILE);
+    auto put_keys = [&](char* to) {
+        stage.store(to);
         if (docs && threadIdx.x < KT) reinterpret_cast<int64_t*>(to + 2 * TILE)[threadIdx.x] = side;
     };
+    const int lane_row = L::template lane_row<R>(lane), lane_col = L::template lane_column<R>(lane);
     int j0 = next(0), buf = 0;
     if (j0 < reach) {
-        fetch(j0);
-        put(lds);
+        fetch_keys(j0);
+        put_keys(lds);
+        stage.load(vp, a.v_token, j0, seq.end, dim);
+        stage.store(lds + TILE);
     }
     __syncthreads();
     // MASKED: some query of the block does not see some key of the tile
     auto step = [&](auto masked) __attribute__((always_inline)) {
         constexpr bool MASKED = decltype(masked)::value;
         const int j1 = next(j0 + KT);
-        if (j1 < reach) fetch(j1);
+        if (j1 < reach) fetch_keys(j1);
+        char* ahead = lds + (buf ^ 1) * BUFFER;
         const char *kt = lds + buf * BUFFER, *vt = kt + TILE;
         const int64_t* kdocs = reinterpret_cast<const int64_t*>(kt + 2 * TILE);
-        if (!MASKED || j0 < wreach) {
-            Acc<R> s[KT / R];
+        const bool busy = !MASKED || j0 < wreach;
+        Acc<R> s[KT / R];
+        if (busy) {
 #pragma unroll
             for (int t = 0; t < KT / R; ++t) {
                 s[t] = Acc<R>{};
 #pragma unroll
-                for (int c = 0; c < DP / CK; ++c) s[t] = mma(L::read(kt, t * R + r, g + (64 / R) * c), qf[c], s[t]);
+                for (int c = 0; c < DP / CK; ++c) s[t] = mma(L::template read<R>(kt, lane_row, t * R, c), qf[c], s[t]);
             }
+        }
+        if (j1 < reach) {
+            put_keys(ahead);
+            stage.load(vp, a.v_token, j1, seq.end, dim);
+        }
+        if (busy) {
             // scores: units of `unit` powers of two
             const bool one_document = !MASKED || !docs || docw.one(j0 / SPAN, lane);
             if (capped) {
@@ -162,7 +172,7 @@ __global__ void __launch_bounds__(256, DP == 64 && sizeof(T) == 2 ? 2 : 1) atten
 #pragma unroll
                 for (int c = 0; c < KT / CK; ++c)
 #pragma unroll
-                    for (int d = 0; d < DP / R; ++d) acc[d] = mma(finite_part<T>(L::template read_across<R>(vt, c * CK, d * R, lane)), pf[c], acc[d]);
+                    for (int d = 0; d < DP / R; ++d) acc[d] = mma(finite_part<T>(L::template read_across<R>(vt, lane_col, c * CK, d)), pf[c], acc[d]);
 #pragma unroll 1
                 for (int row = 0; row < KT && j0 + row < reach; ++row)
                     add_not_finite<T, DP, R>(vt, row, j0 + row < mine && (one_document || (doc >= 0 && kdocs[row] == doc)), false, g, acc);
@@ -170,10 +180,10 @@ __global__ void __launch_bounds__(256, DP == 64 && sizeof(T) == 2 ? 2 : 1) atten
 #pragma unroll
                 for (int c = 0; c < KT / CK; ++c)
 #pragma unroll
-                    for (int d = 0; d < DP / R; ++d) acc[d] = mma(L::template read_across<R>(vt, c * CK, d * R, lane), pf[c], acc[d]);
+                    for (int d = 0; d < DP / R; ++d) acc[d] = mma(L::template read_across<R>(vt, lane_col, c * CK, d), pf[c], acc[d]);
             }
         }
-        if (j1 < reach) put(lds + (buf ^ 1) * BUFFER);
+        if (j1 < reach) stage.store(ahead + TILE);
         __syncthreads();
         buf ^= 1;
         j0 = j1;

@@ -80,6 +80,7 @@ __global__ void __launch_bounds__(64 * WAVES) attention_step_kernel(tvl_attentio
             if (j < hi) vv[x] = load_unit<T, WIDE>(vp + (int64_t)j * a.v_token, u % L::UNITS, dim);
         }
     };
+    const int lane_col = L::template lane_column<R>(lane);
     Acc<R> acc[DP / R] = {};
     float m = -__builtin_inff(), base = 0.0f, sum = 0.0f;
     int j0 = lo + wave * STEP;
@@ -150,12 +151,12 @@ __global__ void __launch_bounds__(64 * WAVES) attention_step_kernel(tvl_attentio
         // tokens of a chunk see different keys: an infinity or NaN in a later token's value must not reach an earlier token
         if (here + STEP > all && all < reach && holds_not_finite<T, DP, STEP>(vt, lane)) {
 #pragma unroll
-            for (int d = 0; d < DP / R; ++d) acc[d] = mma(finite_part<T>(L::template read_across<R>(vt, 0, d * R, lane)), pf, acc[d]);
+            for (int d = 0; d < DP / R; ++d) acc[d] = mma(finite_part<T>(L::template read_across<R>(vt, lane_col, 0, d)), pf, acc[d]);
 #pragma unroll 1
             for (int x = 0; x < STEP && here + x < hi; ++x) add_not_finite<T, DP, R>(vt, x, here + x < mine, false, g, acc);
         } else {
 #pragma unroll
-            for (int d = 0; d < DP / R; ++d) acc[d] = mma(L::template read_across<R>(vt, 0, d * R, lane), pf, acc[d]);
+            for (int d = 0; d < DP / R; ++d) acc[d] = mma(L::template read_across<R>(vt, lane_col, 0, d), pf, acc[d]);
         }
         __builtin_amdgcn_wave_barrier();
     }

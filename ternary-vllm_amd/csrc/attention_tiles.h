@@ -64,36 +64,45 @@ template <typename T> __device__ __forceinline__ Frag<T> finite_part(Frag<T> a) 
 }
 
 // ---- tiles in LDS ------------------------------------------------------------------------------
-// Rows of DP elements in 16-byte units.  A unit lies at its place with the low bits exchanged by the row's, so that the 8 rows a
-// b128 read takes at a time, and the 4 rows x 2 units of a transposing read, fall on different banks (rows of 128 bytes and
-// their multiples: 3 bits; rows of 64 and 192 bytes: 2 bits).
+// Rows of DP elements in 16-byte units.  A unit lies at its place with the low three bits exchanged by the row's, so that the 8 rows a
+// b128 read takes at a time, and the 4 rows x 2 units of a transposing read, fall on different banks.  A row's exchange depends on
+// its place among 8 rows only: a lane works out its offset once, and what the compiler knows (chunk, tile, half) is an exclusive-or or
+// an immediate.
 template <typename T, int DP> struct Tile {
     static constexpr int UNITS = DP * (int)sizeof(T) / 16;
     static constexpr int PER = 16 / (int)sizeof(T);          // elements of a unit
     static constexpr int ROW = DP * (int)sizeof(T);
-    __device__ static __forceinline__ int swap_bits(int row) { return UNITS % 8 == 0 ? ((row & 3) << 1) | ((row >> 2) & 1) : (row & 2) | ((row >> 2) & 1); }
+    static_assert(UNITS % 8 == 0, "rows are multiples of 128 bytes");
+    __device__ static __forceinline__ int swap_bits(int row) { return ((row & 3) << 1) | ((row >> 2) & 1); }
     __device__ static __forceinline__ int at(int row, int unit) { return row * ROW + ((unit ^ swap_bits(row)) << 4); }
+    // a lane's offset moved by `unit` units (bits the lane's own unit does not use)
+    __device__ static __forceinline__ int moved(int lane_at, int unit) { return (lane_at ^ ((unit & 7) << 4)) + ((unit & ~7) << 4); }
 
-    // fragment of row `row`, elements 8 c8 .. 8 c8 + 7
-    __device__ static __forceinline__ Frag<T> read(const char* tile, int row, int c8) {
+    // fragments of row `row0 + r`, elements 8 (g + (64 / R) c) ..: a lane's offset, and the read
+    template <int R> __device__ static __forceinline__ int lane_row(int lane) { return at(lane % R, (lane / R) * (8 / PER)); }
+    template <int R> __device__ static __forceinline__ Frag<T> read(const char* tile, int lane_at, int row0, int c) {
         if constexpr (sizeof(T) == 2) {
-            return __builtin_bit_cast(Frag<T>, *reinterpret_cast<const u32x4*>(tile + at(row, c8)));
+            return __builtin_bit_cast(Frag<T>, *reinterpret_cast<const u32x4*>(tile + moved(lane_at, 64 / R * c) + row0 * ROW));
         } else {
-            const f32x4 lo = *reinterpret_cast<const f32x4*>(tile + at(row, 2 * c8)), hi = *reinterpret_cast<const f32x4*>(tile + at(row, 2 * c8 + 1));
+            const f32x4 lo = *reinterpret_cast<const f32x4*>(tile + moved(lane_at, 128 / R * c) + row0 * ROW);
+            const f32x4 hi = *reinterpret_cast<const f32x4*>(tile + moved(lane_at, 128 / R * c + 1) + row0 * ROW);
             return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
         }
     }
 
-    // fragment down the rows: element 4 u + y is row row0 + (K / 2) u + 4 g + y, column col0 + r  (K = CHUNK<R>, col0 a multiple of R)
-    template <int R> __device__ static __forceinline__ Frag<T> read_across(const char* tile, int row0, int col0, int lane) {
-        const int r = lane % R, g = lane / R;
+    // fragments down the rows: element 4 u + y is row row0 + (K / 2) u + 4 g + y, column R d + r  (K = CHUNK<R>, row0 a multiple of 16)
+    template <int R> __device__ static __forceinline__ int lane_column(int lane) {
+        const int r = lane % R, g = lane / R, i = lane & 15;
+        // ds_read_b64_tr_b16: 16 lanes point at 4 rows x 4 pieces of 4 elements and get the 16 columns
+        if constexpr (sizeof(T) == 2) return at(4 * g + (i >> 2), ((r & ~15) >> 3) + ((i & 3) >> 1)) + 8 * (i & 1);
+        return at(4 * g, r >> 2) + 4 * (r & 3);
+    }
+    template <int R> __device__ static __forceinline__ Frag<T> read_across(const char* tile, int lane_at, int row0, int d) {
         if constexpr (sizeof(T) == 2) {
-            // ds_read_b64_tr_b16: 16 lanes point at 4 rows x 4 pieces of 4 elements and get the 16 columns
-            const int i = lane & 15, col = col0 + (r & ~15) + 4 * (i & 3), row = row0 + 4 * g + (i >> 2);
             i16x4 v[2];
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                const char* p = tile + at(row + CHUNK<R> / 2 * u, col >> 3) + 8 * (i & 1);
+                const char* p = tile + moved(lane_at, d * R / PER) + (row0 + CHUNK<R> / 2 * u) * ROW;
                 v[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(p));
             }
             return __builtin_bit_cast(Frag<T>, __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7));
@@ -102,10 +111,8 @@ template <typename T, int DP> struct Tile {
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
-                for (int y = 0; y < 4; ++y) {
-                    const int row = row0 + CHUNK<R> / 2 * u + 4 * g + y;
-                    f[4 * u + y] = *reinterpret_cast<const float*>(tile + at(row, (col0 + r) >> 2) + 4 * (r & 3));
-                }
+                for (int y = 0; y < 4; ++y)
+                    f[4 * u + y] = *reinterpret_cast<const float*>(tile + moved(lane_at, (d * R / PER) ^ (y << 1)) + (row0 + CHUNK<R> / 2 * u + y) * ROW);
             return f;
         }
     }
@@ -175,27 +182,41 @@ __device__ __forceinline__ Frag<T> load_frag(const T* row, int c8, int dim) {
     }
 }
 
-// A tile's way from global memory to LDS through the registers of THREADS threads
+// A tile's way from global memory to LDS through the registers of THREADS threads.  Offsets inside a tile are 32-bit bytes (wide_rows() sees to it for
+// the wide forms), tiles lie at 64-bit places.
 template <typename T, int DP, int ROWS, int THREADS, bool WIDE> struct Stage {
     typedef Tile<T, DP> L;
-    static constexpr int N = ROWS * L::UNITS / THREADS;
-    static_assert(ROWS * L::UNITS % THREADS == 0, "every thread moves the same number of units");
+    static constexpr int N = ROWS * L::UNITS / THREADS, APART = THREADS / L::UNITS;
+    static_assert(ROWS * L::UNITS % THREADS == 0 && THREADS % L::UNITS == 0 && APART % 8 == 0, "every thread moves the same unit of rows APART apart");
     u32x4 v[N];
-    // rows row0 .. row0 + ROWS - 1 of a matrix; rows from `end` on are zero and not read
+    // rows row0 .. row0 + ROWS - 1 of a matrix; rows from `end` on are zero and not read.  One 32-bit offset per lane, the rest is in scalar
+    // registers: per-row offsets get spilled, and a reload waits for the loads in front of it
     __device__ __forceinline__ void load(const T* base, int64_t stride, int row0, int end, int dim) {
+        const int row = threadIdx.x / L::UNITS, unit = threadIdx.x % L::UNITS;
+        const T* tile = base + (int64_t)row0 * stride;
 #pragma unroll
-        for (int x = 0; x < N; ++x) {
-            const int u = threadIdx.x + x * THREADS, row = u / L::UNITS, unit = u % L::UNITS;
-            v[x] = u32x4{0, 0, 0, 0};
-            if (row0 + row < end) v[x] = load_unit<T, WIDE>(base + (int64_t)(row0 + row) * stride, unit, dim);
+        for (int x = 0; x < N; ++x) v[x] = u32x4{0, 0, 0, 0};
+        if constexpr (WIDE) {
+            const uint32_t at = (uint32_t)row * (uint32_t)(stride * (int64_t)sizeof(T)) + 16u * unit;
+            if (unit * L::PER >= dim) return;
+            if (row0 + ROWS <= end) {
+#pragma unroll
+                for (int x = 0; x < N; ++x) v[x] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(tile + (int64_t)(x * APART) * stride) + at);
+            } else {
+#pragma unroll
+                for (int x = 0; x < N; ++x)
+                    if (row0 + x * APART + row < end) v[x] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(tile + (int64_t)(x * APART) * stride) + at);
+            }
+        } else {
+#pragma unroll
+            for (int x = 0; x < N; ++x)
+                if (row0 + row + x * APART < end) v[x] = load_unit<T, false>(tile + (int64_t)(row + x * APART) * stride, unit, dim);
         }
     }
     __device__ __forceinline__ void store(char* tile) const {
+        const int at = L::at(threadIdx.x / L::UNITS, threadIdx.x % L::UNITS);
 #pragma unroll
-        for (int x = 0; x < N; ++x) {
-            const int u = threadIdx.x + x * THREADS;
-            *reinterpret_cast<u32x4*>(tile + L::at(u / L::UNITS, u % L::UNITS)) = v[x];
-        }
+        for (int x = 0; x < N; ++x) *reinterpret_cast<u32x4*>(tile + at + x * APART * L::ROW) = v[x];
     }
 };
 
@@ -333,7 +354,7 @@ struct DocumentWindow {
 
 // Sequence and head of a workgroup.  Workgroups with equal blockIdx % 8 share an L2 (8 XCDs): where the (sequence, key head) pairs divide by 8,
 // each pair's query tiles and heads stay on one of them, so its keys and values are fetched into one L2.  Tiles come last first: with a
-// causal mask those are the long ones.
+// causal mask those are the long ones; few pairs take turns, so that all their long tiles start first.
 struct Place { int pair, head, tile; };
 __device__ __forceinline__ Place place_of(uint32_t id, int pairs, int group, int tiles) {
     const uint32_t per = (uint32_t)group * tiles;
@@ -343,8 +364,8 @@ __device__ __forceinline__ Place place_of(uint32_t id, int pairs, int group, int
         pair = (local / per) * 8 + (id & 7);
         rest = local % per;
     } else {
-        pair = id / per;
-        rest = id % per;
+        pair = id % (uint32_t)pairs;
+        rest = id / (uint32_t)pairs;
     }
     return Place{(int)pair, (int)(rest % group), tiles - 1 - (int)(rest / group)};
 }
@@ -354,9 +375,9 @@ enum Form { PLAIN, GENERAL, ODD };
 
 // host side
 static inline bool featureless(const tvl_attention_args& a) { return a.softcap == 0.0f && a.slopes == nullptr && a.documents == nullptr && a.scale != 0.0f; }
-static inline bool wide_rows(const void* p, int64_t dim, int64_t s0, int64_t s1, int64_t s2, size_t z) {
+static inline bool wide_rows(const void* p, int64_t dim, int64_t batch, int64_t token, int64_t head, size_t z) {
     const int64_t per = (int64_t)(16 / z);
-    return aligned(p, 16) && dim % per == 0 && s0 % per == 0 && s1 % per == 0 && s2 % per == 0;
+    return aligned(p, 16) && dim % per == 0 && batch % per == 0 && token % per == 0 && head % per == 0 && token * (int64_t)z < (int64_t)1 << 25;
 }
 
 int launch_attention_forward(const tvl_attention_args& a, bool cached, const DocumentSpan* spans, hipStream_t st);
