@@ -56,6 +56,12 @@ static size_t maxima_bytes(const tvl_attention_args& a) {
     return any_rows(a) && a.dtype == TVL_F16 ? round256((size_t)a.batch * a.heads * (size_t)ceil_div(a.queries, 64) * 4) : 0;
 }
 
+static size_t slab_bytes(const tvl_attention_args& a) {
+    if (!any_rows(a) || a.keys <= 0 || a.kv_heads <= 0) return 0;
+    const int parts = attention_backward_parts(a);
+    return parts > 1 ? (size_t)parts * 2 * a.batch * a.keys * a.kv_heads * a.dim * 4 : 0;
+}
+
 static int check_workspace(const char* who, size_t need, const void* workspace, size_t bytes) {
     TVL_REQUIRE(need == 0 || (workspace && bytes >= need && aligned(workspace, 256)), "%s: needs %zu bytes of 256-byte aligned workspace", who, need);
     return TVL_OK;
@@ -80,7 +86,9 @@ int tvl_attention(const tvl_attention_args* a, void* workspace, size_t workspace
     return launch_attention_forward(*a, false, spans, st);
 }
 
-size_t tvl_attention_backward_workspace_bytes(const tvl_attention_args* a) { return a ? span_bytes(*a) + delta_bytes(*a) + maxima_bytes(*a) : 0; }
+size_t tvl_attention_backward_workspace_bytes(const tvl_attention_args* a) {
+    return a ? span_bytes(*a) + delta_bytes(*a) + maxima_bytes(*a) + slab_bytes(*a) : 0;
+}
 
 int tvl_attention_backward(const tvl_attention_args* a, const tvl_attention_grads* g, void* workspace, size_t workspace_bytes, void* stream) {
     if (const int rc = check(a, "attention_backward", false); rc != TVL_OK) return rc;
@@ -96,9 +104,10 @@ int tvl_attention_backward(const tvl_attention_args* a, const tvl_attention_grad
     DocumentSpan* spans = a->documents ? reinterpret_cast<DocumentSpan*>(at) : nullptr;
     float* delta = reinterpret_cast<float*>(at + span_bytes(*a));
     float* maxima = maxima_bytes(*a) ? reinterpret_cast<float*>(at + span_bytes(*a) + delta_bytes(*a)) : nullptr;
+    float* slabs = reinterpret_cast<float*>(at + span_bytes(*a) + delta_bytes(*a) + maxima_bytes(*a));
     if (spans)
         if (const int rc = launch_document_spans(*a, spans, st); rc != TVL_OK) return rc;
-    return launch_attention_backward(*a, *g, spans, delta, maxima, st);
+    return launch_attention_backward(*a, *g, spans, delta, maxima, slabs, st);
 }
 
 size_t tvl_cached_attention_workspace_bytes(const tvl_attention_args* a) {

@@ -8,9 +8,19 @@
 namespace tvl {
 
 constexpr int GT = 64;    // rows of a staged tile
-#ifndef XB
-#define XB (DP == 128 && sizeof(T) == 2)
+constexpr int PIECE = 32; // of them at a time
+// N values of a piece that a lane holds: row of value x (of lane group 0)
+template <int R> constexpr int VALUES = PIECE * R / 64;
+template <int R> __device__ __forceinline__ constexpr int piece_row(int x) { return x / REGS<R> * R + result_row<R>(x % REGS<R>, 0); }
+
+// Shape of a gradient kernel: W waves of R queries or keys each, 128 in all; waves per SIMD its registers are limited to.
+template <typename T, int DP, bool QUERIES> struct Shape {
+#ifndef XR
+#define XR (DP == 64 && sizeof(T) == 2 ? 32 : 16)
+#define XO 2
 #endif
+    static constexpr int R = XR, W = 128 / R, OCCUPANCY = XO;
+};
 
 // power of two that brings float16 score gradients into the type's range: near the largest output gradient, in steps of 2^8 so that it
 // rarely moves; float32 and bfloat16 need none
@@ -61,11 +71,10 @@ __global__ void __launch_bounds__(256) attention_delta_kernel(tvl_attention_args
 
 // dq.  4 waves x 32 queries; per 32 keys: S^T = K Q^T, dP^T = V dO^T, dS^T = P (dP - delta) bend (a lane holds one query), dQ^T += K^T dS^T.
 template <typename T, int DP, Form FORM>
-__global__ void __launch_bounds__(256, DP == 64 && sizeof(T) == 2 ? 2 : 1) attention_dq_kernel(tvl_attention_args a, tvl_attention_grads gr, const DocumentSpan* __restrict__ spans, const float* __restrict__ delta,
+__global__ void __launch_bounds__((64 * Shape<T, DP, true>::W), (Shape<T, DP, true>::OCCUPANCY)) attention_dq_kernel(tvl_attention_args a, tvl_attention_grads gr, const DocumentSpan* __restrict__ spans, const float* __restrict__ delta,
                                                            int tiles) {
     constexpr bool WIDE = FORM != ODD;
-    constexpr int R = 32, QB = 128, CK = CHUNK<R>;
-    constexpr bool BOTH = XB;
+    constexpr int R = Shape<T, DP, true>::R, THREADS = 64 * Shape<T, DP, true>::W, QB = 128, CK = CHUNK<R>, N = VALUES<R>;
     typedef Tile<T, DP> L;
     typedef typename Operand<T>::elem E;
     extern __shared__ __align__(16) char lds[];
@@ -127,97 +136,104 @@ __global__ void __launch_bounds__(256, DP == 64 && sizeof(T) == 2 ? 2 : 1) atten
 
     auto next = [&](int j) { return docs && j < reach ? docw.next(j / SPAN, (reach + SPAN - 1) / SPAN, lane) * SPAN : j; };
     const int lane_row = L::template lane_row<R>(lane), lane_col = L::template lane_column<R>(lane);
-    Stage<T, DP, GT, 256, WIDE> sk, sv;
+    // one set of staging registers: the next keys are on their way during the first half of a tile, the next values during the second
+    Stage<T, DP, GT, THREADS, WIDE> stage;
     int64_t side = -1;
-    auto fetch = [&](int j) {
-        sk.load(kp, a.k_token, j, seq.end, dim);
-        sv.load(vp, a.v_token, j, seq.end, dim);
+    auto fetch_keys = [&](int j) {
+        stage.load(kp, a.k_token, j, seq.end, dim);
         if (docs && threadIdx.x < GT) side = j + (int)threadIdx.x < seq.end ? docs[j + threadIdx.x] : -1;
     };
-    auto put = [&](char* to) {
-        sk.store(to);
-        sv.store(to + TILE);
+    auto put_keys = [&](char* to) {
+        stage.store(to);
         if (docs && threadIdx.x < GT) reinterpret_cast<int64_t*>(to + 2 * TILE)[threadIdx.x] = side;
     };
     int j0 = next(0), buf = 0;
     if (j0 < reach) {
-        fetch(j0);
-        put(lds);
+        fetch_keys(j0);
+        put_keys(lds);
+        stage.load(vp, a.v_token, j0, seq.end, dim);
+        stage.store(lds + TILE);
     }
     __syncthreads();
     // MASKED: some query of the block does not see some key of the tile
     auto step = [&](auto masked) __attribute__((always_inline)) {
         constexpr bool MASKED = decltype(masked)::value;
         const int j1 = next(j0 + GT);
-        if (j1 < reach) fetch(j1);
+        char* ahead = lds + (buf ^ 1) * BUFFER;
+        if (j1 < reach) fetch_keys(j1);
         const char *kt = lds + buf * BUFFER, *vt = kt + TILE;
         const int64_t* kdocs = reinterpret_cast<const int64_t*>(kt + 2 * TILE);
         const bool one_document = !MASKED || !docs || docw.one(j0 / SPAN, lane);
         auto piece = [&](int t) __attribute__((always_inline)) {
             const int jt = j0 + t;
             if (MASKED && jt >= wreach) return;
-            Acc<R> s = {}, dp = {};
+            float s[N], dp[N];
 #pragma unroll
-            for (int c = 0; c < DP / CK; ++c) {
-                s = mma(L::template read<R>(kt + t * L::ROW, lane_row, 0, c), qf[c], s);
-                dp = mma(L::template read<R>(vt + t * L::ROW, lane_row, 0, c), gf[c], dp);
+            for (int n = 0; n < PIECE / R; ++n) {
+                Acc<R> u = {}, w = {};
+#pragma unroll
+                for (int c = 0; c < DP / CK; ++c) {
+                    u = mma(L::template read<R>(kt + t * L::ROW, lane_row, n * R, c), qf[c], u);
+                    w = mma(L::template read<R>(vt + t * L::ROW, lane_row, n * R, c), gf[c], w);
+                }
+#pragma unroll
+                for (int x = 0; x < REGS<R>; ++x) { s[n * REGS<R> + x] = u[x]; dp[n * REGS<R> + x] = w[x]; }
             }
-            Frag<T> df[R / CK];
+            Frag<T> df[PIECE / CK];
             if (capped) {
 #pragma unroll
-                for (int x = 0; x < REGS<R>; ++x) {
+                for (int x = 0; x < N; ++x) {
                     const float th = cap_tanh<T>(s[x] * to_cap);
                     s[x] = from_cap * th;
-                    dp[x] = __builtin_fmaf(dp[x], fit, -dl) * (1.0f - th * th);
+                    dp[x] = product(__builtin_fmaf(dp[x], fit, -dl), __builtin_fmaf(-th, th, 1.0f));
                 }
             } else {
 #pragma unroll
-                for (int x = 0; x < REGS<R>; ++x) dp[x] = __builtin_fmaf(dp[x], fit, -dl);
+                for (int x = 0; x < N; ++x) dp[x] = __builtin_fmaf(dp[x], fit, -dl);
             }
             if (biased) {
                 const int here = i + seq.shift - jt - 4 * g;
 #pragma unroll
-                for (int x = 0; x < REGS<R>; ++x) s[x] = __builtin_fmaf(-slope, fabsf((float)(here - result_row<R>(x, 0))), s[x] * pre);
+                for (int x = 0; x < N; ++x) s[x] = __builtin_fmaf(-slope, fabsf((float)(here - piece_row<R>(x))), s[x] * pre);
             }
 #pragma unroll
-            for (int x = 0; x < REGS<R>; ++x) dp[x] *= __builtin_amdgcn_exp2f(__builtin_fmaf(s[x], unit, -lse));
-            if (MASKED && (jt + R > wall || !one_document)) {
+            for (int x = 0; x < N; ++x) dp[x] = product(dp[x], __builtin_amdgcn_exp2f(__builtin_fmaf(s[x], unit, -lse)));
+            if (MASKED && (jt + PIECE > wall || !one_document)) {
                 const int left = mine - jt - 4 * g;
 #pragma unroll
-                for (int x = 0; x < REGS<R>; ++x)
-                    if (result_row<R>(x, 0) >= left) dp[x] = 0.0f;
+                for (int x = 0; x < N; ++x)
+                    if (piece_row<R>(x) >= left) dp[x] = 0.0f;
                 if (!one_document) {
 #pragma unroll
-                    for (int x = 0; x < REGS<R>; ++x)
-                        if (!same_document<R>(kdocs + t + 4 * g, x, doc)) dp[x] = 0.0f;
+                    for (int x = 0; x < N; ++x)
+                        if (!same_document(kdocs + t + 4 * g + piece_row<R>(x), doc)) dp[x] = 0.0f;
                 }
             }
             // score gradients are rounded to the operands' type for the last product; its sum is float32
 #pragma unroll
-            for (int x = 0; x < REGS<R>; ++x) df[x / 8][x % 8] = (E)dp[x];
-            if (MASKED && (!one_document || (jt + R > wall && wall < wreach)) && holds_not_finite<T, DP, R>(kt + t * L::ROW, lane)) {
+            for (int x = 0; x < N; ++x) df[x / 8][x % 8] = (E)dp[x];
+            if (MASKED && (!one_document || (jt + PIECE > wall && wall < wreach)) && holds_not_finite<T, DP, PIECE>(kt + t * L::ROW, lane)) {
 #pragma unroll
-                for (int c = 0; c < R / CK; ++c)
+                for (int c = 0; c < PIECE / CK; ++c)
 #pragma unroll
                     for (int d = 0; d < DP / R; ++d) acc[d] = mma(finite_part<T>(L::template read_across<R>(kt + t * L::ROW, lane_col, c * CK, d)), df[c], acc[d]);
 #pragma unroll 1
-                for (int row = 0; row < R && jt + row < reach; ++row)
+                for (int row = 0; row < PIECE && jt + row < reach; ++row)
                     add_not_finite<T, DP, R>(kt, t + row, jt + row < mine && (one_document || (doc >= 0 && kdocs[t + row] == doc)), true, g, acc);
             } else {
 #pragma unroll
-                for (int c = 0; c < R / CK; ++c)
+                for (int c = 0; c < PIECE / CK; ++c)
 #pragma unroll
                     for (int d = 0; d < DP / R; ++d) acc[d] = mma(L::template read_across<R>(kt + t * L::ROW, lane_col, c * CK, d), df[c], acc[d]);
             }
         };
-        if constexpr (BOTH && !MASKED) {
-            piece(0);
-            piece(R);
-        } else {
-#pragma unroll 1
-            for (int t = 0; t < GT; t += R) piece(t);
+        piece(0);
+        if (j1 < reach) {
+            put_keys(ahead);
+            stage.load(vp, a.v_token, j1, seq.end, dim);
         }
-        if (j1 < reach) put(lds + (buf ^ 1) * BUFFER);
+        piece(PIECE);
+        if (j1 < reach) stage.store(ahead + TILE);
         __syncthreads();
         buf ^= 1;
         j0 = j1;
@@ -235,25 +251,26 @@ __global__ void __launch_bounds__(256, DP == 64 && sizeof(T) == 2 ? 2 : 1) atten
 #pragma unroll
         for (int x = 0; x < REGS<R>; ++x) {
             const int col = d * R + result_row<R>(x, g);
-            if (col < dim) op[col] = from_float<T>(acc[d][x] * back);
+            if (col < dim) op[col] = from_float<T>(product(acc[d][x], back));
         }
 }
 
 // dk, dv.  4 waves x 32 keys; over the heads that share them and tiles of 64 queries: S = Q K^T, dP = dO V^T (a lane holds one key, K and V stay in
 // registers), dV^T += dO^T P, dK^T += Q^T dS.
 template <typename T, int DP, Form FORM>
-__global__ void __launch_bounds__(256, DP == 64 && sizeof(T) == 2 ? 2 : 1) attention_dkv_kernel(tvl_attention_args a, tvl_attention_grads gr, const DocumentSpan* __restrict__ spans, const float* __restrict__ delta,
-                                                            const float* __restrict__ maxima, int tiles) {
+__global__ void __launch_bounds__((64 * Shape<T, DP, false>::W), (Shape<T, DP, false>::OCCUPANCY)) attention_dkv_kernel(tvl_attention_args a, tvl_attention_grads gr, const DocumentSpan* __restrict__ spans, const float* __restrict__ delta,
+                                                            const float* __restrict__ maxima, int tiles, int parts, float* __restrict__ slabs) {
     constexpr bool WIDE = FORM != ODD;
-    constexpr int R = 32, KB = 128, CK = CHUNK<R>;
-    constexpr bool BOTH = XB;
+    constexpr int R = Shape<T, DP, false>::R, THREADS = 64 * Shape<T, DP, false>::W, KB = 128, CK = CHUNK<R>, N = VALUES<R>;
     typedef Tile<T, DP> L;
     typedef typename Operand<T>::elem E;
     extern __shared__ __align__(16) char lds[];
     constexpr int TILE = GT * L::ROW, STEP = 2 * TILE + 2 * GT * 4 + (FORM == PLAIN ? 0 : GT * 8);     // q, grad_out, log-sums, deltas, documents
 
     const int group = (int)(a.heads / a.kv_heads), pairs = (int)(a.batch * a.kv_heads);
-    const Place at = place_of(blockIdx.x, pairs, 1, tiles);
+    // `parts` workgroups share the heads of a group
+    const Place at = place_of(blockIdx.x, pairs, parts, tiles);
+    const int share = group / parts, head0 = at.head * share;
     const int b = at.pair / (int)a.kv_heads, hk = at.pair % (int)a.kv_heads;
     const int wave = wave_number(), lane = threadIdx.x % 64, r = lane % R, g = lane / R;
     const int k0 = (tiles - 1 - at.tile) * KB, kw = k0 + wave * R, j = kw + r;    // with a causal mask the first keys have the most queries
@@ -280,8 +297,8 @@ __global__ void __launch_bounds__(256, DP == 64 && sizeof(T) == 2 ? 2 : 1) atten
     // float16: one power of two for all that this workgroup adds up
     int e = 0;
     if constexpr (__is_same(T, f16)) {
-        const int n = group * ((queries + GT - 1) / GT);
-        const float* mp = maxima + ((int64_t)b * a.heads + hk * group) * ((queries + GT - 1) / GT);
+        const int n = share * ((queries + GT - 1) / GT);
+        const float* mp = maxima + ((int64_t)b * a.heads + hk * group + head0) * ((queries + GT - 1) / GT);
         float top = 0.0f;
         for (int x = lane; x < n; x += 64) top = fmaxf(top, mp[x]);
         for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
@@ -296,7 +313,7 @@ __global__ void __launch_bounds__(256, DP == 64 && sizeof(T) == 2 ? 2 : 1) atten
     // query i sees key j from i = j - shift on (all of them for keys in the prefix)
     int begin = seq.causal && k0 >= seq.prefix ? k0 - seq.shift : 0;
     begin = begin < 0 ? 0 : begin / GT * GT;
-    const int steps = begin < queries ? (queries - begin + GT - 1) / GT : 0, total = steps * group;
+    const int steps = begin < queries ? (queries - begin + GT - 1) / GT : 0, total = steps * share;
     // steps in order: tiles of the first head, then of the next; tiles without a document of the block's are skipped
     auto next = [&](int n) {
         if (!docs) return n;
@@ -308,13 +325,12 @@ __global__ void __launch_bounds__(256, DP == 64 && sizeof(T) == 2 ? 2 : 1) atten
         return n;
     };
     const int lane_row = L::template lane_row<R>(lane), lane_col = L::template lane_column<R>(lane);
-    Stage<T, DP, GT, 256, WIDE> sq, sg;
+    Stage<T, DP, GT, THREADS, WIDE> stage;
     float side = 0.0f;      // threads 0..63: a log-sum, 64..127: a delta
     int64_t qdoc = -1;      // threads 0..63
-    auto fetch = [&](int n) {
-        const int h = hk * group + n / steps, i0 = begin + (n % steps) * GT;
-        sq.load((const T*)a.q + b * a.q_batch + h * a.q_head, a.q_token, i0, queries, dim);
-        sg.load((const T*)gr.grad_out + b * gr.g_batch + h * gr.g_head, gr.g_token, i0, queries, dim);
+    auto fetch_queries = [&](int n) {
+        const int h = hk * group + head0 + n / steps, i0 = begin + (n % steps) * GT;
+        stage.load((const T*)a.q + b * a.q_batch + h * a.q_head, a.q_token, i0, queries, dim);
         const int i = i0 + (threadIdx.x & 63);
         const int64_t row = ((int64_t)b * a.heads + h) * queries + i;
         // a query behind the last gets weights exp(-inf) = 0
@@ -322,99 +338,110 @@ __global__ void __launch_bounds__(256, DP == 64 && sizeof(T) == 2 ? 2 : 1) atten
         else if (threadIdx.x < 128) side = i < queries ? delta[row] * fit : 0.0f;
         if (docs && threadIdx.x < GT) qdoc = i < queries ? docs[i] : -1;
     };
-    auto put = [&](char* to) {
-        sq.store(to);
-        sg.store(to + TILE);
+    auto put_queries = [&](char* to) {
+        stage.store(to);
         if (threadIdx.x < 128) *reinterpret_cast<float*>(to + 2 * TILE + 4 * threadIdx.x) = side;
         if (docs && threadIdx.x < GT) reinterpret_cast<int64_t*>(to + 2 * TILE + 2 * GT * 4)[threadIdx.x] = qdoc;
     };
+    auto fetch_grads = [&](int n) {
+        stage.load((const T*)gr.grad_out + b * gr.g_batch + (hk * group + head0 + n / steps) * gr.g_head, gr.g_token, begin + (n % steps) * GT, queries, dim);
+    };
     int n = next(0), buf = 0;
     if (n < total) {
-        fetch(n);
-        put(lds);
+        fetch_queries(n);
+        put_queries(lds);
+        fetch_grads(n);
+        stage.store(lds + TILE);
     }
     __syncthreads();
     // MASKED: some query of the tile does not see some key of the block
     auto step = [&](auto masks) __attribute__((always_inline)) {
         constexpr bool MASKED = decltype(masks)::value;
         const int n1 = next(n + 1);
-        if (n1 < total) fetch(n1);
+        char* ahead = lds + (buf ^ 1) * STEP;
+        if (n1 < total) fetch_queries(n1);
         const char *qt = lds + buf * STEP, *gt = qt + TILE;
         const float *lses = reinterpret_cast<const float*>(qt + 2 * TILE), *deltas = lses + GT;
         const int64_t* qdocs = reinterpret_cast<const int64_t*>(deltas + GT);
-        const int h = hk * group + n / steps, i0 = begin + (n % steps) * GT;
+        const int h = hk * group + head0 + n / steps, i0 = begin + (n % steps) * GT;
         const float slope = biased ? a.slopes[h] * LOG2E : 0.0f;
         const bool one_document = !MASKED || !docs || docw.one(i0 / SPAN, lane);
         auto piece = [&](int t) __attribute__((always_inline)) {
             const int it = i0 + t;
-            const int ilast = it + R < queries ? it + R - 1 : queries - 1;
+            const int ilast = it + PIECE < queries ? it + PIECE - 1 : queries - 1;
             if (MASKED && (it >= queries || kw >= keys)) return;
             if (MASKED && seq.limit(ilast) <= kw) return;                              // none of these queries sees a key of the wave
-            Acc<R> s = {}, dp = {};
+            float s[N], dp[N];
 #pragma unroll
-            for (int c = 0; c < DP / CK; ++c) {
-                s = mma(L::template read<R>(qt + t * L::ROW, lane_row, 0, c), kf[c], s);
-                dp = mma(L::template read<R>(gt + t * L::ROW, lane_row, 0, c), vf[c], dp);
+            for (int n = 0; n < PIECE / R; ++n) {
+                Acc<R> u = {}, w = {};
+#pragma unroll
+                for (int c = 0; c < DP / CK; ++c) {
+                    u = mma(L::template read<R>(qt + t * L::ROW, lane_row, n * R, c), kf[c], u);
+                    w = mma(L::template read<R>(gt + t * L::ROW, lane_row, n * R, c), vf[c], w);
+                }
+#pragma unroll
+                for (int x = 0; x < REGS<R>; ++x) { s[n * REGS<R> + x] = u[x]; dp[n * REGS<R> + x] = w[x]; }
             }
             const bool masked = MASKED && (seq.limit(it) < kw + R || !one_document);
-            Frag<T> pf[R / CK], df[R / CK];
+            Frag<T> pf[PIECE / CK], df[PIECE / CK];
             const float *ls = lses + t + 4 * g, *dl = deltas + t + 4 * g;
             if (capped) {
 #pragma unroll
-                for (int x = 0; x < REGS<R>; ++x) {
+                for (int x = 0; x < N; ++x) {
                     const float th = cap_tanh<T>(s[x] * to_cap);
                     s[x] = from_cap * th;
-                    dp[x] = __builtin_fmaf(dp[x], fit, -dl[result_row<R>(x, 0)]) * (1.0f - th * th);
+                    dp[x] = product(__builtin_fmaf(dp[x], fit, -dl[piece_row<R>(x)]), __builtin_fmaf(-th, th, 1.0f));
                 }
             } else {
 #pragma unroll
-                for (int x = 0; x < REGS<R>; ++x) dp[x] = __builtin_fmaf(dp[x], fit, -dl[result_row<R>(x, 0)]);
+                for (int x = 0; x < N; ++x) dp[x] = __builtin_fmaf(dp[x], fit, -dl[piece_row<R>(x)]);
             }
             if (biased) {
                 const int here = it + 4 * g + seq.shift - j;
 #pragma unroll
-                for (int x = 0; x < REGS<R>; ++x) s[x] = __builtin_fmaf(-slope, fabsf((float)(here + result_row<R>(x, 0))), s[x] * pre);
+                for (int x = 0; x < N; ++x) s[x] = __builtin_fmaf(-slope, fabsf((float)(here + piece_row<R>(x))), s[x] * pre);
             }
 #pragma unroll
-            for (int x = 0; x < REGS<R>; ++x) {
-                s[x] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x], unit, -ls[result_row<R>(x, 0)]));
-                dp[x] *= s[x];
+            for (int x = 0; x < N; ++x) {
+                s[x] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x], unit, -ls[piece_row<R>(x)]));
+                dp[x] = product(dp[x], s[x]);
             }
             if (MASKED && masked) {
                 // query i = it + 4 g + row sees key j if j is in its sequence's prefix or not behind its place
-                const int from = j >= seq.end ? R : (!seq.causal || j < seq.prefix ? -R : j - seq.shift - it - 4 * g);
+                const int from = j >= seq.end ? PIECE : (!seq.causal || j < seq.prefix ? -PIECE : j - seq.shift - it - 4 * g);
 #pragma unroll
-                for (int x = 0; x < REGS<R>; ++x)
-                    if (result_row<R>(x, 0) < from) s[x] = dp[x] = 0.0f;
+                for (int x = 0; x < N; ++x)
+                    if (piece_row<R>(x) < from) s[x] = dp[x] = 0.0f;
                 if (!one_document) {
 #pragma unroll
-                    for (int x = 0; x < REGS<R>; ++x)
-                        if (!same_document<R>(qdocs + t + 4 * g, x, doc)) s[x] = dp[x] = 0.0f;
+                    for (int x = 0; x < N; ++x)
+                        if (!same_document(qdocs + t + 4 * g + piece_row<R>(x), doc)) s[x] = dp[x] = 0.0f;
                 }
             }
             // weights and score gradients are rounded to the operands' type for the last products; their sums are float32
 #pragma unroll
-            for (int x = 0; x < REGS<R>; ++x) {
+            for (int x = 0; x < N; ++x) {
                 pf[x / 8][x % 8] = (E)s[x];
                 df[x / 8][x % 8] = (E)dp[x];
             }
-            if (MASKED && masked && (holds_not_finite<T, DP, R>(gt + t * L::ROW, lane) || holds_not_finite<T, DP, R>(qt + t * L::ROW, lane))) {
+            if (MASKED && masked && (holds_not_finite<T, DP, PIECE>(gt + t * L::ROW, lane) || holds_not_finite<T, DP, PIECE>(qt + t * L::ROW, lane))) {
 #pragma unroll
-                for (int c = 0; c < R / CK; ++c)
+                for (int c = 0; c < PIECE / CK; ++c)
 #pragma unroll
                     for (int d = 0; d < DP / R; ++d) {
                         dv[d] = mma(finite_part<T>(L::template read_across<R>(gt + t * L::ROW, lane_col, c * CK, d)), pf[c], dv[d]);
                         dk[d] = mma(finite_part<T>(L::template read_across<R>(qt + t * L::ROW, lane_col, c * CK, d)), df[c], dk[d]);
                     }
 #pragma unroll 1
-                for (int row = 0; row < R && it + row < queries; ++row) {
+                for (int row = 0; row < PIECE && it + row < queries; ++row) {
                     const bool sees = j < seq.limit(it + row) && (one_document || (doc >= 0 && qdocs[t + row] == doc));
                     add_not_finite<T, DP, R>(gt, t + row, sees, false, g, dv);
                     add_not_finite<T, DP, R>(qt, t + row, sees, true, g, dk);
                 }
             } else {
 #pragma unroll
-                for (int c = 0; c < R / CK; ++c)
+                for (int c = 0; c < PIECE / CK; ++c)
 #pragma unroll
                     for (int d = 0; d < DP / R; ++d) {
                         dv[d] = mma(L::template read_across<R>(gt + t * L::ROW, lane_col, c * CK, d), pf[c], dv[d]);
@@ -422,14 +449,13 @@ __global__ void __launch_bounds__(256, DP == 64 && sizeof(T) == 2 ? 2 : 1) atten
                     }
             }
         };
-        if constexpr (BOTH && !MASKED) {
-            piece(0);
-            piece(R);
-        } else {
-#pragma unroll 1
-            for (int t = 0; t < GT; t += R) piece(t);
+        piece(0);
+        if (n1 < total) {
+            put_queries(ahead);
+            fetch_grads(n1);
         }
-        if (n1 < total) put(lds + (buf ^ 1) * STEP);
+        piece(PIECE);
+        if (n1 < total) stage.store(ahead + TILE);
         __syncthreads();
         buf ^= 1;
         n = n1;
@@ -450,34 +476,71 @@ __global__ void __launch_bounds__(256, DP == 64 && sizeof(T) == 2 ? 2 : 1) atten
 #pragma unroll
         for (int x = 0; x < REGS<R>; ++x) {
             const int col = d * R + result_row<R>(x, g);
-            if (col < dim) {
-                ((T*)gr.dk)[row + col] = from_float<T>(dk[d][x] * back);
+            if (col >= dim) continue;
+            if (parts > 1) {
+                const int64_t all = (int64_t)a.batch * keys * a.kv_heads * dim;
+                slabs[at.head * 2 * all + row + col] = dk[d][x] * back;
+                slabs[(at.head * 2 + 1) * all + row + col] = dv[d][x];
+            } else {
+                ((T*)gr.dk)[row + col] = from_float<T>(product(dk[d][x], back));
                 ((T*)gr.dv)[row + col] = from_float<T>(dv[d][x]);
             }
         }
 }
 
+// dk and dv from the parts of a group's heads, added in order: bound by HBM
+template <typename T>
+__global__ void __launch_bounds__(256) attention_gather_kernel(const float* __restrict__ slabs, int parts, int64_t n, T* __restrict__ dk, T* __restrict__ dv) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+        float x = 0.0f, y = 0.0f;
+        for (int p = 0; p < parts; ++p) {
+            x += slabs[p * 2 * n + i];
+            y += slabs[(p * 2 + 1) * n + i];
+        }
+        dk[i] = from_float<T>(x);
+        dv[i] = from_float<T>(y);
+    }
+}
+
+// Parts of a group's heads: a key tile whose workgroup takes all heads in turn is the longest chain of the pass, so where the key tiles alone do not
+// give two workgroups per compute unit the heads are divided (float32 sums through memory, added in order by a second launch).  8191 tokens in
+// documents, 16 / 4 heads of 128, one part: 947 us, of which the 45 tiles x 4 heads of the longest document's first keys are the chain.
+int attention_backward_parts(const tvl_attention_args& a) {
+    if (a.queries == 0) return 1;      // sums of nothing: no workspace either
+    const int64_t tiles = a.batch * a.kv_heads * ceil_div(a.keys, 128);
+    const int group = (int)(a.heads / a.kv_heads);
+    for (int p = 1; p < group; ++p)
+        if (group % p == 0 && tiles * p >= 512) return p;
+    return group;
+}
+
 template <typename T, int DP, Form FORM>
-static int launch_gradients(const tvl_attention_args& a, const tvl_attention_grads& g, const DocumentSpan* spans, const float* delta, const float* maxima, hipStream_t st) {
+static int launch_gradients(const tvl_attention_args& a, const tvl_attention_grads& g, const DocumentSpan* spans, const float* delta, const float* maxima, float* slabs, hipStream_t st) {
     if (g.dq && a.queries > 0) {
         const int tiles = (int)ceil_div(a.queries, 128);
         const size_t bytes = 4 * GT * (size_t)Tile<T, DP>::ROW + (FORM == PLAIN ? 0 : 2 * GT * 8);
         if (bytes > 65536) TVL_HIP_CHECK(hipFuncSetAttribute((const void*)attention_dq_kernel<T, DP, FORM>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
-        hipLaunchKernelGGL((attention_dq_kernel<T, DP, FORM>), dim3((unsigned)(a.batch * a.heads * tiles)), dim3(256), bytes, st, a, g, spans, delta, tiles);
+        hipLaunchKernelGGL((attention_dq_kernel<T, DP, FORM>), dim3((unsigned)(a.batch * a.heads * tiles)), dim3(64 * Shape<T, DP, true>::W), bytes, st, a, g, spans, delta, tiles);
         TVL_LAUNCH_CHECK();
     }
     if (g.dk && a.keys > 0) {
-        const int tiles = (int)ceil_div(a.keys, 128);
+        const int tiles = (int)ceil_div(a.keys, 128), parts = attention_backward_parts(a);
         const size_t bytes = 2 * (2 * GT * (size_t)Tile<T, DP>::ROW + 2 * GT * 4 + (FORM == PLAIN ? 0 : GT * 8));
         if (bytes > 65536) TVL_HIP_CHECK(hipFuncSetAttribute((const void*)attention_dkv_kernel<T, DP, FORM>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
-        hipLaunchKernelGGL((attention_dkv_kernel<T, DP, FORM>), dim3((unsigned)(a.batch * a.kv_heads * tiles)), dim3(256), bytes, st, a, g, spans, delta, maxima, tiles);
+        hipLaunchKernelGGL((attention_dkv_kernel<T, DP, FORM>), dim3((unsigned)(a.batch * a.kv_heads * tiles * parts)), dim3(64 * Shape<T, DP, false>::W), bytes, st, a, g, spans, delta, maxima,
+                           tiles, parts, slabs);
         TVL_LAUNCH_CHECK();
+        if (parts > 1) {
+            const int64_t n = a.batch * a.keys * a.kv_heads * a.dim, blocks = ceil_div(n, 256);
+            hipLaunchKernelGGL((attention_gather_kernel<T>), dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, st, slabs, parts, n, (T*)g.dk, (T*)g.dv);
+            TVL_LAUNCH_CHECK();
+        }
     }
     return TVL_OK;
 }
 
 template <typename T>
-static int launch_backward(const tvl_attention_args& a, const tvl_attention_grads& g, const DocumentSpan* spans, float* delta, float* maxima, hipStream_t st) {
+static int launch_backward(const tvl_attention_args& a, const tvl_attention_grads& g, const DocumentSpan* spans, float* delta, float* maxima, float* slabs, hipStream_t st) {
     const size_t z = sizeof(T);
     const bool grad = wide_rows(g.grad_out, a.dim, g.g_batch, g.g_token, g.g_head, z);
     const bool wide = grad && wide_rows(a.q, a.dim, a.q_batch, a.q_token, a.q_head, z) && wide_rows(a.k, a.dim, a.k_batch, a.k_token, a.k_head, z) &&
@@ -489,15 +552,16 @@ static int launch_backward(const tvl_attention_args& a, const tvl_attention_grad
         else hipLaunchKernelGGL((attention_delta_kernel<T, false>), dim3(n), dim3(256), 0, st, a, g, delta, maxima, blocks);
         TVL_LAUNCH_CHECK();
     }
-    if (!wide) return launch_gradients<T, 128, ODD>(a, g, spans, delta, maxima, st);
-    if (a.dim <= 64) return featureless(a) ? launch_gradients<T, 64, PLAIN>(a, g, spans, delta, maxima, st) : launch_gradients<T, 64, GENERAL>(a, g, spans, delta, maxima, st);
-    return featureless(a) ? launch_gradients<T, 128, PLAIN>(a, g, spans, delta, maxima, st) : launch_gradients<T, 128, GENERAL>(a, g, spans, delta, maxima, st);
+    // odd rows take the same shapes: the same sums in the same order
+    if (!wide) return a.dim <= 64 ? launch_gradients<T, 64, ODD>(a, g, spans, delta, maxima, slabs, st) : launch_gradients<T, 128, ODD>(a, g, spans, delta, maxima, slabs, st);
+    if (a.dim <= 64) return featureless(a) ? launch_gradients<T, 64, PLAIN>(a, g, spans, delta, maxima, slabs, st) : launch_gradients<T, 64, GENERAL>(a, g, spans, delta, maxima, slabs, st);
+    return featureless(a) ? launch_gradients<T, 128, PLAIN>(a, g, spans, delta, maxima, slabs, st) : launch_gradients<T, 128, GENERAL>(a, g, spans, delta, maxima, slabs, st);
 }
 
-int launch_attention_backward(const tvl_attention_args& a, const tvl_attention_grads& g, const DocumentSpan* spans, float* delta, float* maxima, hipStream_t st) {
-    if (a.dtype == TVL_F32) return launch_backward<float>(a, g, spans, delta, maxima, st);
-    if (a.dtype == TVL_F16) return launch_backward<f16>(a, g, spans, delta, maxima, st);
-    return launch_backward<bf16_t>(a, g, spans, delta, maxima, st);
+int launch_attention_backward(const tvl_attention_args& a, const tvl_attention_grads& g, const DocumentSpan* spans, float* delta, float* maxima, float* slabs, hipStream_t st) {
+    if (a.dtype == TVL_F32) return launch_backward<float>(a, g, spans, delta, maxima, slabs, st);
+    if (a.dtype == TVL_F16) return launch_backward<f16>(a, g, spans, delta, maxima, slabs, st);
+    return launch_backward<bf16_t>(a, g, spans, delta, maxima, slabs, st);
 }
 
 }  // namespace tvl

@@ -139,7 +139,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attention_forward
                     for (int t = 0; t < KT / R; ++t)
 #pragma unroll
                         for (int x = 0; x < REGS<R>; ++x)
-                            if (!same_document<R>(kdocs + t * R + 4 * g, x, doc)) s[t][x] = -__builtin_inff();
+                            if (!same_document(kdocs + t * R + result_row<R>(x, g), doc)) s[t][x] = -__builtin_inff();
                 }
             }
             float top = s[0][0];
@@ -207,7 +207,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attention_forward
             const int col = d * R + result_row<R>(x, g);
             T v[4];
 #pragma unroll
-            for (int y = 0; y < 4; ++y) v[y] = from_float<T>(nan ? __builtin_nanf("") : (empty ? 0.0f : acc[d][x + y] * inv));
+            for (int y = 0; y < 4; ++y) v[y] = from_float<T>(nan ? __builtin_nanf("") : (empty ? 0.0f : product(acc[d][x + y], inv)));
             if constexpr (WIDE) {
                 typedef uint32_t quad __attribute__((ext_vector_type(sizeof(T))));
                 if (col < dim) *reinterpret_cast<quad*>(op + col) = *reinterpret_cast<const quad*>(v);
@@ -256,7 +256,7 @@ static int launch_forward_t(const tvl_attention_args& a, const DocumentSpan* spa
     const size_t z = sizeof(T);
     const bool wide = wide_rows(a.q, a.dim, a.q_batch, a.q_token, a.q_head, z) && wide_rows(a.k, a.dim, a.k_batch, a.k_token, a.k_head, z) &&
                       wide_rows(a.v, a.dim, a.v_batch, a.v_token, a.v_head, z) && wide_rows(a.out, a.dim, a.o_batch, a.o_token, a.o_head, z);
-    if (!wide) return launch_forward<T, 128, CACHED, ODD>(a, spans, st);
+    if (!wide) return a.dim <= 64 ? launch_forward<T, 64, CACHED, ODD>(a, spans, st) : launch_forward<T, 128, CACHED, ODD>(a, spans, st);
     if (a.dim <= 64) return featureless(a) ? launch_forward<T, 64, CACHED, PLAIN>(a, spans, st) : launch_forward<T, 64, CACHED, GENERAL>(a, spans, st);
     return featureless(a) ? launch_forward<T, 128, CACHED, PLAIN>(a, spans, st) : launch_forward<T, 128, CACHED, GENERAL>(a, spans, st);
 }

@@ -64,28 +64,34 @@ template <typename T> __device__ __forceinline__ Frag<T> finite_part(Frag<T> a) 
 }
 
 // ---- tiles in LDS ------------------------------------------------------------------------------
-// Rows of DP elements in 16-byte units.  A unit lies at its place with the low three bits exchanged by the row's, so that the 8 rows a
-// b128 read takes at a time, and the 4 rows x 2 units of a transposing read, fall on different banks.  A row's exchange depends on
-// its place among 8 rows only: a lane works out its offset once, and what the compiler knows (chunk, tile, half) is an exclusive-or or
-// an immediate.
+// Rows of DP elements in 16-byte units.  LDS has 64 banks of 4 bytes: 16 lanes of a b128 read, 32 lanes of a transposing b64 read, go together.  A
+// unit lies at its place with its low bits exchanged by the row's, so that 16 rows at one place of a row, and 4 rows x 4 neighbouring
+// units, all fall on different banks.  The exchange is an exclusive-or of bits of the row's number: a lane works out its offset
+// once, and what the compiler knows (chunk, tile, half) is an exclusive-or or an immediate.
 template <typename T, int DP> struct Tile {
     static constexpr int UNITS = DP * (int)sizeof(T) / 16;
     static constexpr int PER = 16 / (int)sizeof(T);          // elements of a unit
     static constexpr int ROW = DP * (int)sizeof(T);
+    static constexpr int LOW = UNITS % 16 == 0 ? 15 : 7;     // unit bits that are exchanged
     static_assert(UNITS % 8 == 0, "rows are multiples of 128 bytes");
-    __device__ static __forceinline__ int swap_bits(int row) { return ((row & 3) << 1) | ((row >> 2) & 1); }
+    // rows of 128 bytes: two fill the banks, so 8 pairs; longer rows: each fills them
+    __device__ static __forceinline__ constexpr int swap_bits(int row) {
+        return LOW == 7 ? ((row >> 1) & 1) << 2 | ((row >> 3) & 1) << 1 | ((row >> 2) & 1) : (row & 3) << 2 | ((row >> 2) & 3);
+    }
     __device__ static __forceinline__ int at(int row, int unit) { return row * ROW + ((unit ^ swap_bits(row)) << 4); }
-    // a lane's offset moved by `unit` units (bits the lane's own unit does not use)
-    __device__ static __forceinline__ int moved(int lane_at, int unit) { return (lane_at ^ ((unit & 7) << 4)) + ((unit & ~7) << 4); }
+    // a lane's offset moved by `unit` units and `rows` rows (bits that the lane's own unit and row do not use)
+    __device__ static __forceinline__ int moved(int lane_at, int unit, int rows) {
+        return (lane_at ^ (((unit ^ swap_bits(rows)) & LOW) << 4)) + ((unit & ~LOW) << 4) + rows * ROW;
+    }
 
-    // fragments of row `row0 + r`, elements 8 (g + (64 / R) c) ..: a lane's offset, and the read
+    // fragments of row `row0 + r`, elements 8 (g + (64 / R) c) ..: a lane's offset, and the read  (row0 a multiple of 32)
     template <int R> __device__ static __forceinline__ int lane_row(int lane) { return at(lane % R, (lane / R) * (8 / PER)); }
     template <int R> __device__ static __forceinline__ Frag<T> read(const char* tile, int lane_at, int row0, int c) {
         if constexpr (sizeof(T) == 2) {
-            return __builtin_bit_cast(Frag<T>, *reinterpret_cast<const u32x4*>(tile + moved(lane_at, 64 / R * c) + row0 * ROW));
+            return __builtin_bit_cast(Frag<T>, *reinterpret_cast<const u32x4*>(tile + moved(lane_at, 64 / R * c, 0) + row0 * ROW));
         } else {
-            const f32x4 lo = *reinterpret_cast<const f32x4*>(tile + moved(lane_at, 128 / R * c) + row0 * ROW);
-            const f32x4 hi = *reinterpret_cast<const f32x4*>(tile + moved(lane_at, 128 / R * c + 1) + row0 * ROW);
+            const f32x4 lo = *reinterpret_cast<const f32x4*>(tile + moved(lane_at, 128 / R * c, 0) + row0 * ROW);
+            const f32x4 hi = *reinterpret_cast<const f32x4*>(tile + moved(lane_at, 128 / R * c + 1, 0) + row0 * ROW);
             return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
         }
     }
@@ -102,7 +108,7 @@ template <typename T, int DP> struct Tile {
             i16x4 v[2];
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                const char* p = tile + moved(lane_at, d * R / PER) + (row0 + CHUNK<R> / 2 * u) * ROW;
+                const char* p = tile + moved(lane_at, d * R / PER, CHUNK<R> / 2 * u) + row0 * ROW;
                 v[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(p));
             }
             return __builtin_bit_cast(Frag<T>, __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7));
@@ -112,7 +118,7 @@ template <typename T, int DP> struct Tile {
             for (int u = 0; u < 2; ++u)
 #pragma unroll
                 for (int y = 0; y < 4; ++y)
-                    f[4 * u + y] = *reinterpret_cast<const float*>(tile + moved(lane_at, (d * R / PER) ^ (y << 1)) + (row0 + CHUNK<R> / 2 * u + y) * ROW);
+                    f[4 * u + y] = *reinterpret_cast<const float*>(tile + moved(lane_at, d * R / PER, CHUNK<R> / 2 * u + y) + row0 * ROW);
             return f;
         }
     }
@@ -187,7 +193,7 @@ __device__ __forceinline__ Frag<T> load_frag(const T* row, int c8, int dim) {
 template <typename T, int DP, int ROWS, int THREADS, bool WIDE> struct Stage {
     typedef Tile<T, DP> L;
     static constexpr int N = ROWS * L::UNITS / THREADS, APART = THREADS / L::UNITS;
-    static_assert(ROWS * L::UNITS % THREADS == 0 && THREADS % L::UNITS == 0 && APART % 8 == 0, "every thread moves the same unit of rows APART apart");
+    static_assert(ROWS * L::UNITS % THREADS == 0 && THREADS % L::UNITS == 0 && APART % 8 == 0 && (APART % 16 == 0 || APART == 8), "every thread moves the same unit of rows APART apart");
     u32x4 v[N];
     // rows row0 .. row0 + ROWS - 1 of a matrix; rows from `end` on are zero and not read.  One 32-bit offset per lane, the rest is in scalar
     // registers: per-row offsets get spilled, and a reload waits for the loads in front of it
@@ -216,7 +222,7 @@ template <typename T, int DP, int ROWS, int THREADS, bool WIDE> struct Stage {
     __device__ __forceinline__ void store(char* tile) const {
         const int at = L::at(threadIdx.x / L::UNITS, threadIdx.x % L::UNITS);
 #pragma unroll
-        for (int x = 0; x < N; ++x) *reinterpret_cast<u32x4*>(tile + at + x * APART * L::ROW) = v[x];
+        for (int x = 0; x < N; ++x) *reinterpret_cast<u32x4*>(tile + L::moved(at, 0, x * APART)) = v[x];
     }
 };
 
@@ -231,8 +237,8 @@ __device__ __forceinline__ void both_halves(float v, float& lo, float& hi) {
 // the wave's number in its workgroup, known to be the same for all its lanes
 __device__ __forceinline__ int wave_number() { return __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64); }
 
-// whether the row of result register x is of document `doc` (none if negative); `docs`: the documents of rows 4 g + .. of a tile, staged behind it in LDS
-template <int R> __device__ __forceinline__ bool same_document(const int64_t* docs, int x, int64_t doc) { return (docs[result_row<R>(x, 0)] == doc) & (doc >= 0); }
+// whether a token is of document `doc` (none if negative): its document is staged beside its tile in LDS
+__device__ __forceinline__ bool same_document(const int64_t* staged, int64_t doc) { return (*staged == doc) & (doc >= 0); }
 
 // maximum / sum over the lanes that hold one column (the groups g)
 template <int R> __device__ __forceinline__ float column_max(float v) {
@@ -258,6 +264,13 @@ constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 template <typename T> __device__ __forceinline__ float cap_tanh(float y) {
     if constexpr (sizeof(T) == 4) return tanhf(y);
     return 1.0f - 2.0f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(y * (2.0f * LOG2E)) + 1.0f);
+}
+
+// a product that is rounded to float32 before anything else happens to it: never part of a fused or mixed-precision instruction, so the same bits
+// in every form of a kernel
+__device__ __forceinline__ float product(float x, float y) {
+#pragma clang fp contract(off)
+    return x * y;
 }
 
 // Sequence b of a call.  Places and limits fit 32 bits: tokens are at most 2^30.
@@ -381,7 +394,8 @@ static inline bool wide_rows(const void* p, int64_t dim, int64_t batch, int64_t 
 }
 
 int launch_attention_forward(const tvl_attention_args& a, bool cached, const DocumentSpan* spans, hipStream_t st);
-int launch_attention_backward(const tvl_attention_args& a, const tvl_attention_grads& g, const DocumentSpan* spans, float* delta, float* maxima, hipStream_t st);
+int launch_attention_backward(const tvl_attention_args& a, const tvl_attention_grads& g, const DocumentSpan* spans, float* delta, float* maxima, float* slabs, hipStream_t st);
+int attention_backward_parts(const tvl_attention_args& a);
 bool attention_step_serves(const tvl_attention_args& a);
 size_t attention_step_bytes(const tvl_attention_args& a);
 int launch_attention_step(const tvl_attention_args& a, float* parts, hipStream_t st);
