@@ -11,6 +11,10 @@ matmul epilogue, ``utils/conversion.py:185-187``) and fc2 - with random ternary 
 same LayerNorm output, so by default they run as ONE packed matmul over 6144 + 8192 channels whose activation
 starts at channel 6144 (``DecoderConfig.fuse_qkv_fc1``): three launches per block instead of four.
 
+What stands between the products - rotation, cache write, attention - is either the reference's sequence of tensor operations (the
+default) or, with ``DecoderConfig.fuse_attention``, two calls of :mod:`attention_ops`: ``rotary_cache`` takes the joint projection's output
+straight into the cache and ``cached_attention`` reads its filled part, instead of ~15 launches and a softmax over all ``max_len`` slots.
+
 A decode step has ~100 short kernels; launched one by one it is bound by the host.  The step is therefore
 captured once into a HIP graph (static cache buffers, position kept on the device) and replayed.
 """
@@ -23,7 +27,7 @@ from typing import Dict, List, Optional
 
 import torch
 
-from . import custom_ops_mod as ops
+from . import attention_ops, custom_ops_mod as ops
 
 
 @dataclass
@@ -39,6 +43,7 @@ class DecoderConfig:
     max_len: int = 1024
     fuse_qkv_fc1: bool = True     # Wqkv | fc1 as one packed matrix, tanh-GELU from channel 3 * hidden on
     fuse_residual: bool = True    # the block's closing attn + mlp + residual as part of fc2's call (same bits as the separate additions)
+    fuse_attention: bool = False  # rotation + cache write as one launch, attention over the filled part of the cache (float32 rotation and softmax: other roundings than the tensor operations)
 
     @property
     def head_dim(self) -> int:
@@ -140,6 +145,7 @@ class TernaryDecoderStack:
         gen = torch.Generator().manual_seed(seed)
         self.blocks = [Block(cfg, gen, self.device, dtype) for _ in range(cfg.blocks)]
         self.cos, self.sin = _rope_tables(cfg, self.device, dtype)
+        self.table = attention_ops.rotary_table(cfg.rotary_dim, cfg.max_len, cfg.rope_theta, device=self.device) if cfg.fuse_attention else None
         shape = (cfg.blocks, batch, cfg.heads, cfg.max_len, cfg.head_dim)
         self.k_cache = torch.zeros(shape, device=self.device, dtype=dtype)
         self.v_cache = torch.zeros(shape, device=self.device, dtype=dtype)
@@ -151,25 +157,33 @@ class TernaryDecoderStack:
         self.fused_calls = True                    # tests that swap `linear` for the dense twin turn this off too
 
     # ------------------------------------------------------------------ one block, any number of new tokens
-    def _block(self, i: int, blk: Block, h: torch.Tensor, positions: torch.Tensor, mask: torch.Tensor) -> torch.Tensor:
-        cfg = self.cfg
-        b, t, _ = h.shape
-        x = torch.nn.functional.layer_norm(h, (cfg.hidden,), blk.ln_w.to(h.dtype), blk.ln_b.to(h.dtype), cfg.eps)
-        if blk.qkv_fc1 is not None:
-            z = self.linear(blk.qkv_fc1, x).to(h.dtype)
-            qkv, fc1_out = z[..., : 3 * cfg.hidden].reshape(b, t, 3, cfg.heads, cfg.head_dim), z[..., 3 * cfg.hidden:]
-        else:
-            qkv, fc1_out = self.linear(blk.wqkv, x).to(h.dtype).view(b, t, 3, cfg.heads, cfg.head_dim), None
-        q, k, v = (qkv[:, :, j].transpose(1, 2) for j in range(3))            # [b, heads, t, hd]
+    def _attend(self, i: int, qkv: torch.Tensor, positions: torch.Tensor, mask: Optional[torch.Tensor], cache_len) -> torch.Tensor:
+        """Rotated new tokens into the cache of block i, and their attention over it: ``qkv [b, t, 3 * hidden]`` -> ``[b, t, hidden]``."""
+        cfg, (b, t, _) = self.cfg, qkv.shape
+        if cfg.fuse_attention:
+            q = attention_ops.rotary_cache(qkv, self.table, self.k_cache[i], self.v_cache[i], cache_len, cfg.heads)
+            return attention_ops.cached_attention(q, self.k_cache[i], self.v_cache[i], cache_len).reshape(b, t, cfg.hidden)
+        q, k, v = (qkv.reshape(b, t, 3, cfg.heads, cfg.head_dim)[:, :, j].transpose(1, 2) for j in range(3))            # [b, heads, t, hd]
         rd = cfg.rotary_dim
-        cos, sin = self.cos[positions].to(h.dtype), self.sin[positions].to(h.dtype)   # [t, rd]
+        cos, sin = self.cos[positions].to(qkv.dtype), self.sin[positions].to(qkv.dtype)   # [t, rd]
         q = torch.cat([q[..., :rd] * cos + _rotate_half(q[..., :rd]) * sin, q[..., rd:]], dim=-1)
         k = torch.cat([k[..., :rd] * cos + _rotate_half(k[..., :rd]) * sin, k[..., rd:]], dim=-1)
         kc, vc = self.k_cache[i], self.v_cache[i]
         kc.index_copy_(2, positions, k.to(kc.dtype))
         vc.index_copy_(2, positions, v.to(vc.dtype))
-        att = torch.nn.functional.scaled_dot_product_attention(q, kc.to(h.dtype), vc.to(h.dtype), attn_mask=mask)
-        att = att.transpose(1, 2).reshape(b, t, cfg.hidden)
+        att = torch.nn.functional.scaled_dot_product_attention(q, kc.to(qkv.dtype), vc.to(qkv.dtype), attn_mask=mask)
+        return att.transpose(1, 2).reshape(b, t, cfg.hidden)
+
+    def _block(self, i: int, blk: Block, h: torch.Tensor, positions: torch.Tensor, mask: Optional[torch.Tensor], cache_len) -> torch.Tensor:
+        cfg = self.cfg
+        b, t, _ = h.shape
+        x = torch.nn.functional.layer_norm(h, (cfg.hidden,), blk.ln_w.to(h.dtype), blk.ln_b.to(h.dtype), cfg.eps)
+        if blk.qkv_fc1 is not None:
+            z = self.linear(blk.qkv_fc1, x).to(h.dtype)
+            qkv, fc1_out = z[..., : 3 * cfg.hidden], z[..., 3 * cfg.hidden:]
+        else:
+            qkv, fc1_out = self.linear(blk.wqkv, x).to(h.dtype), None
+        att = self._attend(i, qkv, positions, mask, cache_len)
         attn_out = self.linear(blk.out_proj, att).to(h.dtype)
         if fc1_out is None:
             fc1_out = self.linear(blk.fc1, x).to(h.dtype)
@@ -179,11 +193,11 @@ class TernaryDecoderStack:
         mlp = self.linear(blk.fc2, fc1_out).to(h.dtype)
         return attn_out + mlp + h
 
-    def _forward(self, h: torch.Tensor, positions: torch.Tensor) -> torch.Tensor:
+    def _forward(self, h: torch.Tensor, positions: torch.Tensor, cache_len) -> torch.Tensor:
         # a new token at position p attends to cache slots <= p (slots beyond the filled part are masked out)
-        mask = torch.arange(self.cfg.max_len, device=self.device)[None, :] <= positions[:, None]    # [t, max_len]
+        mask = None if self.cfg.fuse_attention else torch.arange(self.cfg.max_len, device=self.device)[None, :] <= positions[:, None]    # [t, max_len]
         for i, blk in enumerate(self.blocks):
-            h = self._block(i, blk, h, positions, mask)
+            h = self._block(i, blk, h, positions, mask, cache_len)
         return h
 
     # ------------------------------------------------------------------ prefill and decode
@@ -193,13 +207,13 @@ class TernaryDecoderStack:
     def prefill(self, emb: torch.Tensor) -> torch.Tensor:
         t = emb.shape[1]
         positions = torch.arange(t, device=self.device)
-        out = self._forward(emb, positions)
+        out = self._forward(emb, positions, 0)
         self.pos.fill_(t)
         return out
 
     def decode_step(self, emb: torch.Tensor) -> torch.Tensor:
         """One new token per sequence, launched kernel by kernel."""
-        out = self._forward(emb, self.pos.view(1))
+        out = self._forward(emb, self.pos.view(1), self.pos)
         self.pos += 1
         return out
 
@@ -276,7 +290,7 @@ def run(cfg: DecoderConfig, batch: int, prompt_len: int, steps: int, device="cud
     mm_s = (time.perf_counter() - t0) / 20
     return {
         "matmuls_only_ms_per_step": mm_s * 1e3, "matmuls_only_weight_stream_GBps": stack.packed_weight_bytes() / mm_s / 1e9,
-        "batch": batch, "prompt_len": prompt_len, "steps": steps, "blocks": cfg.blocks, "graph": use_graph,
+        "batch": batch, "prompt_len": prompt_len, "steps": steps, "blocks": cfg.blocks, "graph": use_graph, "fused_attention": cfg.fuse_attention,
         "prefill_ms": prefill_s * 1e3, "prefill_tokens_per_s": batch * prompt_len / prefill_s,
         "decode_ms_per_step": decode_s / steps * 1e3, "decode_tokens_per_s": batch * steps / decode_s,
         "packed_weight_MB": stack.packed_weight_bytes() / 1e6,

@@ -655,3 +655,30 @@ def test_decode_step_captured_and_replayed(tv, dev):
         torch.cuda.synchronize()
         assert torch.equal(out, want) and torch.equal(lens, lens2), n
     assert torch.equal(k, k2) and torch.equal(v, v2)
+
+
+@pytest.mark.parametrize("fused_product", [True, False])
+def test_decode_harness_with_fused_attention(tv, dev, fused_product):
+    """The decoder stack with rotary_cache + cached_attention against the same stack with the tensor operations (float32: both evaluate the same sums to
+    about 1e-6 an operation; the bound is that of packed against dense products), and its captured step against the eager one bit for bit."""
+    from ternary_vllm_amd import decode_harness as dh
+    kw = dict(hidden=256, heads=4, intermediate=1024, blocks=2, max_len=64, fuse_qkv_fc1=fused_product)
+    torch.manual_seed(3)
+    prompt = torch.randn(2, 19, 256, device=dev)
+    toks = [torch.randn(2, 1, 256, device=dev) for _ in range(4)]
+
+    def run(fuse, graph):
+        st = dh.TernaryDecoderStack(dh.DecoderConfig(fuse_attention=fuse, **kw), batch=2, device=dev, dtype=torch.float32, seed=11)
+        with torch.no_grad():
+            outs = [st.prefill(prompt)]
+            if graph:
+                st.capture_decode(toks[0])
+            outs += [(st.decode_graph(t) if graph else st.decode_step(t)).clone() for t in toks]
+        assert int(st.pos) == 19 + len(toks)
+        return outs
+
+    plain, fused, replay = run(False, False), run(True, False), run(True, True)
+    for a, b in zip(fused, plain):
+        assert a.shape == b.shape and float((a - b).abs().max()) <= 2e-4 * max(1.0, float(b.abs().max()))
+    for a, b in zip(fused, replay):
+        assert torch.equal(a, b)
