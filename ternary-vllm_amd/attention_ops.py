@@ -56,22 +56,29 @@ def _same(t: torch.Tensor, like: torch.Tensor, name: str) -> None:
         raise ValueError(f"{name}: {t.dtype} on {t.device}, the other operands are {like.dtype} on {like.device}")
 
 
+# the current stream's handle without a Stream object around it (3 us less a call)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def _run(fn, device: torch.device, *args) -> None:
-    if torch.cuda.current_device() == device.index:   # skip the device guard when it is a no-op
-        ops._check(fn(*args, torch.cuda.current_stream(device).cuda_stream))
+    index = device.index
+    if torch.cuda.current_device() == index:   # skip the device guard when it is a no-op
+        status = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(device):
-            ops._check(fn(*args, torch.cuda.current_stream(device).cuda_stream))
+            status = fn(*args, _raw_stream(index))
+    if status:
+        ops._check(status)
 
 
 def _apply(fn, name: str, inputs, *rest) -> torch.Tensor:
     """``fn.apply``, refused where recording it into a HIP graph would end the process: on a leaf whose gradient node was made by an
     eager call on another stream and still lives, the backward pass would join that stream into the capture.  A node's own
     metadata (it lives as long as the node) carries the stream of the call that made it."""
-    leaves = [x for x in inputs if x.is_leaf and x.requires_grad]
+    leaves = [x for x in inputs if x.requires_grad and x.is_leaf]
     if not leaves:
         return fn.apply(*inputs, *rest)
-    stream = torch.cuda.current_stream(inputs[0].device).cuda_stream
+    stream = _raw_stream(inputs[0].device.index)
     if torch.cuda.is_current_stream_capturing():
         if any(torch.autograd.graph.get_gradient_edge(x).node.metadata.get("tvl_stream", stream) != stream for x in leaves):
             raise RuntimeError(f"{name}: an eager graph of one of these leaves is still alive and belongs to another stream; its backward pass cannot be "
@@ -140,7 +147,7 @@ def _ld_table(table: torch.Tensor) -> int:
 
 def _rotary(x: torch.Tensor, positions: torch.Tensor, table: torch.Tensor, interleaved: bool, inverse: bool) -> torch.Tensor:
     b, t, h, d = x.shape
-    y = torch.empty((b, t, h, d), dtype=x.dtype, device=x.device)
+    y = x.new_empty((b, t, h, d))
     pb, pt = (0, positions.stride(0)) if positions.dim() == 1 else positions.stride()
     xs, ys = x.stride(), y.stride()
     args = _ROTARY.pack(_ROTARY.size, x.data_ptr(), y.data_ptr(), positions.data_ptr(), table.data_ptr(), b, t, h, d, table.shape[1], table.shape[0],
@@ -177,7 +184,7 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, table: torch.Tensor, interl
     if positions.dtype != torch.int64 or positions.device != x.device or positions.shape not in ((t,), (b, t)):
         raise ValueError(f"rotary: positions must be int64 [{t}] or [{b}, {t}] on {x.device}, got {tuple(positions.shape)} {positions.dtype} on {positions.device}")
     _check_table(table, d, x.device, "rotary")
-    if torch.is_grad_enabled() and x.requires_grad:
+    if x.requires_grad and torch.is_grad_enabled():
         return _apply(_RotaryFn, "rotary", (x,), positions, table, bool(interleaved))
     return _rotary(x, positions, table, interleaved, False)
 
@@ -211,6 +218,11 @@ def _apart(t: torch.Tensor) -> bool:
 
 
 def _check_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, like: torch.Tensor, b: int, d: int, name: str, written: bool):
+    if (isinstance(k_cache, torch.Tensor) and isinstance(v_cache, torch.Tensor) and k_cache.dtype is like.dtype and v_cache.dtype is like.dtype
+            and k_cache.device == like.device and v_cache.device == like.device and k_cache.dim() == 4 and k_cache.shape == v_cache.shape
+            and k_cache.shape[0] == b and k_cache.shape[3] == d and k_cache.is_contiguous() and v_cache.is_contiguous()
+            and not (k_cache.requires_grad or v_cache.requires_grad)):
+        return      # the common case
     for c, what in ((k_cache, "k_cache"), (v_cache, "v_cache")):
         ops._gpu(c, f"{name}({what})")
         if c.dim() != 4 or c.shape != k_cache.shape or c.shape[0] != b or c.shape[3] != d:
@@ -237,7 +249,7 @@ def rotary_cache(qkv: torch.Tensor, table: torch.Tensor, k_cache: torch.Tensor, 
     ops._gpu(qkv, "rotary_cache(qkv)")
     if qkv.dim() != 3 or qkv.dtype not in _FLOATS:
         raise ValueError(f"rotary_cache: qkv must be a float [batch, tokens, channels] tensor, got {tuple(qkv.shape)} {qkv.dtype}")
-    if torch.is_grad_enabled() and qkv.requires_grad:
+    if qkv.requires_grad and torch.is_grad_enabled():
         raise ValueError("rotary_cache is a serving form without gradients: call it under torch.no_grad(), or use rotary")
     if qkv.shape[2] > 1 and qkv.stride(2) != 1:
         qkv = qkv.contiguous()
@@ -254,7 +266,7 @@ def rotary_cache(qkv: torch.Tensor, table: torch.Tensor, k_cache: torch.Tensor, 
         raise ValueError("rotary_cache: k_cache and v_cache are the same memory")
     _check_table(table, d, qkv.device, "rotary_cache")
     at, stride, value, n, count = _lengths(cache_len, count, b, t, slots, qkv.device, "rotary_cache")
-    q = torch.empty((b, t, heads, d), dtype=qkv.dtype, device=qkv.device)
+    q = qkv.new_empty((b, t, heads, d))
     ks, vs = k_cache.stride(), v_cache.stride()
     args = _ROTARY_CACHE.pack(_ROTARY_CACHE.size, qkv.data_ptr(), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), table.data_ptr(), at, n,
                               b, t, heads, hk, d, table.shape[1], slots, table.shape[0], _ld_table(table), qkv.stride(0), qkv.stride(1),
@@ -277,7 +289,9 @@ def _prefix(prefix, b: int, device: torch.device, name: str):
 
 
 def _scale_cap(scale, softcap, d: int, name: str):
-    scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
+    if scale is None and softcap == 0.0:
+        return d ** -0.5, 0.0
+    scale = d ** -0.5 if scale is None else float(scale)
     softcap = 0.0 if softcap is None else float(softcap)
     if not math.isfinite(scale) or not (softcap >= 0.0 and math.isfinite(softcap)):
         raise ValueError(f"{name}: scale={scale} must be finite, softcap={softcap} finite and not negative")
@@ -304,7 +318,7 @@ def _attention_args(q, k, v, out, lse, causal, scale, softcap, slopes, prefix_at
 
 def _attention(q, k, v, causal, scale, softcap, slopes, prefix_at, prefix_value, documents, want_lse):
     b, tq, hq, d = q.shape
-    out = torch.empty((b, tq, hq, d), dtype=q.dtype, device=q.device)
+    out = q.new_empty((b, tq, hq, d))
     lse = torch.empty((b, hq, tq), dtype=torch.float32, device=q.device) if want_lse else None
     args = _attention_args(q, k, v, out, lse, causal, scale, softcap, slopes, prefix_at, prefix_value, documents)
     need = ops._lib.tvl_attention_workspace_bytes(args)
@@ -377,7 +391,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool = 
             raise ValueError(f"attention: documents must be int64 [{b}, {tq}] on {q.device} with as many queries as keys, got {tuple(documents.shape)} {documents.dtype} for {k.shape[1]} keys")
         if tq > 1 and documents.stride(1) != 1:
             documents = documents.contiguous()
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+    if (q.requires_grad or k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
         return _apply(_AttentionFn, "attention", (q, k, v), bool(causal), scale, softcap, slopes, prefix if prefix is not None else value, documents)
     return _attention(q, k, v, bool(causal), scale, softcap, slopes, at, value, documents, False)[0]
 
@@ -393,7 +407,7 @@ def cached_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     the cache gives a row of NaN (an int ``cache_len`` is checked here instead).  Only the filled part of the cache is read.  No gradients."""
     q = _heads(q, "cached_attention(q)")
     b, t, hq, d = q.shape
-    if torch.is_grad_enabled() and q.requires_grad:
+    if q.requires_grad and torch.is_grad_enabled():
         raise ValueError("cached_attention is a serving form without gradients: call it under torch.no_grad(), or use attention")
     _check_cache(k_cache, v_cache, q, b, d, "cached_attention", False)
     hk, slots = k_cache.shape[1], k_cache.shape[2]
@@ -406,7 +420,7 @@ def cached_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
         slopes = _vector(slopes, hq, torch.float32, q.device, "cached_attention(slopes)")
     prefix_at, prefix_value, prefix = _prefix(prefix, b, q.device, "cached_attention")
     at, stride, value, n, count = _lengths(cache_len, count, b, t, slots, q.device, "cached_attention")
-    out = torch.empty((b, t, hq, d), dtype=q.dtype, device=q.device)
+    out = q.new_empty((b, t, hq, d))
     qs, ks, vs, os_ = q.stride(), k_cache.stride(), v_cache.stride(), out.stride()
     args = _ATTENTION.pack(_ATTENTION.size, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), 0,
                            slopes.data_ptr() if slopes is not None else 0, prefix_at, 0, at, n, b, t, slots, hq, hk, d, qs[0], qs[1], qs[2],
