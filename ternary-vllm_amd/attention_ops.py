@@ -262,8 +262,9 @@ def rotary_cache(qkv: torch.Tensor, table: torch.Tensor, k_cache: torch.Tensor, 
     if heads < 0 or width < (heads + 2 * hk) * d:
         raise ValueError(f"rotary_cache: rows of {width} channels do not hold {heads} query and 2 x {hk} key / value heads of {d}")
     _check_cache(k_cache, v_cache, qkv, b, d, "rotary_cache", True)
-    if k_cache.data_ptr() == v_cache.data_ptr() and k_cache.numel():
-        raise ValueError("rotary_cache: k_cache and v_cache are the same memory")
+    ka, va = k_cache.data_ptr(), v_cache.data_ptr()
+    if k_cache.numel() and (ka == va or (abs(ka - va) < k_cache.nbytes and k_cache.is_contiguous() and v_cache.is_contiguous())):
+        raise ValueError("rotary_cache: k_cache and v_cache share memory")
     _check_table(table, d, qkv.device, "rotary_cache")
     at, stride, value, n, count = _lengths(cache_len, count, b, t, slots, qkv.device, "rotary_cache")
     q = qkv.new_empty((b, t, heads, d))

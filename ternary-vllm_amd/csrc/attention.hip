@@ -41,13 +41,20 @@ static int check(const tvl_attention_args* a, const char* who, bool cached) {
     TVL_REQUIRE(a->keys == 0 || (a->k && a->v), "%s: NULL key or value pointer", who);
     TVL_REQUIRE(aligned(a->q, z) && aligned(a->k, z) && aligned(a->v, z) && aligned(a->out, z) && aligned(a->lse, 4) && aligned(a->slopes, 4) && aligned(a->prefix, 8) &&
                     aligned(a->documents, 8) && aligned(a->cache_len, 8) && aligned(a->count, 8), "%s: misaligned pointer", who);
+    TVL_REQUIRE(a->q_token >= 0 && a->k_token >= 0 && a->v_token >= 0, "%s: negative token stride", who);      // lane offsets inside a tile are unsigned
     TVL_REQUIRE(rows_apart(a->dim, a->batch, a->o_batch, a->queries, a->o_token, a->heads, a->o_head), "%s: rows of the output overlap", who);
     return TVL_OK;
 }
 
+// whether the sizes of a block make sense: a caller asks for its workspace before any entry point has checked them
+static bool sized(const tvl_attention_args* a) {
+    return a && a->struct_bytes == sizeof(tvl_attention_args) && a->batch > 0 && a->queries >= 0 && a->keys >= 0 && a->heads > 0 && a->kv_heads > 0 && a->heads % a->kv_heads == 0 &&
+           a->dim >= 1 && a->dim <= ATTENTION_MAX_DIM;
+}
+
 // parts of a workspace, each a multiple of 256 bytes
 static size_t round256(size_t v) { return (v + 255) & ~size_t(255); }
-static bool any_rows(const tvl_attention_args& a) { return a.batch > 0 && a.heads > 0 && a.queries > 0; }
+static bool any_rows(const tvl_attention_args& a) { return a.queries > 0; }
 static size_t span_bytes(const tvl_attention_args& a) {
     return a.documents && any_rows(a) ? round256((size_t)a.batch * (size_t)ceil_div(a.queries, SPAN) * sizeof(DocumentSpan)) : 0;
 }
@@ -57,7 +64,7 @@ static size_t maxima_bytes(const tvl_attention_args& a) {
 }
 
 static size_t slab_bytes(const tvl_attention_args& a) {
-    if (!any_rows(a) || a.keys <= 0 || a.kv_heads <= 0) return 0;
+    if (!any_rows(a) || a.keys == 0) return 0;
     const int parts = attention_backward_parts(a);
     return parts > 1 ? (size_t)parts * 2 * a.batch * a.keys * a.kv_heads * a.dim * 4 : 0;
 }
@@ -73,7 +80,7 @@ using namespace tvl;
 
 extern "C" {
 
-size_t tvl_attention_workspace_bytes(const tvl_attention_args* a) { return a ? span_bytes(*a) : 0; }
+size_t tvl_attention_workspace_bytes(const tvl_attention_args* a) { return sized(a) ? span_bytes(*a) : 0; }
 
 int tvl_attention(const tvl_attention_args* a, void* workspace, size_t workspace_bytes, void* stream) {
     if (const int rc = check(a, "attention", false); rc != TVL_OK) return rc;
@@ -87,7 +94,7 @@ int tvl_attention(const tvl_attention_args* a, void* workspace, size_t workspace
 }
 
 size_t tvl_attention_backward_workspace_bytes(const tvl_attention_args* a) {
-    return a ? span_bytes(*a) + delta_bytes(*a) + maxima_bytes(*a) + slab_bytes(*a) : 0;
+    return sized(a) ? span_bytes(*a) + delta_bytes(*a) + maxima_bytes(*a) + slab_bytes(*a) : 0;
 }
 
 int tvl_attention_backward(const tvl_attention_args* a, const tvl_attention_grads* g, void* workspace, size_t workspace_bytes, void* stream) {
@@ -96,6 +103,7 @@ int tvl_attention_backward(const tvl_attention_args* a, const tvl_attention_grad
     if (a->batch == 0 || (a->queries == 0 && a->keys == 0)) return TVL_OK;
     const size_t z = dtype_size(a->dtype);
     TVL_REQUIRE(a->queries == 0 || (a->lse && g->grad_out), "attention_backward: NULL lse or grad_out pointer");
+    TVL_REQUIRE(g->g_token >= 0, "attention_backward: negative token stride");
     TVL_REQUIRE((g->dk != nullptr) == (g->dv != nullptr), "attention_backward: dk and dv go together");
     TVL_REQUIRE(aligned(g->grad_out, z) && aligned(g->dq, z) && aligned(g->dk, z) && aligned(g->dv, z), "attention_backward: misaligned pointer");
     if (const int rc = check_workspace("attention_backward", tvl_attention_backward_workspace_bytes(a), workspace, workspace_bytes); rc != TVL_OK) return rc;
@@ -111,7 +119,7 @@ int tvl_attention_backward(const tvl_attention_args* a, const tvl_attention_grad
 }
 
 size_t tvl_cached_attention_workspace_bytes(const tvl_attention_args* a) {
-    return a && any_rows(*a) && a->kv_heads > 0 && attention_step_serves(*a) ? round256(attention_step_bytes(*a)) : 0;
+    return sized(a) && any_rows(*a) && attention_step_serves(*a) ? round256(attention_step_bytes(*a)) : 0;
 }
 
 int tvl_cached_attention(const tvl_attention_args* a, void* workspace, size_t workspace_bytes, void* stream) {

@@ -182,7 +182,7 @@ int tvl_rotary_cache(const tvl_rotary_cache_args* a, void* stream) {
     TVL_REQUIRE(a->ld_table >= a->rotary_dim, "rotary_cache: table rows hold %lld values, rotary_dim=%lld", (long long)a->ld_table, (long long)a->rotary_dim);
     if (a->batch == 0 || a->tokens == 0 || a->heads + a->kv_heads == 0 || a->dim == 0) return TVL_OK;
     TVL_REQUIRE(a->batch <= (1 << 30), "rotary_cache: batch too large");
-    TVL_REQUIRE(a->qkv && a->q && (a->table || a->table_rows == 0 || a->rotary_dim == 0) && ((a->k_cache && a->v_cache) || a->slots == 0 || a->kv_heads == 0), "rotary_cache: NULL pointer");
+    TVL_REQUIRE(a->qkv && (a->q || a->heads == 0) && (a->table || a->table_rows == 0 || a->rotary_dim == 0) && ((a->k_cache && a->v_cache) || a->slots == 0 || a->kv_heads == 0), "rotary_cache: NULL pointer");
     const size_t z = dtype_size(a->dtype);
     TVL_REQUIRE(aligned(a->qkv, z) && aligned(a->q, z) && aligned(a->k_cache, z) && aligned(a->v_cache, z) && aligned(a->table, 4) && aligned(a->cache_len, 8) &&
                     aligned(a->count, 8), "rotary_cache: misaligned pointer");

@@ -62,6 +62,25 @@ def test_attention_refuses_missing_blocks_and_workspace():
     assert lib.tvl_attention_backward(attention_args(batch=0), grads_args(), None, 0, None) == 0
 
 
+@pytest.mark.parametrize("kw", [dict(heads=1), dict(heads=3), dict(heads=0), dict(kv_heads=0), dict(kv_heads=-1), dict(batch=-1), dict(queries=-1), dict(keys=-1), dict(dim=0), dict(dim=-1),
+                                dict(size=8)])
+def test_workspaces_of_sizes_that_make_no_sense(kw):
+    """A caller asks for a workspace before any check: no division by zero, no size, and the call itself is refused."""
+    a = attention_args(documents=P, **kw)
+    for name in ("attention", "attention_backward", "cached_attention"):
+        assert getattr(lib, f"tvl_{name}_workspace_bytes")(a) == 0
+        assert getattr(lib, f"tvl_{name}_workspace_bytes")(None) == 0
+    assert lib.tvl_attention(a, None, 0, None) == 1 and lib.tvl_cached_attention(a, None, 0, None) == 1
+
+
+@pytest.mark.parametrize("name", ["q_token", "k_token", "v_token"])
+def test_negative_token_strides_are_refused(name):
+    a = attention_args(**{name: -64})
+    for call in (lambda: lib.tvl_attention(a, None, 0, None), lambda: lib.tvl_cached_attention(a, None, 0, None), lambda: lib.tvl_attention_backward(a, grads_args(), P, 1 << 40, None)):
+        assert call() == 1 and b"stride" in lib.tvl_last_error()
+    assert lib.tvl_attention_backward(attention_args(), grads_args(g_token=-64), P, 1 << 40, None) == 1 and b"stride" in lib.tvl_last_error()
+
+
 def rotary_args(**kw):
     f = dict(size=A._ROTARY.size, x=P, y=P, positions=P, table=P, batch=2, tokens=3, heads=4, dim=64, rotary_dim=32, table_rows=16, ld_table=32,
              x_batch=0, x_token=0, x_head=0, y_batch=0, y_token=0, y_head=0, pos_batch=0, pos_token=0, dtype=1, interleaved=0, inverse=0, reserved=0)

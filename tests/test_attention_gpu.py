@@ -161,6 +161,27 @@ def test_rotary_cache_positions_outside_and_refusals(tv, dev):
             call()
 
 
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+def test_rotary_cache_without_query_heads(tv, dev, kind):
+    """Keys and values alone: the caches get what they get beside query heads."""
+    g = torch.Generator().manual_seed(5)
+    qkv = normal(g, 2, 3, 8 * 16, dtype=TYPES[kind]).to(dev)
+    table = tv.rotary_table(16, 9, device=dev)
+    k, v, k1, v1 = (torch.zeros(2, 2, 9, 16, dtype=TYPES[kind], device=dev) for _ in range(4))
+    tv.rotary_cache(qkv, table, k, v, 4, 4)
+    q = tv.rotary_cache(qkv[..., 4 * 16:], table, k1, v1, 4, 0)
+    assert q.shape == (2, 3, 0, 16) and torch.equal(k, k1) and torch.equal(v, v1) and torch.equal(v1[:, :, 4:7], qkv[..., 6 * 16:].unflatten(2, (2, 16)).transpose(1, 2))
+
+
+def test_rotary_cache_refuses_caches_that_share_memory(tv, dev):
+    table, qkv, kv = tv.rotary_table(16, 9, device=dev), torch.zeros(2, 3, 8 * 16, device=dev), torch.zeros(3, 2, 9, 16, device=dev)
+    for k, v in ((kv[:2], kv[:2]), (kv[:2], kv[1:]), (kv[1:], kv[:2])):
+        with pytest.raises(ValueError, match="share"):
+            tv.rotary_cache(qkv, table, k, v, 0, 4)
+    both = torch.zeros(2, 2, 2, 9, 16, device=dev)      # side by side in one tensor: fine
+    tv.rotary_cache(qkv, table, both[:, 0], both[:, 1], 0, 4)
+
+
 # ---------------------------------------------------------------------------------------------------------- attention
 
 def run_case(tv, dev, kind, b, tq, tk, hq, hk, d, causal=False, prefix=None, documents=None, softcap=0.0, slopes=False, scale=None, seed=0, gscale=0.02, qscale=1.0):
