@@ -1,6 +1,8 @@
 // Backward attention: delta = rowsum(out * grad_out), then dq per query tile and dk, dv per key tile.  The scores are formed again from
-// q, k and the saved log-sum, twice (14 instead of 10 products per pair, head and element): every gradient is then summed in
+// q, k and the saved log-sum, twice (14 instead of 10 operations per pair, head and element): every gradient is then summed in
 // the registers of one workgroup, in a fixed order, without atomics.
+// GPU times below: A = 4 x 2048 causal tokens, 32 heads of 64, bf16; B = 8191 tokens in 7 documents, 16 / 4 heads of 128, capped, bf16; C = 128 x 197 tokens,
+// 12 heads of 64, f16.
 #include "attention_tiles.h"
 
 #include <type_traits>
@@ -13,13 +15,12 @@ constexpr int PIECE = 32; // of them at a time
 template <int R> constexpr int VALUES = PIECE * R / 64;
 template <int R> __device__ __forceinline__ constexpr int piece_row(int x) { return x / REGS<R> * R + result_row<R>(x % REGS<R>, 0); }
 
-// Shape of a gradient kernel: W waves of R queries or keys each, 128 in all; waves per SIMD its registers are limited to.
-template <typename T, int DP, bool QUERIES> struct Shape {
-#ifndef XR
-#define XR (DP == 64 && sizeof(T) == 2 ? 32 : 16)
-#define XO 2
-#endif
-    static constexpr int R = XR, W = 128 / R, OCCUPANCY = XO;
+// Shape of a gradient kernel: W waves of R queries or keys each, 128 in all, its registers limited to OCCUPANCY waves per SIMD.  16-bit heads of 64
+// fit two waves per SIMD at R = 32, whose products read LDS half as often: the pass over 4 x 2048 causal tokens, 32 heads, bf16, takes 519 us, at R = 16
+// 659.  Longer rows and float32 fit them at R = 16 only: 8192 tokens, 16 heads of 128, f16 2613 us, at R = 32 with one wave 2862; float32 (2 x 1024 causal,
+// 8 heads) of 64 260 against 287, of 128 490 against 581.  Four waves per SIMD spill: 6571.
+template <typename T, int DP> struct Shape {
+    static constexpr int R = DP == 64 && sizeof(T) == 2 ? 32 : 16, W = 128 / R, OCCUPANCY = 2;
 };
 
 // power of two that brings float16 score gradients into the type's range: near the largest output gradient, in steps of 2^8 so that it
@@ -32,7 +33,8 @@ __device__ __forceinline__ int range_exponent(float top) {
 }
 __device__ __forceinline__ float power_of_two(int e) { return __builtin_bit_cast(float, (uint32_t)(e + 127) << 23); }
 
-// delta[row] and, for float16, the largest finite |grad_out| of every 64 rows.  16 lanes per row, 16 bytes each: bound by HBM.
+// delta[row] and, for float16, the largest finite |grad_out| of every 64 rows.  16 lanes per row, 16 bytes each: one read of both
+// tensors, bound by HBM (A: 12 us, 5.6 TB/s; B: 11.7; C: 20 us, 3.9 TB/s).
 template <typename T, bool WIDE>
 __global__ void __launch_bounds__(256) attention_delta_kernel(tvl_attention_args a, tvl_attention_grads gr, float* __restrict__ delta, float* __restrict__ maxima, int blocks) {
     constexpr int PER = 16 / (int)sizeof(T);
@@ -69,12 +71,14 @@ __global__ void __launch_bounds__(256) attention_delta_kernel(tvl_attention_args
     }
 }
 
-// dq.  4 waves x 32 queries; per 32 keys: S^T = K Q^T, dP^T = V dO^T, dS^T = P (dP - delta) bend (a lane holds one query), dQ^T += K^T dS^T.
+// dq.  W waves x R queries; per 32 keys: S^T = K Q^T, dP^T = V dO^T, dS^T = P (dP - delta) bend (a lane holds one query), dQ^T += K^T dS^T.  Six operations per
+// pair and element.  A: 201 us (513 TFLOP/s), B: 386, C: 107.  The matrix cores are busy 39 % of the time at heads of 64 and 26 %
+// at 128: exponentials and conversions on the vector ALU and the operands' way out of LDS (no bank conflicts left) wait for each other with two waves per SIMD.
 template <typename T, int DP, Form FORM>
-__global__ void __launch_bounds__((64 * Shape<T, DP, true>::W), (Shape<T, DP, true>::OCCUPANCY)) attention_dq_kernel(tvl_attention_args a, tvl_attention_grads gr, const DocumentSpan* __restrict__ spans, const float* __restrict__ delta,
+__global__ void __launch_bounds__((64 * Shape<T, DP>::W), (Shape<T, DP>::OCCUPANCY)) attention_dq_kernel(tvl_attention_args a, tvl_attention_grads gr, const DocumentSpan* __restrict__ spans, const float* __restrict__ delta,
                                                            int tiles) {
     constexpr bool WIDE = FORM != ODD;
-    constexpr int R = Shape<T, DP, true>::R, THREADS = 64 * Shape<T, DP, true>::W, QB = 128, CK = CHUNK<R>, N = VALUES<R>;
+    constexpr int R = Shape<T, DP>::R, THREADS = 64 * Shape<T, DP>::W, QB = 128, CK = CHUNK<R>, N = VALUES<R>;
     typedef Tile<T, DP> L;
     typedef typename Operand<T>::elem E;
     extern __shared__ __align__(16) char lds[];
@@ -255,13 +259,14 @@ __global__ void __launch_bounds__((64 * Shape<T, DP, true>::W), (Shape<T, DP, tr
         }
 }
 
-// dk, dv.  4 waves x 32 keys; over the heads that share them and tiles of 64 queries: S = Q K^T, dP = dO V^T (a lane holds one key, K and V stay in
-// registers), dV^T += dO^T P, dK^T += Q^T dS.
+// dk, dv.  W waves x R keys; over the heads that share them and tiles of 64 queries: S = Q K^T, dP = dO V^T (a lane holds one key, K and V stay in
+// registers), dV^T += dO^T P, dK^T += Q^T dS.  Eight operations per pair and element.  A: 290 us (474 TFLOP/s), C: 180, B: 947 with a group's heads in one workgroup;
+// bound as dq is, matrix cores busy 31 % and 22 %.
 template <typename T, int DP, Form FORM>
-__global__ void __launch_bounds__((64 * Shape<T, DP, false>::W), (Shape<T, DP, false>::OCCUPANCY)) attention_dkv_kernel(tvl_attention_args a, tvl_attention_grads gr, const DocumentSpan* __restrict__ spans, const float* __restrict__ delta,
+__global__ void __launch_bounds__((64 * Shape<T, DP>::W), (Shape<T, DP>::OCCUPANCY)) attention_dkv_kernel(tvl_attention_args a, tvl_attention_grads gr, const DocumentSpan* __restrict__ spans, const float* __restrict__ delta,
                                                             const float* __restrict__ maxima, int tiles, int parts, float* __restrict__ slabs) {
     constexpr bool WIDE = FORM != ODD;
-    constexpr int R = Shape<T, DP, false>::R, THREADS = 64 * Shape<T, DP, false>::W, KB = 128, CK = CHUNK<R>, N = VALUES<R>;
+    constexpr int R = Shape<T, DP>::R, THREADS = 64 * Shape<T, DP>::W, KB = 128, CK = CHUNK<R>, N = VALUES<R>;
     typedef Tile<T, DP> L;
     typedef typename Operand<T>::elem E;
     extern __shared__ __align__(16) char lds[];
@@ -503,8 +508,9 @@ __global__ void __launch_bounds__(256) attention_gather_kernel(const float* __re
 }
 
 // Parts of a group's heads: a key tile whose workgroup takes all heads in turn is the longest chain of the pass, so where the key tiles alone do not
-// give two workgroups per compute unit the heads are divided (float32 sums through memory, added in order by a second launch).  8191 tokens in
-// documents, 16 / 4 heads of 128, one part: 947 us, of which the 45 tiles x 4 heads of the longest document's first keys are the chain.
+// give two workgroups per compute unit the heads are divided (float32 sums through memory, added in order by a second launch).  B in one part: 947 us, of
+// which the 45 tiles x 4 heads of the longest document's first keys are the chain; in two parts the chain is half as long and 67 MB of sums, written once and read
+// once, are 27 us.  The division itself has not been timed.
 int attention_backward_parts(const tvl_attention_args& a) {
     if (a.queries == 0) return 1;      // sums of nothing: no workspace either
     const int64_t tiles = a.batch * a.kv_heads * ceil_div(a.keys, 128);
@@ -520,14 +526,14 @@ static int launch_gradients(const tvl_attention_args& a, const tvl_attention_gra
         const int tiles = (int)ceil_div(a.queries, 128);
         const size_t bytes = 4 * GT * (size_t)Tile<T, DP>::ROW + (FORM == PLAIN ? 0 : 2 * GT * 8);
         if (bytes > 65536) TVL_HIP_CHECK(hipFuncSetAttribute((const void*)attention_dq_kernel<T, DP, FORM>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
-        hipLaunchKernelGGL((attention_dq_kernel<T, DP, FORM>), dim3((unsigned)(a.batch * a.heads * tiles)), dim3(64 * Shape<T, DP, true>::W), bytes, st, a, g, spans, delta, tiles);
+        hipLaunchKernelGGL((attention_dq_kernel<T, DP, FORM>), dim3((unsigned)(a.batch * a.heads * tiles)), dim3(64 * Shape<T, DP>::W), bytes, st, a, g, spans, delta, tiles);
         TVL_LAUNCH_CHECK();
     }
     if (g.dk && a.keys > 0) {
         const int tiles = (int)ceil_div(a.keys, 128), parts = attention_backward_parts(a);
         const size_t bytes = 2 * (2 * GT * (size_t)Tile<T, DP>::ROW + 2 * GT * 4 + (FORM == PLAIN ? 0 : GT * 8));
         if (bytes > 65536) TVL_HIP_CHECK(hipFuncSetAttribute((const void*)attention_dkv_kernel<T, DP, FORM>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
-        hipLaunchKernelGGL((attention_dkv_kernel<T, DP, FORM>), dim3((unsigned)(a.batch * a.kv_heads * tiles * parts)), dim3(64 * Shape<T, DP, false>::W), bytes, st, a, g, spans, delta, maxima,
+        hipLaunchKernelGGL((attention_dkv_kernel<T, DP, FORM>), dim3((unsigned)(a.batch * a.kv_heads * tiles * parts)), dim3(64 * Shape<T, DP>::W), bytes, st, a, g, spans, delta, maxima,
                            tiles, parts, slabs);
         TVL_LAUNCH_CHECK();
         if (parts > 1) {

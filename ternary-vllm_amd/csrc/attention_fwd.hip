@@ -6,10 +6,14 @@
 namespace tvl {
 
 // One workgroup: 4 waves x 32 queries of one head; keys and values come in tiles of 64 through LDS, two buffers, the next tile's loads in
-// flight while this one is used.  Per wave and tile: S^T = K Q^T (a lane holds 32 scores of ONE query: maximum and sum are plain loops
+// flight while this one is used: its keys during the scores, its values during the rest, through one set of registers (two sets spill at heads of 128).  Per wave and tile: S^T = K Q^T (a lane holds 32 scores of ONE query: maximum and sum are plain loops
 // over its registers plus one exchange with the other half), weights 2^(s - m) rounded to the operands' type as the second product's operand,
 // O^T += V^T P^T.  m is kept until a score exceeds it by 8 (in powers of two): the weights stay below 2^8, exact in float32 sums, and the
-// accumulator is almost never rescaled.
+// accumulator is almost never rescaled.  Tiles that every query sees whole run in a loop without masks.
+// Heads of 128: 8192 x 8192, 16 heads, f16 697 us (790 TFLOP/s), causal bf16 16 / 4 heads 351 us (780), capped 568; heads of 64: 4 x 2048, 32 heads, bf16
+// 207 us (660 TFLOP/s), causal 148-157 us (440-465), 128 x 197, 12 heads, f16 62 us (246).  A score costs an exponential and about four other vector instructions
+// whatever the head's length, so heads of 64 are bound by the vector ALU; heads of 128 reach 70 % of the rate of a large library product.  One set of registers
+// instead of two, and banks without conflicts, took them from 883 to 697 us.
 template <typename T, int DP, bool CACHED, Form FORM>
 __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attention_forward_kernel(tvl_attention_args a, const DocumentSpan* __restrict__ spans, int tiles) {
     constexpr bool WIDE = FORM != ODD;
@@ -220,7 +224,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attention_forward
     if (!CACHED && a.lse && g == 0) a.lse[((int64_t)b * a.heads + h) * queries + i] = sum == 0.0f ? -__builtin_inff() : (base + __builtin_amdgcn_logf(sum)) * LN2;
 }
 
-// spans[b][n] of tokens 64 n .. 64 n + 63
+// spans[b][n] of tokens 64 n .. 64 n + 63: 64 KB for 8191 tokens, bound by the launch (4.9 us)
 __global__ void __launch_bounds__(64) document_spans_kernel(const int64_t* __restrict__ documents, int64_t stride, int tokens, int blocks, DocumentSpan* __restrict__ spans) {
     const int b = blockIdx.x / blocks, n = blockIdx.x % blocks, i = n * SPAN + threadIdx.x;
     const int64_t doc = documents[b * stride + (i < tokens ? i : n * SPAN)];

