@@ -94,8 +94,9 @@ class Attention:
         e_delta = (G.abs() * (self.out_tol + u * self.out.abs())).sum(-1, keepdim=True) + (d + 4) * F32 * (G.abs() * self.out.abs()).sum(-1, keepdim=True)
         raw = p * (dp - delta).abs()
         e = (e_p + u * 1.01) * core.abs() + p * (e_dp + e_delta) + 2.0 ** -19 * raw + 8 * F32 * p * (dp.abs() + delta.abs())
-        # float16 score gradients are rounded relative to the largest gradient: half the smallest step of that scale
-        e = e + self.step * 4 * G.abs().amax() * self.see[:, None].double()
+        # float16 score gradients are rounded as multiples of 2^m: half the smallest step there is 2^-25 2^m.  m is a multiple of 8 with top / 2^m in
+        # [2^-4, 2^4) for the largest output gradient top that the workgroup looks at, so 2^m <= 16 top <= 16 max |G|
+        e = e + self.step * 16 * G.abs().amax() * self.see[:, None].double()
         e = e * abs(self.scale)
         dq = ds @ K
         dq_tol = e @ K.abs() + u * dq.abs() + self.step + (tk + 16) * F32 * (ds.abs() @ K.abs()) + 1e-30
