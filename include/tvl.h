@@ -211,8 +211,9 @@ int tvl_ternary_mm_f32(const float* x, int64_t m, int64_t k, int64_t ld_x, const
 /* The reference evaluates these steps as separate tensor operations (impl/tf/moondream/layers.py:244-268 rotation and cache,
  * impl/tf/attention.py:87-105 mask, the softmax after it).  Every argument block is a HOST structure that is read before the
  * call returns; the pointers inside it are device pointers.  `struct_bytes` is sizeof the structure as the caller knows it.
- * Strides are in elements; the last dimension (the elements of a head) is dense.  All of f32 / f16 / bf16; every sum,
- * maximum and angle is held in float32, each result rounded once to its type. */
+ * Strides are in elements; the last dimension (the elements of a head) is dense.  What a call writes overlaps nothing else that it
+ * reads or writes, except where said.  All of f32 / f16 / bf16; every sum, maximum and angle is held in float32, each result rounded
+ * once to its type. */
 
 /* Rotary positions.  y[b,t,h,:] = x[b,t,h,:] with the first `rotary_dim` elements of every head turned by its token's angles;
  * the remaining elements are copied.  Pair i of a head is elements (i, i + rotary_dim/2), or (2i, 2i+1) when `interleaved`:
@@ -222,7 +223,7 @@ int tvl_ternary_mm_f32(const float* x, int64_t m, int64_t k, int64_t ld_x, const
 typedef struct tvl_rotary_args {
     uint64_t struct_bytes;
     const void* x;             /* [batch, tokens, heads, dim] */
-    void* y;                   /* the same shape; may be x itself */
+    void* y;                   /* the same shape; may be x itself with x's strides */
     const int64_t* positions;  /* element (b, t) at b * pos_batch + t * pos_token */
     const float* table;        /* [table_rows, ld_table >= rotary_dim] */
     int64_t batch, tokens, heads, dim, rotary_dim, table_rows, ld_table;
@@ -239,7 +240,7 @@ int tvl_rotary(const tvl_rotary_args* args, void* stream);
 typedef struct tvl_rotary_cache_args {
     uint64_t struct_bytes;
     const void* qkv;            /* [batch, tokens, (heads + 2 kv_heads) * dim] */
-    void* q;                    /* [batch, tokens, heads, dim], dense */
+    void* q;                    /* [batch, tokens, heads, dim], dense; not read or written (NULL) with 0 heads */
     void* k_cache;              /* [batch, kv_heads, slots, dim] */
     void* v_cache;
     const float* table;         /* [table_rows, ld_table >= rotary_dim] */
@@ -262,7 +263,8 @@ int tvl_rotary_cache(const tvl_rotary_cache_args* args, void* stream);
  *
  * tvl_cached_attention: k and v are caches of `keys` slots.  Query i of sequence b sits at p_i = cache_len[b] + i; count[b] of
  * the queries are real (rows beyond give zeros); the cache holds cache_len[b] + count[b] keys, and query i sees key j of
- * them if j <= p_i or j < prefix.  A query whose place is negative or beyond the cache gives NaN.  `causal`, `documents`, `lse` unused. */
+ * them if j <= p_i or j < prefix.  A query whose place is negative or beyond the cache gives NaN.  `causal`, `documents`, `lse` unused.
+ * Token strides are not negative; rows of the output are apart from each other. */
 typedef struct tvl_attention_args {
     uint64_t struct_bytes;
     const void* q;              /* [batch, queries, heads, dim] */
@@ -291,8 +293,8 @@ typedef struct tvl_attention_grads {
     void* dv;
     int64_t g_batch, g_token, g_head;
 } tvl_attention_grads;
-/* `workspace`: tvl_*_workspace_bytes(args) bytes of device memory (256-byte aligned; 0 = none needed); contents need no
- * initialisation and are not preserved. */
+/* `workspace`: tvl_*_workspace_bytes(args) bytes of device memory (256-byte aligned; 0 = none needed, or sizes that the call refuses);
+ * contents need no initialisation and are not preserved. */
 int tvl_attention(const tvl_attention_args* args, void* workspace, size_t workspace_bytes, void* stream);
 size_t tvl_attention_workspace_bytes(const tvl_attention_args* args);
 int tvl_attention_backward(const tvl_attention_args* args, const tvl_attention_grads* grads, void* workspace, size_t workspace_bytes, void* stream);
