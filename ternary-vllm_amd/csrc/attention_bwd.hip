@@ -216,7 +216,7 @@ __global__ void __launch_bounds__((64 * Shape<T, DP>::W), (Shape<T, DP>::OCCUPAN
             // score gradients are rounded to the operands' type for the last product; its sum is float32
 #pragma unroll
             for (int x = 0; x < N; ++x) df[x / 8][x % 8] = (E)dp[x];
-            if (MASKED && (!one_document || (jt + PIECE > wall && wall < wreach)) && holds_not_finite<T, DP, PIECE>(kt + t * L::ROW, lane)) {
+            if (MASKED && (!one_document || (jt + PIECE > wall && wall < seq.end)) && holds_not_finite<T, DP, PIECE>(kt + t * L::ROW, lane)) {
 #pragma unroll
                 for (int c = 0; c < PIECE / CK; ++c)
 #pragma unroll

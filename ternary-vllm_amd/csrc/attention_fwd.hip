@@ -171,8 +171,8 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attention_forward
                     // weights are rounded to the operands' type for the second product (relative 2^-11 / 2^-8 each, the sum stays float32)
                     pf[(t * REGS<R> + x) / 8][x % 8] = (typename Operand<T>::elem)w;
                 }
-            // queries of the wave that see different keys of this tile: an infinity or NaN in a value must not reach the others
-            if (MASKED && (!one_document || (j0 + KT > wall && wall < wreach)) && holds_not_finite<T, DP, KT>(vt, lane)) {
+            // keys of this tile that some query of the wave does not see (a prefix may end here for all of them): an infinity or NaN in their values must not reach it
+            if (MASKED && (!one_document || (j0 + KT > wall && wall < seq.end)) && holds_not_finite<T, DP, KT>(vt, lane)) {
 #pragma unroll
                 for (int c = 0; c < KT / CK; ++c)
 #pragma unroll

@@ -371,6 +371,29 @@ def test_attention_infinities_and_nan_behind_a_mask_stay_there(tv, dev, kind, ba
     assert torch.equal(got[0][:, :-1], want[0][:, :-1])
 
 
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_attention_infinities_behind_a_prefix_that_ends_inside_a_tile(tv, dev, kind, bad):
+    """Queries that all see the same prefix, with spoiled keys behind it in the same tile: they keep their bits, results and gradients."""
+    g = torch.Generator().manual_seed(37)
+    for d, t, prefix, at in ((64, 190, 70, 100), (128, 190, 70, 71), (64, 330, 230, 240)):
+        clean = [normal(g, 2, t, h, d, dtype=TYPES[kind]) for h in (4, 2, 2, 4)]
+        results = []
+        for spoil in (False, True):
+            x = [y.clone() for y in clean]
+            if spoil:
+                x[1][:, at:] = bad
+                x[2][:, at:] = bad
+            leaves = [y.to(dev).requires_grad_(True) for y in x[:3]]
+            out = tv.attention(*leaves, causal=True, prefix=prefix)
+            (dq,) = torch.autograd.grad(out, leaves[0], x[3].to(dev))
+            with torch.no_grad():
+                cached = tv.cached_attention(leaves[0], *(y.transpose(1, 2).contiguous() for y in leaves[1:]), 0, prefix=prefix)
+            results.append([out[:, :at], dq[:, :at], cached[:, :at]])
+        for x, y, name in zip(*results, ("out", "dq", "cached")):
+            assert torch.equal(x, y), (name, d)
+
+
 def test_attention_visible_infinities_show(tv, dev):
     """A value of +-infinity that a query sees gives that infinity (NaN for both signs), at its element alone."""
     q, k, v = (torch.randn(1, 40, 1, 64, device=dev) for _ in range(3))
