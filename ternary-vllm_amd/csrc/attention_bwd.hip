@@ -17,8 +17,8 @@ template <int R> __device__ __forceinline__ constexpr int piece_row(int x) { ret
 
 // Shape of a gradient kernel: W waves of R queries or keys each, 128 in all, its registers limited to OCCUPANCY waves per SIMD.  16-bit heads of 64
 // fit two waves per SIMD at R = 32, whose products read LDS half as often: the pass over 4 x 2048 causal tokens, 32 heads, bf16, takes 519 us, at R = 16
-// 659.  Longer rows and float32 fit them at R = 16 only: 8192 tokens, 16 heads of 128, f16 2613 us, at R = 32 with one wave 2862; float32 (2 x 1024 causal,
-// 8 heads) of 64 260 against 287, of 128 490 against 581.  Four waves per SIMD spill: 6571.
+// 659.  Longer rows and float32 fit them (but for a few registers) at R = 16 only: 8192 tokens, 16 heads of 128, f16 2613 us, at R = 32 with one wave
+// 2862; float32 (2 x 1024 causal, 8 heads) of 64 260 against 287, of 128 490 against 581.  Four waves per SIMD spill: 6571.
 template <typename T, int DP> struct Shape {
     static constexpr int R = DP == 64 && sizeof(T) == 2 ? 32 : 16, W = 128 / R, OCCUPANCY = 2;
 };
