@@ -664,6 +664,13 @@ gemm_mfma16_kernel(const TX* __restrict__ x, int m, int k, int64_t ld_x, const u
         }
     };
 
+    // One row group of an epilogue with an activation at a time: without the fence the compiler (no packed float32 instructions) starts the
+    // exponentials of all of them and keeps what they left in scratch memory, 17 to 311 registers by form.
+    auto row_fence = [&](int i, int tp) __attribute__((always_inline)) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) asm volatile("" : "+v"(acc[i][tp + t]));
+    };
+
     auto store_tile_full = [&]() __attribute__((always_inline)) {
         if constexpr (sizeof(TY) == 2 && !SPLIT) {
         const float cl = fabsf(clip);
@@ -694,6 +701,7 @@ gemm_mfma16_kernel(const TX* __restrict__ x, int m, int k, int64_t ld_x, const u
                 constexpr bool CLIP16 = std::is_same<TY, f16>::value && MODE == 0;
     #pragma unroll
                 for (int i = 0; i < MT; ++i) {
+                    if constexpr (ACT != TVL_ACT_NONE) row_fence(i, tp);
                     uint2 pk[2];
     #pragma unroll
                     for (int t = 0; t < 2; ++t) {
@@ -761,6 +769,7 @@ gemm_mfma16_kernel(const TX* __restrict__ x, int m, int k, int64_t ld_x, const u
                 }
     #pragma unroll
             for (int i = 0; i < MT; ++i) {
+                if constexpr (ACT != TVL_ACT_NONE) row_fence(i, tp);
                 const int gm = m0 + wr * WM + 16 * i + c;
                 float v[2][4];
     #pragma unroll
