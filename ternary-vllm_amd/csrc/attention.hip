@@ -59,10 +59,6 @@ static size_t span_bytes(const tvl_attention_args& a) {
     return a.documents && any_rows(a) ? round256((size_t)a.batch * (size_t)ceil_div(a.queries, SPAN) * sizeof(DocumentSpan)) : 0;
 }
 static size_t delta_bytes(const tvl_attention_args& a) { return any_rows(a) ? round256((size_t)a.batch * a.heads * a.queries * 4) : 0; }
-static size_t maxima_bytes(const tvl_attention_args& a) {
-    return any_rows(a) && a.dtype == TVL_F16 ? round256((size_t)a.batch * a.heads * (size_t)ceil_div(a.queries, 64) * 4) : 0;
-}
-
 static size_t slab_bytes(const tvl_attention_args& a) {
     if (!any_rows(a) || a.keys == 0) return 0;
     const int parts = attention_backward_parts(a);
@@ -94,7 +90,7 @@ int tvl_attention(const tvl_attention_args* a, void* workspace, size_t workspace
 }
 
 size_t tvl_attention_backward_workspace_bytes(const tvl_attention_args* a) {
-    return sized(a) ? span_bytes(*a) + delta_bytes(*a) + maxima_bytes(*a) + slab_bytes(*a) : 0;
+    return sized(a) ? span_bytes(*a) + delta_bytes(*a) + slab_bytes(*a) : 0;
 }
 
 int tvl_attention_backward(const tvl_attention_args* a, const tvl_attention_grads* g, void* workspace, size_t workspace_bytes, void* stream) {
@@ -111,11 +107,10 @@ int tvl_attention_backward(const tvl_attention_args* a, const tvl_attention_grad
     char* at = static_cast<char*>(workspace);
     DocumentSpan* spans = a->documents ? reinterpret_cast<DocumentSpan*>(at) : nullptr;
     float* delta = reinterpret_cast<float*>(at + span_bytes(*a));
-    float* maxima = maxima_bytes(*a) ? reinterpret_cast<float*>(at + span_bytes(*a) + delta_bytes(*a)) : nullptr;
-    float* slabs = reinterpret_cast<float*>(at + span_bytes(*a) + delta_bytes(*a) + maxima_bytes(*a));
+    float* slabs = reinterpret_cast<float*>(at + span_bytes(*a) + delta_bytes(*a));
     if (spans)
         if (const int rc = launch_document_spans(*a, spans, st); rc != TVL_OK) return rc;
-    return launch_attention_backward(*a, *g, spans, delta, maxima, slabs, st);
+    return launch_attention_backward(*a, *g, spans, delta, slabs, st);
 }
 
 size_t tvl_cached_attention_workspace_bytes(const tvl_attention_args* a) {

@@ -23,24 +23,38 @@ template <typename T, int DP> struct Shape {
     static constexpr int R = DP == 64 && sizeof(T) == 2 ? 32 : 16, W = 128 / R, OCCUPANCY = 2;
 };
 
-// power of two that brings float16 score gradients into the type's range: near the largest output gradient, in steps of 2^8 so that it
-// rarely moves; float32 and bfloat16 need none
-__device__ __forceinline__ int range_exponent(float top) {
-    if (!(top > 0.0f)) return 0;
-    const int e = (int)((__builtin_bit_cast(uint32_t, top) >> 23) & 255) - 127;
-    const int m = ((e + 4) >> 3) * 8;
-    return m < -112 ? -112 : (m > 112 ? 112 : m);
+// float16 score gradients are multiplied by a power of two `fit` in front of their rounding, one for every column (a query of dq, a key of dk), which
+// follows the largest one of the column so far: it is chosen so that this one lies in [2^7, 2^8), kept until one exceeds 2^15, and the column's sum
+// is rescaled when it moves, as a softmax's maximum is.  Nothing overflows however large values and output gradients are, a gradient below 2^-21 of
+// its column's largest is off by at most 2^-32 of that one, and no column depends on what another one holds.  (A power of two for a whole
+// sequence, from its largest output gradient, made infinities of large values and zeros of the gradients of small documents beside large ones.)
+// What is not finite spoils its own column.
+template <typename T, int R, int N, int D>
+__device__ __forceinline__ void follow_range(const float (&ds)[N], Acc<R> (&acc)[D], float& fit) {
+    float top = 0.0f;
+#pragma unroll
+    for (int x = 0; x < N; ++x) top = fmaxf(top, fabsf(ds[x]));
+    top = column_max<R>(top);
+    const bool grow = top * fit > 32768.0f;
+    if (__any(grow)) {
+        // 2^(7 - exponent), not below 2^-100
+        const int e = (int)(__builtin_bit_cast(uint32_t, top) >> 23) - 127 - 7;
+        const float now = grow ? __builtin_bit_cast(float, (uint32_t)(127 - (e < 100 ? e : 100)) << 23) : fit;
+        const float shrink = now * __builtin_bit_cast(float, (254u << 23) - __builtin_bit_cast(uint32_t, fit));
+        fit = now;
+#pragma unroll
+        for (int d = 0; d < D; ++d) acc[d] *= shrink;
+    }
 }
-__device__ __forceinline__ float power_of_two(int e) { return __builtin_bit_cast(float, (uint32_t)(e + 127) << 23); }
+// before the first: whatever is not zero fits or moves it
+constexpr float FIT_START = 0x1p100f;
 
-// delta[row] and, for float16, the largest finite |grad_out| of every 64 rows.  16 lanes per row, 16 bytes each: one read of both
-// tensors, bound by HBM (A: 12 us, 5.6 TB/s; B: 11.7; C: 20 us, 3.9 TB/s).
+// delta[row].  16 lanes per row, 16 bytes each: one read of both tensors, bound by HBM (A: 12 us, 5.6 TB/s; B: 11.7; C: 20 us, 3.9 TB/s).
 template <typename T, bool WIDE>
-__global__ void __launch_bounds__(256) attention_delta_kernel(tvl_attention_args a, tvl_attention_grads gr, float* __restrict__ delta, float* __restrict__ maxima, int blocks) {
+__global__ void __launch_bounds__(256) attention_delta_kernel(tvl_attention_args a, tvl_attention_grads gr, float* __restrict__ delta, int blocks) {
     constexpr int PER = 16 / (int)sizeof(T);
     const int bh = blockIdx.x / blocks, n = blockIdx.x % blocks, h = bh % (int)a.heads, b = bh / (int)a.heads;
     const int lane = threadIdx.x % 16, row = threadIdx.x / 16, dim = (int)a.dim, queries = (int)a.queries;
-    float top = 0.0f;
 #pragma unroll
     for (int p = 0; p < GT / 16; ++p) {
         const int i = n * GT + p * 16 + row;
@@ -52,22 +66,11 @@ __global__ void __launch_bounds__(256) attention_delta_kernel(tvl_attention_args
                 const u32x4 x = load_unit<T, WIDE>(op, u, dim), y = load_unit<T, WIDE>(gp, u, dim);
                 const T *xe = reinterpret_cast<const T*>(&x), *ye = reinterpret_cast<const T*>(&y);
 #pragma unroll
-                for (int e = 0; e < PER; ++e) {
-                    const float gv = to_float(ye[e]);
-                    sum += to_float(xe[e]) * gv;
-                    if (!not_finite(gv)) top = fmaxf(top, fabsf(gv));
-                }
+                for (int e = 0; e < PER; ++e) sum += to_float(xe[e]) * to_float(ye[e]);
             }
         }
         for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
         if (i < queries && lane == 0) delta[(int64_t)bh * queries + i] = sum;
-    }
-    if constexpr (__is_same(T, f16)) {      // no other type has memory for them
-        __shared__ float part[4];
-        for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-        if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = top;
-        __syncthreads();
-        if (threadIdx.x == 0) maxima[blockIdx.x] = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
     }
 }
 
@@ -108,7 +111,7 @@ __global__ void __launch_bounds__((64 * Shape<T, DP>::W), (Shape<T, DP>::OCCUPAN
         docw.start(spans + (int64_t)b * ((queries + SPAN - 1) / SPAN), queries, q0, QB);
     }
     Frag<T> qf[DP / CK], gf[DP / CK];
-    float lse = 0.0f, dl = 0.0f, top = 0.0f;
+    float lse = 0.0f, dl = 0.0f;
 #pragma unroll
     for (int c = 0; c < DP / CK; ++c) {
         qf[c] = gf[c] = Frag<T>{};
@@ -116,22 +119,13 @@ __global__ void __launch_bounds__((64 * Shape<T, DP>::W), (Shape<T, DP>::OCCUPAN
             qf[c] = load_frag<T, WIDE>((const T*)a.q + b * a.q_batch + (int64_t)i * a.q_token + h * a.q_head, g + (64 / R) * c, dim);
             gf[c] = load_frag<T, WIDE>((const T*)gr.grad_out + b * gr.g_batch + (int64_t)i * gr.g_token + h * gr.g_head, g + (64 / R) * c, dim);
         }
-        if constexpr (__is_same(T, f16)) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (!not_finite((float)gf[c][e])) top = fmaxf(top, fabsf((float)gf[c][e]));
-        }
     }
     if (i < queries) {
         const int64_t row = ((int64_t)b * a.heads + h) * queries + i;
         lse = a.lse[row] * LOG2E;
         dl = delta[row];
     }
-    // float16: every query's own power of two
-    int e = 0;
-    if constexpr (__is_same(T, f16)) e = range_exponent(column_max<R>(top));
-    const float fit = power_of_two(-e);
-    dl *= fit;
+    float fit = __is_same(T, f16) ? FIT_START : 1.0f;
     const float slope = a.slopes ? a.slopes[h] * LOG2E : 0.0f;
     const bool capped = FORM != PLAIN && a.softcap > 0.0f, biased = FORM != PLAIN && a.slopes != nullptr;
     const float to_log2 = a.scale * LOG2E, to_cap = capped ? a.scale / a.softcap : 0.0f, from_cap = a.softcap * LOG2E;
@@ -189,11 +183,11 @@ __global__ void __launch_bounds__((64 * Shape<T, DP>::W), (Shape<T, DP>::OCCUPAN
                 for (int x = 0; x < N; ++x) {
                     const float th = cap_tanh<T>(s[x] * to_cap);
                     s[x] = from_cap * th;
-                    dp[x] = product(__builtin_fmaf(dp[x], fit, -dl), __builtin_fmaf(-th, th, 1.0f));
+                    dp[x] = product(dp[x] - dl, __builtin_fmaf(-th, th, 1.0f));
                 }
             } else {
 #pragma unroll
-                for (int x = 0; x < N; ++x) dp[x] = __builtin_fmaf(dp[x], fit, -dl);
+                for (int x = 0; x < N; ++x) dp[x] -= dl;
             }
             if (biased) {
                 const int here = i + seq.shift - jt - 4 * g;
@@ -214,8 +208,9 @@ __global__ void __launch_bounds__((64 * Shape<T, DP>::W), (Shape<T, DP>::OCCUPAN
                 }
             }
             // score gradients are rounded to the operands' type for the last product; its sum is float32
+            if constexpr (__is_same(T, f16)) follow_range<T, R>(dp, acc, fit);
 #pragma unroll
-            for (int x = 0; x < N; ++x) df[x / 8][x % 8] = (E)dp[x];
+            for (int x = 0; x < N; ++x) df[x / 8][x % 8] = (E)(__is_same(T, f16) ? product(dp[x], fit) : dp[x]);
             if (MASKED && (!one_document || (jt + PIECE > wall && wall < seq.end)) && holds_not_finite<T, DP, PIECE>(kt + t * L::ROW, lane)) {
 #pragma unroll
                 for (int c = 0; c < PIECE / CK; ++c)
@@ -248,7 +243,7 @@ __global__ void __launch_bounds__((64 * Shape<T, DP>::W), (Shape<T, DP>::OCCUPAN
         while (j0 < reach && !clean(j0)) step(std::true_type{});
     }
     if (i >= queries) return;
-    const float back = a.scale * power_of_two(e);
+    const float back = a.scale / fit;
     T* op = (T*)gr.dq + (((int64_t)b * queries + i) * a.heads + h) * dim;
 #pragma unroll
     for (int d = 0; d < DP / R; ++d)
@@ -264,7 +259,7 @@ __global__ void __launch_bounds__((64 * Shape<T, DP>::W), (Shape<T, DP>::OCCUPAN
 // bound as dq is, matrix cores busy 31 % and 22 %.
 template <typename T, int DP, Form FORM>
 __global__ void __launch_bounds__((64 * Shape<T, DP>::W), (Shape<T, DP>::OCCUPANCY)) attention_dkv_kernel(tvl_attention_args a, tvl_attention_grads gr, const DocumentSpan* __restrict__ spans, const float* __restrict__ delta,
-                                                            const float* __restrict__ maxima, int tiles, int parts, float* __restrict__ slabs) {
+                                                            int tiles, int parts, float* __restrict__ slabs) {
     constexpr bool WIDE = FORM != ODD;
     constexpr int R = Shape<T, DP>::R, THREADS = 64 * Shape<T, DP>::W, KB = 128, CK = CHUNK<R>, N = VALUES<R>;
     typedef Tile<T, DP> L;
@@ -299,17 +294,7 @@ __global__ void __launch_bounds__((64 * Shape<T, DP>::W), (Shape<T, DP>::OCCUPAN
             vf[c] = load_frag<T, WIDE>((const T*)a.v + b * a.v_batch + (int64_t)j * a.v_token + hk * a.v_head, g + (64 / R) * c, dim);
         }
     }
-    // float16: one power of two for all that this workgroup adds up
-    int e = 0;
-    if constexpr (__is_same(T, f16)) {
-        const int n = share * ((queries + GT - 1) / GT);
-        const float* mp = maxima + ((int64_t)b * a.heads + hk * group + head0) * ((queries + GT - 1) / GT);
-        float top = 0.0f;
-        for (int x = lane; x < n; x += 64) top = fmaxf(top, mp[x]);
-        for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-        e = range_exponent(top);
-    }
-    const float fit = power_of_two(-e);
+    float fit = __is_same(T, f16) ? FIT_START : 1.0f;
     const bool capped = FORM != PLAIN && a.softcap > 0.0f, biased = FORM != PLAIN && a.slopes != nullptr;
     const float to_log2 = a.scale * LOG2E, to_cap = capped ? a.scale / a.softcap : 0.0f, from_cap = a.softcap * LOG2E;
     const float pre = capped ? 1.0f : to_log2, unit = capped || biased ? 1.0f : to_log2;
@@ -340,7 +325,7 @@ __global__ void __launch_bounds__((64 * Shape<T, DP>::W), (Shape<T, DP>::OCCUPAN
         const int64_t row = ((int64_t)b * a.heads + h) * queries + i;
         // a query behind the last gets weights exp(-inf) = 0
         if (threadIdx.x < 64) side = i < queries ? a.lse[row] * LOG2E : __builtin_inff();
-        else if (threadIdx.x < 128) side = i < queries ? delta[row] * fit : 0.0f;
+        else if (threadIdx.x < 128) side = i < queries ? delta[row] : 0.0f;
         if (docs && threadIdx.x < GT) qdoc = i < queries ? docs[i] : -1;
     };
     auto put_queries = [&](char* to) {
@@ -396,11 +381,11 @@ __global__ void __launch_bounds__((64 * Shape<T, DP>::W), (Shape<T, DP>::OCCUPAN
                 for (int x = 0; x < N; ++x) {
                     const float th = cap_tanh<T>(s[x] * to_cap);
                     s[x] = from_cap * th;
-                    dp[x] = product(__builtin_fmaf(dp[x], fit, -dl[piece_row<R>(x)]), __builtin_fmaf(-th, th, 1.0f));
+                    dp[x] = product(dp[x] - dl[piece_row<R>(x)], __builtin_fmaf(-th, th, 1.0f));
                 }
             } else {
 #pragma unroll
-                for (int x = 0; x < N; ++x) dp[x] = __builtin_fmaf(dp[x], fit, -dl[piece_row<R>(x)]);
+                for (int x = 0; x < N; ++x) dp[x] -= dl[piece_row<R>(x)];
             }
             if (biased) {
                 const int here = it + 4 * g + seq.shift - j;
@@ -425,10 +410,11 @@ __global__ void __launch_bounds__((64 * Shape<T, DP>::W), (Shape<T, DP>::OCCUPAN
                 }
             }
             // weights and score gradients are rounded to the operands' type for the last products; their sums are float32
+            if constexpr (__is_same(T, f16)) follow_range<T, R>(dp, dk, fit);
 #pragma unroll
             for (int x = 0; x < N; ++x) {
                 pf[x / 8][x % 8] = (E)s[x];
-                df[x / 8][x % 8] = (E)dp[x];
+                df[x / 8][x % 8] = (E)(__is_same(T, f16) ? product(dp[x], fit) : dp[x]);
             }
             if (MASKED && masked && (holds_not_finite<T, DP, PIECE>(gt + t * L::ROW, lane) || holds_not_finite<T, DP, PIECE>(qt + t * L::ROW, lane))) {
 #pragma unroll
@@ -474,7 +460,7 @@ __global__ void __launch_bounds__((64 * Shape<T, DP>::W), (Shape<T, DP>::OCCUPAN
         while (n < total && clean(n)) step(std::false_type{});
     }
     if (j >= keys) return;
-    const float back = a.scale * power_of_two(e);
+    const float back = a.scale / fit;
     const int64_t row = (((int64_t)b * keys + j) * a.kv_heads + hk) * dim;
 #pragma unroll
     for (int d = 0; d < DP / R; ++d)
@@ -521,7 +507,7 @@ int attention_backward_parts(const tvl_attention_args& a) {
 }
 
 template <typename T, int DP, Form FORM>
-static int launch_gradients(const tvl_attention_args& a, const tvl_attention_grads& g, const DocumentSpan* spans, const float* delta, const float* maxima, float* slabs, hipStream_t st) {
+static int launch_gradients(const tvl_attention_args& a, const tvl_attention_grads& g, const DocumentSpan* spans, const float* delta, float* slabs, hipStream_t st) {
     if (g.dq && a.queries > 0) {
         const int tiles = (int)ceil_div(a.queries, 128);
         const size_t bytes = 4 * GT * (size_t)Tile<T, DP>::ROW + (FORM == PLAIN ? 0 : 2 * GT * 8);
@@ -533,7 +519,7 @@ static int launch_gradients(const tvl_attention_args& a, const tvl_attention_gra
         const int tiles = (int)ceil_div(a.keys, 128), parts = attention_backward_parts(a);
         const size_t bytes = 2 * (2 * GT * (size_t)Tile<T, DP>::ROW + 2 * GT * 4 + (FORM == PLAIN ? 0 : GT * 8));
         if (bytes > 65536) TVL_HIP_CHECK(hipFuncSetAttribute((const void*)attention_dkv_kernel<T, DP, FORM>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
-        hipLaunchKernelGGL((attention_dkv_kernel<T, DP, FORM>), dim3((unsigned)(a.batch * a.kv_heads * tiles * parts)), dim3(64 * Shape<T, DP>::W), bytes, st, a, g, spans, delta, maxima,
+        hipLaunchKernelGGL((attention_dkv_kernel<T, DP, FORM>), dim3((unsigned)(a.batch * a.kv_heads * tiles * parts)), dim3(64 * Shape<T, DP>::W), bytes, st, a, g, spans, delta,
                            tiles, parts, slabs);
         TVL_LAUNCH_CHECK();
         if (parts > 1) {
@@ -546,7 +532,7 @@ static int launch_gradients(const tvl_attention_args& a, const tvl_attention_gra
 }
 
 template <typename T>
-static int launch_backward(const tvl_attention_args& a, const tvl_attention_grads& g, const DocumentSpan* spans, float* delta, float* maxima, float* slabs, hipStream_t st) {
+static int launch_backward(const tvl_attention_args& a, const tvl_attention_grads& g, const DocumentSpan* spans, float* delta, float* slabs, hipStream_t st) {
     const size_t z = sizeof(T);
     const bool grad = wide_rows(g.grad_out, a.dim, g.g_batch, g.g_token, g.g_head, z);
     const bool wide = grad && wide_rows(a.q, a.dim, a.q_batch, a.q_token, a.q_head, z) && wide_rows(a.k, a.dim, a.k_batch, a.k_token, a.k_head, z) &&
@@ -554,20 +540,20 @@ static int launch_backward(const tvl_attention_args& a, const tvl_attention_grad
     if (a.queries > 0) {
         const int blocks = (int)ceil_div(a.queries, GT);
         const unsigned n = (unsigned)(a.batch * a.heads * blocks);
-        if (grad && wide_rows(a.out, a.dim, a.o_batch, a.o_token, a.o_head, z)) hipLaunchKernelGGL((attention_delta_kernel<T, true>), dim3(n), dim3(256), 0, st, a, g, delta, maxima, blocks);
-        else hipLaunchKernelGGL((attention_delta_kernel<T, false>), dim3(n), dim3(256), 0, st, a, g, delta, maxima, blocks);
+        if (grad && wide_rows(a.out, a.dim, a.o_batch, a.o_token, a.o_head, z)) hipLaunchKernelGGL((attention_delta_kernel<T, true>), dim3(n), dim3(256), 0, st, a, g, delta, blocks);
+        else hipLaunchKernelGGL((attention_delta_kernel<T, false>), dim3(n), dim3(256), 0, st, a, g, delta, blocks);
         TVL_LAUNCH_CHECK();
     }
     // odd rows take the same shapes: the same sums in the same order
-    if (!wide) return a.dim <= 64 ? launch_gradients<T, 64, ODD>(a, g, spans, delta, maxima, slabs, st) : launch_gradients<T, 128, ODD>(a, g, spans, delta, maxima, slabs, st);
-    if (a.dim <= 64) return featureless(a) ? launch_gradients<T, 64, PLAIN>(a, g, spans, delta, maxima, slabs, st) : launch_gradients<T, 64, GENERAL>(a, g, spans, delta, maxima, slabs, st);
-    return featureless(a) ? launch_gradients<T, 128, PLAIN>(a, g, spans, delta, maxima, slabs, st) : launch_gradients<T, 128, GENERAL>(a, g, spans, delta, maxima, slabs, st);
+    if (!wide) return a.dim <= 64 ? launch_gradients<T, 64, ODD>(a, g, spans, delta, slabs, st) : launch_gradients<T, 128, ODD>(a, g, spans, delta, slabs, st);
+    if (a.dim <= 64) return featureless(a) ? launch_gradients<T, 64, PLAIN>(a, g, spans, delta, slabs, st) : launch_gradients<T, 64, GENERAL>(a, g, spans, delta, slabs, st);
+    return featureless(a) ? launch_gradients<T, 128, PLAIN>(a, g, spans, delta, slabs, st) : launch_gradients<T, 128, GENERAL>(a, g, spans, delta, slabs, st);
 }
 
-int launch_attention_backward(const tvl_attention_args& a, const tvl_attention_grads& g, const DocumentSpan* spans, float* delta, float* maxima, float* slabs, hipStream_t st) {
-    if (a.dtype == TVL_F32) return launch_backward<float>(a, g, spans, delta, maxima, slabs, st);
-    if (a.dtype == TVL_F16) return launch_backward<f16>(a, g, spans, delta, maxima, slabs, st);
-    return launch_backward<bf16_t>(a, g, spans, delta, maxima, slabs, st);
+int launch_attention_backward(const tvl_attention_args& a, const tvl_attention_grads& g, const DocumentSpan* spans, float* delta, float* slabs, hipStream_t st) {
+    if (a.dtype == TVL_F32) return launch_backward<float>(a, g, spans, delta, slabs, st);
+    if (a.dtype == TVL_F16) return launch_backward<f16>(a, g, spans, delta, slabs, st);
+    return launch_backward<bf16_t>(a, g, spans, delta, slabs, st);
 }
 
 }  // namespace tvl

@@ -394,7 +394,7 @@ static inline bool wide_rows(const void* p, int64_t dim, int64_t batch, int64_t 
 }
 
 int launch_attention_forward(const tvl_attention_args& a, bool cached, const DocumentSpan* spans, hipStream_t st);
-int launch_attention_backward(const tvl_attention_args& a, const tvl_attention_grads& g, const DocumentSpan* spans, float* delta, float* maxima, float* slabs, hipStream_t st);
+int launch_attention_backward(const tvl_attention_args& a, const tvl_attention_grads& g, const DocumentSpan* spans, float* delta, float* slabs, hipStream_t st);
 int attention_backward_parts(const tvl_attention_args& a);
 bool attention_step_serves(const tvl_attention_args& a);
 size_t attention_step_bytes(const tvl_attention_args& a);

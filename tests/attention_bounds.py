@@ -1,0 +1,43 @@
+"""Tighter element-wise bounds than tests/attention_reference.py where float16 loses digits: the size of its subnormal numbers counts relative to what the kernels
+scale by.
+
+Score gradients: every column (a query of dq, a key of dk) is multiplied by a power of two that brings its largest score gradient so far to 2^7 or more, up to
+2^15.  float16 holds multiples of 2^-24 at the lower end, so a rounding there is off by at most 2^-25 / 2^7 = 2^-32 of the column's own largest one,
+whatever other columns hold."""
+import torch
+
+import attention_reference as R
+
+
+class Tight(R.Attention):
+    def grads(self, go):
+        b, tq, tk, hq, hk, d = self.shape
+        n, u, F32 = hq // hk, self.u, R.F32
+        G = go.double().transpose(1, 2)
+        G = torch.where(self.see.any(2)[:, None, :, None], G, torch.zeros_like(G))
+        p, V, K, Q, see = self.p, self.V, self.K, self.Q, self.see[:, None].double()
+        half = self.dtype == torch.float16
+        dp = G @ V.transpose(2, 3)
+        delta = (G * self.out).sum(-1, keepdim=True)
+        core = p * (dp - delta) * self.bend
+        # the same roundings as in the reference: weights, dp, delta (of the rounded output), the cap's slope, the score gradient's own
+        e_p = 2 * self.ds + (tk + 16) * F32
+        e_dp = (d + 4) * F32 * (G.abs() @ V.abs().transpose(2, 3))
+        e_delta = (G.abs() * (self.out_tol + u * self.out.abs())).sum(-1, keepdim=True) + (d + 4) * F32 * (G.abs() * self.out.abs()).sum(-1, keepdim=True)
+        e = (e_p + u * 1.01) * core.abs() + p * (e_dp + e_delta) + 2.0 ** -19 * p * (dp - delta).abs() + 8 * F32 * p * (dp.abs() + delta.abs())
+        size = core.abs() + e
+        step = 2.0 ** -32 if half else 0.0
+        group = lambda x: x.view(b, hk, n, tq, tk)
+        e_q = (e + step * size.amax(-1, keepdim=True) * see) * abs(self.scale)
+        e_k = (e + step * group(size).amax((2, 3), keepdim=True).expand(b, hk, n, 1, tk).reshape(b, hq, 1, tk) * see) * abs(self.scale)
+        least = 2.0 ** -25 if half else 0.0             # of the results
+        ds = core * self.scale
+        shared = lambda x: x.view(b, hk, n, tk, d).sum(2)
+        dq, dk, dv = ds @ K, shared(ds.transpose(2, 3) @ Q), shared(p.transpose(2, 3) @ G)
+        dq_tol = e_q @ K.abs() + u * dq.abs() + least + (tk + 16) * F32 * (ds.abs() @ K.abs()) + 1e-30
+        terms = n * tq + 16
+        dk_tol = shared(e_k.transpose(2, 3) @ Q.abs()) + u * dk.abs() + least + terms * F32 * shared(ds.abs().transpose(2, 3) @ Q.abs()) + 1e-30
+        e_w = (u * 1.01 + e_p) * p + self.step * see
+        dv_tol = shared(e_w.transpose(2, 3) @ G.abs()) + u * dv.abs() + least + terms * F32 * shared(p.transpose(2, 3) @ G.abs()) + 1e-30
+        rows = lambda x: x.transpose(1, 2)
+        return [(rows(dq), rows(dq_tol)), (rows(dk), rows(dk_tol)), (rows(dv), rows(dv_tol))]

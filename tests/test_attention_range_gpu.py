@@ -1,0 +1,117 @@
+"""Attention where numbers of very different size meet: score gradients of large values, of losses that differ by many powers of ten between documents,
+tokens and queries, against float64 within the bounds of tests/attention_bounds.py."""
+import math
+import os
+import sys
+
+import pytest
+import torch
+
+sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
+import attention_reference as R  # noqa: E402
+from attention_bounds import Tight  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+
+
+@pytest.fixture(scope="module")
+def tv():
+    import ternary_vllm_amd
+    return ternary_vllm_amd
+
+
+def normal(gen, *shape, dtype=torch.float32, scale=1.0):
+    return (torch.randn(shape, generator=gen) * scale).to(dtype)
+
+
+def within(got, want, tol, what):
+    """R.within; where the exact value may lie beyond the type's largest one, the infinity of its sign is a rounding of it."""
+    got, want = got.detach().cpu(), want.to(torch.float64)
+    beyond = (want.abs() + tol >= torch.finfo(got.dtype).max) & (got == torch.copysign(torch.full_like(want, math.inf), want))
+    R.within(torch.where(beyond, want, got.double()), want, tol, what)
+
+
+def run_training(tv, dev, q, k, v, go, causal=False, documents=None, softcap=0.0, prefix=None, scale=None):
+    """Result and gradients within Tight's bounds; returns them."""
+    b, tq, tk = q.shape[0], q.shape[1], k.shape[1]
+    see, place = R.sees(b, tq, tk, causal, torch.full((b,), prefix or 0), documents)
+    ref = Tight(q, k, v, see, place, scale, softcap)
+    leaves = [x.to(dev).requires_grad_(True) for x in (q, k, v)]
+    out = tv.attention(*leaves, causal=causal, softcap=softcap, prefix=prefix, scale=scale, documents=None if documents is None else documents.to(dev))
+    within(out, *ref.forward(), what="out")
+    grads = torch.autograd.grad(out, leaves, go.to(dev))
+    for name, got, (want, tol) in zip(("dq", "dk", "dv"), grads, ref.grads(go)):
+        within(got, want, tol, name)
+    return [out.detach(), *grads]
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("value,gradient", [(70.0, 0.0624), (3000.0, 0.0624), (70.0, 15.0), (60000.0, 0.001)])
+def test_score_gradients_of_large_values(tv, dev, kind, d, value, gradient):
+    """Rows of values of one sign against output gradients of one sign: their products, far beyond float16's range here and there, belong to gradients that are not."""
+    dt = TYPES[kind]
+    # one query, two keys of equal score: dq = scale * gradient * value * d * (k0 - k1) / 2 * 2 / 2
+    q, go = torch.zeros(1, 1, 1, d, dtype=dt), torch.full((1, 1, 1, d), gradient, dtype=dt)
+    k, v = torch.zeros(1, 2, 1, d, dtype=dt), torch.full((1, 2, 1, d), value, dtype=dt)
+    q[..., 1] = 1.0                                     # apart from the keys: the scores stay 0
+    k[:, 0, :, 0], k[:, 1, :, 0] = 0.25, -0.25
+    v[:, 1] = -v[:, 1]
+    want = d ** -0.5 * float(go[0, 0, 0, 0]) * float(v[0, 0, 0, 0]) * d * 0.25
+    _, dq, dk, _ = run_training(tv, dev, q, k, v, go)
+    assert abs(float(dq[0, 0, 0, 0]) - want) <= 2.0 ** -7 * want and abs(float(dk[0, 0, 0, 1]) - 2 * want) <= 2.0 ** -7 * 2 * want
+    g = torch.Generator().manual_seed(d)
+    t = 150
+    sign = torch.where(torch.rand(1, t, 2, 1, generator=g) < 0.5, -1.0, 1.0)
+    q, k = normal(g, 1, t, 4, d, dtype=dt, scale=0.01), normal(g, 1, t, 2, d, dtype=dt, scale=0.01)
+    v = (sign * value * (1 + 0.02 * torch.randn(1, t, 2, d, generator=g))).to(dt)
+    go = (gradient * (1 + 0.02 * torch.randn(1, t, 4, d, generator=g))).to(dt)
+    run_training(tv, dev, q, k, v, go, causal=True)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("small,large", [(0.01, 15.0), (1e-4, 100.0), (0.02, 30000.0)])
+def test_documents_of_different_losses(tv, dev, kind, d, causal, small, large):
+    """A document's gradients have the accuracy they have alone, beside documents of much larger ones, and the same bits."""
+    dt = TYPES[kind]
+    g = torch.Generator().manual_seed(91 + d)
+    t = 260
+    ids = torch.where(torch.arange(t) < 100, 0, torch.where(torch.arange(t) < 230, 1, 2))[None]
+    q, k, v, go = (normal(g, 1, t, h, d, dtype=dt, scale=s) for h, s in ((4, 1.0), (2, 1.0), (2, 1.0), (4, small)))
+    loud = go.clone()
+    loud[:, 100:230] = (torch.rand(1, 130, 4, d, generator=g) * large).to(dt)
+    alone = run_training(tv, dev, q, k, v, go, causal, ids)
+    beside = run_training(tv, dev, q, k, v, loud, causal, ids)
+    for x, y in zip(alone, beside):
+        assert torch.equal(x[:, :100], y[:, :100]) and torch.equal(x[:, 230:], y[:, 230:])
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("large", [100.0, 30000.0])
+def test_a_large_gradient_at_a_token_that_others_do_not_see(tv, dev, kind, d, large):
+    dt = TYPES[kind]
+    g = torch.Generator().manual_seed(95 + d)
+    t = 400
+    q, k, v, go = (normal(g, 1, t, h, d, dtype=dt, scale=s) for h, s in ((2, 1.0), (1, 1.0), (1, 1.0), (2, 0.02)))
+    loud = go.clone()
+    loud[:, 0, :, 0] = large                             # the first query sees the first key alone
+    alone, beside = run_training(tv, dev, q, k, v, go, True), run_training(tv, dev, q, k, v, loud, True)
+    assert torch.equal(alone[2][:, 1:], beside[2][:, 1:]) and torch.equal(alone[1][:, 1:], beside[1][:, 1:])
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("softcap", [0.0, 5.0])
+def test_gradients_of_every_size_at_once(tv, dev, kind, softcap):
+    """Queries whose output gradients differ by powers of ten from token to token, in rising, falling and mixed order."""
+    dt = TYPES[kind]
+    g = torch.Generator().manual_seed(97)
+    for order in (torch.arange(200), torch.arange(199, -1, -1), torch.randperm(200, generator=g)):
+        size = 10.0 ** (order.double() / 199 * 8 - 6)     # 1e-6 .. 1e2
+        q, k, v, go = (normal(g, 1, 200, h, 64) for h in (2, 2, 2, 2))
+        go = go * size[None, :, None, None].float()
+        run_training(tv, dev, *(x.to(dt) for x in (q, k, v, go)), causal=False, softcap=softcap)
+        run_training(tv, dev, *(x.to(dt) for x in (q, k, v, go)), causal=True, softcap=softcap)
