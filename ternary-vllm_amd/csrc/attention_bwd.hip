@@ -295,6 +295,7 @@ __global__ void __launch_bounds__((64 * Shape<T, DP>::W), (Shape<T, DP>::OCCUPAN
         }
     }
     float fit = __is_same(T, f16) ? FIT_START : 1.0f;
+    constexpr float UP = BACKWARD_LIFT<T>;
     const bool capped = FORM != PLAIN && a.softcap > 0.0f, biased = FORM != PLAIN && a.slopes != nullptr;
     const float to_log2 = a.scale * LOG2E, to_cap = capped ? a.scale / a.softcap : 0.0f, from_cap = a.softcap * LOG2E;
     const float pre = capped ? 1.0f : to_log2, unit = capped || biased ? 1.0f : to_log2;
@@ -316,7 +317,7 @@ __global__ void __launch_bounds__((64 * Shape<T, DP>::W), (Shape<T, DP>::OCCUPAN
     };
     const int lane_row = L::template lane_row<R>(lane), lane_col = L::template lane_column<R>(lane);
     Stage<T, DP, GT, THREADS, WIDE> stage;
-    float side = 0.0f;      // threads 0..63: a log-sum, 64..127: a delta
+    float side = 0.0f;      // threads 0..63: a log-sum (less UP: weights and score gradients come out 2^UP times as large), 64..127: a delta
     int64_t qdoc = -1;      // threads 0..63
     auto fetch_queries = [&](int n) {
         const int h = hk * group + head0 + n / steps, i0 = begin + (n % steps) * GT;
@@ -324,7 +325,7 @@ __global__ void __launch_bounds__((64 * Shape<T, DP>::W), (Shape<T, DP>::OCCUPAN
         const int i = i0 + (threadIdx.x & 63);
         const int64_t row = ((int64_t)b * a.heads + h) * queries + i;
         // a query behind the last gets weights exp(-inf) = 0
-        if (threadIdx.x < 64) side = i < queries ? a.lse[row] * LOG2E : __builtin_inff();
+        if (threadIdx.x < 64) side = i < queries ? a.lse[row] * LOG2E - UP : __builtin_inff();
         else if (threadIdx.x < 128) side = i < queries ? delta[row] : 0.0f;
         if (docs && threadIdx.x < GT) qdoc = i < queries ? docs[i] : -1;
     };
@@ -460,7 +461,7 @@ __global__ void __launch_bounds__((64 * Shape<T, DP>::W), (Shape<T, DP>::OCCUPAN
         while (n < total && clean(n)) step(std::false_type{});
     }
     if (j >= keys) return;
-    const float back = a.scale / fit;
+    const float down = 1.0f / (float)(1 << (int)UP), back = a.scale / fit * down;
     const int64_t row = (((int64_t)b * keys + j) * a.kv_heads + hk) * dim;
 #pragma unroll
     for (int d = 0; d < DP / R; ++d)
@@ -471,10 +472,10 @@ __global__ void __launch_bounds__((64 * Shape<T, DP>::W), (Shape<T, DP>::OCCUPAN
             if (parts > 1) {
                 const int64_t all = (int64_t)a.batch * keys * a.kv_heads * dim;
                 slabs[at.head * 2 * all + row + col] = dk[d][x] * back;
-                slabs[(at.head * 2 + 1) * all + row + col] = dv[d][x];
+                slabs[(at.head * 2 + 1) * all + row + col] = dv[d][x] * down;
             } else {
                 ((T*)gr.dk)[row + col] = from_float<T>(product(dk[d][x], back));
-                ((T*)gr.dv)[row + col] = from_float<T>(dv[d][x]);
+                ((T*)gr.dv)[row + col] = from_float<T>(product(dv[d][x], down));
             }
         }
 }

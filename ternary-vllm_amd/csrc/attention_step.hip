@@ -136,7 +136,7 @@ __global__ void __launch_bounds__(64 * WAVES) attention_step_kernel(tvl_attentio
         if (__any(grow)) {
             const float now = grow ? top : m, shrink = grow ? __builtin_amdgcn_exp2f(m - now) : 1.0f;
             m = now;
-            base = m == -__builtin_inff() ? 0.0f : m;
+            base = m == -__builtin_inff() ? 0.0f : m - LIFT<T>;
             sum *= shrink;
 #pragma unroll
             for (int d = 0; d < DP / R; ++d) acc[d] *= shrink;

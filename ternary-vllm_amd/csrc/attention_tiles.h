@@ -266,6 +266,13 @@ template <typename T> __device__ __forceinline__ float cap_tanh(float y) {
     return 1.0f - 2.0f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(y * (2.0f * LOG2E)) + 1.0f);
 }
 
+// float16 holds 2^15 and no digits below 2^-25: softmax weights rounded to it are formed 2^LIFT times as large, so that a long row's many small ones,
+// which the float32 sum counts, count in the products too.  In the forward pass the largest weight of a row then lies in [2^7, 2^15] (its
+// running maximum may lag by 2^8) and a weight is off by at most 2^-32 of it; the backward pass lifts weights relative to their sum, at most 1 but for the
+// log-sum's rounding.  The other types have float32's range.
+template <typename T> constexpr float LIFT = __is_same(T, f16) ? 7.0f : 0.0f;
+template <typename T> constexpr float BACKWARD_LIFT = __is_same(T, f16) ? 12.0f : 0.0f;
+
 // a product that is rounded to float32 before anything else happens to it: never part of a fused or mixed-precision instruction, so the same bits
 // in every form of a kernel
 __device__ __forceinline__ float product(float x, float y) {

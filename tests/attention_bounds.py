@@ -3,13 +3,22 @@ scale by.
 
 Score gradients: every column (a query of dq, a key of dk) is multiplied by a power of two that brings its largest score gradient so far to 2^7 or more, up to
 2^15.  float16 holds multiples of 2^-24 at the lower end, so a rounding there is off by at most 2^-25 / 2^7 = 2^-32 of the column's own largest one,
-whatever other columns hold."""
+whatever other columns hold.
+
+Softmax weights: in the forward pass the largest weight of a row is 2^7 or more when float16 rounds it, so a small one is off by 2^-32 of the largest; the
+backward pass rounds 2^12 times the weight (at most 2^12), so by 2^-37."""
 import torch
 
 import attention_reference as R
 
 
 class Tight(R.Attention):
+    def __init__(self, q, k, v, see, *rest):
+        super().__init__(q, k, v, see, *rest)
+        if self.dtype == torch.float16:
+            seen = see[:, None].double() @ self.V.abs()
+            self.out_tol = self.out_tol - self.step * seen + 2.0 ** -32 * seen
+
     def grads(self, go):
         b, tq, tk, hq, hk, d = self.shape
         n, u, F32 = hq // hk, self.u, R.F32
@@ -37,7 +46,7 @@ class Tight(R.Attention):
         dq_tol = e_q @ K.abs() + u * dq.abs() + least + (tk + 16) * F32 * (ds.abs() @ K.abs()) + 1e-30
         terms = n * tq + 16
         dk_tol = shared(e_k.transpose(2, 3) @ Q.abs()) + u * dk.abs() + least + terms * F32 * shared(ds.abs().transpose(2, 3) @ Q.abs()) + 1e-30
-        e_w = (u * 1.01 + e_p) * p + self.step * see
+        e_w = (u * 1.01 + e_p) * p + (2.0 ** -37 * see if half else 0.0)
         dv_tol = shared(e_w.transpose(2, 3) @ G.abs()) + u * dv.abs() + least + terms * F32 * shared(p.transpose(2, 3) @ G.abs()) + 1e-30
         rows = lambda x: x.transpose(1, 2)
         return [(rows(dq), rows(dq_tol)), (rows(dk), rows(dk_tol)), (rows(dv), rows(dv_tol))]

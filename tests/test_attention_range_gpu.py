@@ -1,5 +1,5 @@
 """Attention where numbers of very different size meet: score gradients of large values, of losses that differ by many powers of ten between documents,
-tokens and queries, against float64 within the bounds of tests/attention_bounds.py."""
+tokens and queries; rows of many small weights: against float64 within the bounds of tests/attention_bounds.py."""
 import math
 import os
 import sys
@@ -115,3 +115,45 @@ def test_gradients_of_every_size_at_once(tv, dev, kind, softcap):
         go = go * size[None, :, None, None].float()
         run_training(tv, dev, *(x.to(dt) for x in (q, k, v, go)), causal=False, softcap=softcap)
         run_training(tv, dev, *(x.to(dt) for x in (q, k, v, go)), causal=True, softcap=softcap)
+
+
+def small_weights(kind, d, queries, keys, away):
+    """One key of value 0 and score 0, all others of value 1 and a score of -away * ln 2: scale 1, the first element of a head carries the score."""
+    dt = TYPES[kind]
+    q, k, v = torch.zeros(1, queries, 2, d, dtype=dt), torch.zeros(1, keys, 1, d, dtype=dt), torch.ones(1, keys, 1, d, dtype=dt)
+    q[..., 0] = 1.0
+    k[..., 0] = -away * math.log(2.0)
+    return q, k, v
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("away", [24.5, 25.2, 28.0, 31.0])
+def test_many_small_weights_count(tv, dev, kind, d, away):
+    """Weights far below the largest one of their row: together they are a result."""
+    q, k, v = small_weights(kind, d, 40, 20000, away)
+    for top in (0, 7000, 19999):                         # where the large score is: the running maximum finds it early or late
+        kt, vt = k.clone(), v.clone()
+        kt[:, top, :, 0], vt[:, top] = 0.0, 0.0
+        see, place = R.sees(1, 40, 20000, False, torch.zeros(1, dtype=torch.int64), None)
+        want, tol = Tight(q, kt, vt, see, place, 1.0).forward()
+        # whole rows, a few tokens over a cache (cut into parts), many tokens over a cache
+        within(tv.attention(q.to(dev), kt.to(dev), vt.to(dev), scale=1.0), want, tol, "attention")
+        if top == 19999:
+            continue                                     # only the last token of a chunk would see it
+        cache = [x.transpose(1, 2).contiguous().to(dev) for x in (kt, vt)]
+        for n in (1, 8, 40):
+            at = 20000 - n
+            see, place = R.sees(1, n, 20000, True, torch.zeros(1, dtype=torch.int64), None, torch.tensor([at]), torch.tensor([n]))
+            want, tol = Tight(q[:, :n], kt, vt, see, place, 1.0).forward()
+            within(tv.cached_attention(q[:, :n].to(dev), *cache, at, scale=1.0), want, tol, f"cached {n}")
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("away", [24.5, 25.2, 28.0, 31.0])
+def test_value_gradients_of_many_small_weights(tv, dev, kind, d, away):
+    q, k, v = small_weights(kind, d, 700, 200, away)
+    k[:, 3, :, 0] = 0.0
+    go = torch.ones(1, 700, 2, d, dtype=TYPES[kind]) * 50
+    run_training(tv, dev, q, k, v, go, scale=1.0)
