@@ -5,8 +5,6 @@
 // 12 heads of 64, f16.
 #include "attention_tiles.h"
 
-#include <type_traits>
-
 namespace tvl {
 
 constexpr int GT = 64;    // rows of a staged tile
@@ -180,10 +178,12 @@ __global__ void __launch_bounds__((64 * Shape<T, DP>::W), (Shape<T, DP>::OCCUPAN
             Frag<T> df[PIECE / CK];
             if (capped) {
 #pragma unroll
+                for (int x = 0; x < N; ++x) s[x] *= to_cap;
+                cap_tanh<T, FORM, N>(s, a.softcap);
+#pragma unroll
                 for (int x = 0; x < N; ++x) {
-                    const float th = cap_tanh<T>(s[x] * to_cap);
-                    s[x] = from_cap * th;
-                    dp[x] = product(dp[x] - dl, __builtin_fmaf(-th, th, 1.0f));
+                    dp[x] = product(dp[x] - dl, __builtin_fmaf(-s[x], s[x], 1.0f));
+                    s[x] *= from_cap;
                 }
             } else {
 #pragma unroll
@@ -379,10 +379,12 @@ __global__ void __launch_bounds__((64 * Shape<T, DP>::W), (Shape<T, DP>::OCCUPAN
             const float *ls = lses + t + 4 * g, *dl = deltas + t + 4 * g;
             if (capped) {
 #pragma unroll
+                for (int x = 0; x < N; ++x) s[x] *= to_cap;
+                cap_tanh<T, FORM, N>(s, a.softcap);
+#pragma unroll
                 for (int x = 0; x < N; ++x) {
-                    const float th = cap_tanh<T>(s[x] * to_cap);
-                    s[x] = from_cap * th;
-                    dp[x] = product(dp[x] - dl[piece_row<R>(x)], __builtin_fmaf(-th, th, 1.0f));
+                    dp[x] = product(dp[x] - dl[piece_row<R>(x)], __builtin_fmaf(-s[x], s[x], 1.0f));
+                    s[x] *= from_cap;
                 }
             } else {
 #pragma unroll
@@ -546,9 +548,10 @@ static int launch_backward(const tvl_attention_args& a, const tvl_attention_grad
         TVL_LAUNCH_CHECK();
     }
     // odd rows take the same shapes: the same sums in the same order
-    if (!wide) return a.dim <= 64 ? launch_gradients<T, 64, ODD>(a, g, spans, delta, slabs, st) : launch_gradients<T, 128, ODD>(a, g, spans, delta, slabs, st);
-    if (a.dim <= 64) return featureless(a) ? launch_gradients<T, 64, PLAIN>(a, g, spans, delta, slabs, st) : launch_gradients<T, 64, GENERAL>(a, g, spans, delta, slabs, st);
-    return featureless(a) ? launch_gradients<T, 128, PLAIN>(a, g, spans, delta, slabs, st) : launch_gradients<T, 128, GENERAL>(a, g, spans, delta, slabs, st);
+    return with_form<T>(a, wide, [&](auto form) {
+        constexpr Form FORM = decltype(form)::value;
+        return a.dim <= 64 ? launch_gradients<T, 64, FORM>(a, g, spans, delta, slabs, st) : launch_gradients<T, 128, FORM>(a, g, spans, delta, slabs, st);
+    });
 }
 
 int launch_attention_backward(const tvl_attention_args& a, const tvl_attention_grads& g, const DocumentSpan* spans, float* delta, float* slabs, hipStream_t st) {

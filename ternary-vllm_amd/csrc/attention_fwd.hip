@@ -1,8 +1,6 @@
 // Forward attention over tiles: tvl_attention, and tvl_cached_attention for chunks of many tokens.
 #include "attention_tiles.h"
 
-#include <type_traits>
-
 namespace tvl {
 
 // One workgroup: 4 waves x 32 queries of one head; keys and values come in tiles of 64 through LDS, two buffers, the next tile's loads in
@@ -117,9 +115,11 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attention_forward
             const bool one_document = !MASKED || !docs || docw.one(j0 / SPAN, lane);
             if (capped) {
 #pragma unroll
-                for (int t = 0; t < KT / R; ++t)
-#pragma unroll
-                    for (int x = 0; x < REGS<R>; ++x) s[t][x] = from_cap * cap_tanh<T>(s[t][x] * to_cap);
+                for (int t = 0; t < KT / R; ++t) {
+                    s[t] *= to_cap;
+                    cap_tanh<T, FORM, REGS<R>>(s[t], a.softcap);
+                    s[t] *= from_cap;
+                }
             }
             if (biased) {
                 const int here = i + seq.shift - j0 - 4 * g;
@@ -260,9 +260,10 @@ static int launch_forward_t(const tvl_attention_args& a, const DocumentSpan* spa
     const size_t z = sizeof(T);
     const bool wide = wide_rows(a.q, a.dim, a.q_batch, a.q_token, a.q_head, z) && wide_rows(a.k, a.dim, a.k_batch, a.k_token, a.k_head, z) &&
                       wide_rows(a.v, a.dim, a.v_batch, a.v_token, a.v_head, z) && wide_rows(a.out, a.dim, a.o_batch, a.o_token, a.o_head, z);
-    if (!wide) return a.dim <= 64 ? launch_forward<T, 64, CACHED, ODD>(a, spans, st) : launch_forward<T, 128, CACHED, ODD>(a, spans, st);
-    if (a.dim <= 64) return featureless(a) ? launch_forward<T, 64, CACHED, PLAIN>(a, spans, st) : launch_forward<T, 64, CACHED, GENERAL>(a, spans, st);
-    return featureless(a) ? launch_forward<T, 128, CACHED, PLAIN>(a, spans, st) : launch_forward<T, 128, CACHED, GENERAL>(a, spans, st);
+    return with_form<T>(a, wide, [&](auto form) {
+        constexpr Form FORM = decltype(form)::value;
+        return a.dim <= 64 ? launch_forward<T, 64, CACHED, FORM>(a, spans, st) : launch_forward<T, 128, CACHED, FORM>(a, spans, st);
+    });
 }
 
 int launch_attention_forward(const tvl_attention_args& a, bool cached, const DocumentSpan* spans, hipStream_t st) {

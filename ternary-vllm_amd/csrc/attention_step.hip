@@ -106,9 +106,11 @@ __global__ void __launch_bounds__(64 * WAVES) attention_step_kernel(tvl_attentio
         if (j0 < hi) fetch(j0);
         if (capped) {
 #pragma unroll
-            for (int t = 0; t < STEP / R; ++t)
-#pragma unroll
-                for (int x = 0; x < REGS<R>; ++x) s[t][x] = from_cap * cap_tanh<T>(s[t][x] * to_cap);
+            for (int t = 0; t < STEP / R; ++t) {
+                s[t] *= to_cap;
+                cap_tanh<T, FORM, REGS<R>>(s[t], a.softcap);
+                s[t] *= from_cap;
+            }
         }
         if (biased) {
             const int away = i + seq.shift - here - 4 * g;
@@ -304,9 +306,11 @@ static int launch_step(const tvl_attention_args& a, float* parts, hipStream_t st
 
 template <typename T>
 static int launch_step_t(const tvl_attention_args& a, float* parts, hipStream_t st) {
-    if (!step_wide(a)) return launch_step<T, 128, ODD>(a, parts, st);
-    if (a.dim <= 64) return featureless(a) ? launch_step<T, 64, PLAIN>(a, parts, st) : launch_step<T, 64, GENERAL>(a, parts, st);
-    return featureless(a) ? launch_step<T, 128, PLAIN>(a, parts, st) : launch_step<T, 128, GENERAL>(a, parts, st);
+    return with_form<T>(a, step_wide(a), [&](auto form) {
+        constexpr Form FORM = decltype(form)::value;
+        if constexpr (FORM == ODD) return launch_step<T, 128, ODD>(a, parts, st);
+        else return a.dim <= 64 ? launch_step<T, 64, FORM>(a, parts, st) : launch_step<T, 128, FORM>(a, parts, st);
+    });
 }
 
 int launch_attention_step(const tvl_attention_args& a, float* parts, hipStream_t st) {

@@ -10,6 +10,8 @@
 #pragma once
 #include "tvl_common.h"
 
+#include <type_traits>
+
 namespace tvl {
 
 constexpr int ATTENTION_MAX_DIM = 128;
@@ -256,14 +258,37 @@ template <int R> __device__ __forceinline__ float column_sum(float v) {
     return v;
 }
 
+// Forms of a kernel.  PLAIN: wide rows, no cap, no bias, no documents.  GENERAL: wide rows, all of them.  CAP_FAR: the same for 16-bit operands under a cap
+// above SHORT_CAP.  ODD: any rows.  (Both ways to cap in one form
+// spill more: 8192 causal tokens, 16 / 4 heads of 128, bf16, forward, capped at 50, 731 us against 543; capped at 65 758.)
+enum Form { PLAIN, GENERAL, CAP_FAR, ODD };
+
 // ---- what a query sees, and its scores ---------------------------------------------------------
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
-// tanh: 1 - 2 / (e^2y + 1) from one hardware exponential and reciprocal (2^-21 off at most) for 16-bit operands, the library's for float32
-template <typename T> __device__ __forceinline__ float cap_tanh(float y) {
-    if constexpr (sizeof(T) == 4) return tanhf(y);
-    return 1.0f - 2.0f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(y * (2.0f * LOG2E)) + 1.0f);
+// x = tanh(x) for N scores divided by the cap.  float32: the library's.  16-bit operands: 1 - 2 / (e^2x + 1) from one hardware
+// exponential and reciprocal, off by 2^-21 at most wherever x lies; times a cap of up to 64 that is 2^-15 of a power of e, a sixteenth of the
+// rounding of a float16 weight.  Larger caps meet scores that are small beside them, where only a relative error is small enough:
+// (1 - e) / (1 + e) with e = exp(-2 |x|) from 1 on, and below it the continued fraction x / (1 + x^2 / (3 + x^2 / (5 + x^2 / (7 + x^2 / 9)))), 2^-24 off
+// at 1.
+constexpr float SHORT_CAP = 64.0f;
+template <typename T, Form FORM, int N, typename V> __device__ __forceinline__ void cap_tanh(V& x, float cap) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = tanhf(x[i]);
+    } else if (FORM == GENERAL || (FORM == ODD && cap <= SHORT_CAP)) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = 1.0f - 2.0f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x[i] * (2.0f * LOG2E)) + 1.0f);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const float a = fabsf(x[i]), y = a * a, e = __builtin_amdgcn_exp2f(a * (-2.0f * LOG2E));
+            const bool low = a < 1.0f;
+            const float above = low ? a * __builtin_fmaf(y, y + 105.0f, 945.0f) : 1.0f - e, below = low ? __builtin_fmaf(y, __builtin_fmaf(15.0f, y, 420.0f), 945.0f) : 1.0f + e;
+            x[i] = copysignf(above * __builtin_amdgcn_rcpf(below), x[i]);
+        }
+    }
 }
 
 // float16 holds 2^15 and no digits below 2^-25: softmax weights rounded to it are formed 2^LIFT times as large, so that a long row's many small ones,
@@ -390,11 +415,16 @@ __device__ __forceinline__ Place place_of(uint32_t id, int pairs, int group, int
     return Place{(int)pair, (int)(rest % group), tiles - 1 - (int)(rest / group)};
 }
 
-// Forms of a kernel.  PLAIN: wide rows, no cap, no bias, no documents.  GENERAL: wide rows, all of them.  ODD: any rows.
-enum Form { PLAIN, GENERAL, ODD };
-
 // host side
 static inline bool featureless(const tvl_attention_args& a) { return a.softcap == 0.0f && a.slopes == nullptr && a.documents == nullptr && a.scale != 0.0f; }
+// launch(form) for the call, the form as a compile-time value
+template <typename T, typename F> static inline int with_form(const tvl_attention_args& a, bool wide, F launch) {
+    if (!wide) return launch(std::integral_constant<Form, ODD>{});
+    if (featureless(a)) return launch(std::integral_constant<Form, PLAIN>{});
+    if constexpr (sizeof(T) == 2)
+        if (a.softcap > SHORT_CAP) return launch(std::integral_constant<Form, CAP_FAR>{});
+    return launch(std::integral_constant<Form, GENERAL>{});
+}
 static inline bool wide_rows(const void* p, int64_t dim, int64_t batch, int64_t token, int64_t head, size_t z) {
     const int64_t per = (int64_t)(16 / z);
     return aligned(p, 16) && dim % per == 0 && batch % per == 0 && token % per == 0 && head % per == 0 && token * (int64_t)z < (int64_t)1 << 25;

@@ -6,15 +6,23 @@ Score gradients: every column (a query of dq, a key of dk) is multiplied by a po
 whatever other columns hold.
 
 Softmax weights: in the forward pass the largest weight of a row is 2^7 or more when float16 rounds it, so a small one is off by 2^-32 of the largest; the
-backward pass rounds 2^12 times the weight (at most 2^12), so by 2^-37."""
+backward pass rounds 2^12 times the weight (at most 2^12), so by 2^-37.
+
+Caps: 16-bit operands take a short tanh that is off by 2^-21 up to a cap of 64; beyond, and for float32, the error is relative: the quotient by the cap, the
+tanh (its own form and one hardware exponential and reciprocal) and the product with the cap are within 2^-20 of the capped score together."""
 import torch
 
 import attention_reference as R
 
 
 class Tight(R.Attention):
-    def __init__(self, q, k, v, see, *rest):
-        super().__init__(q, k, v, see, *rest)
+    def __init__(self, q, k, v, see, place, scale=None, softcap=0.0, slopes=None):
+        super().__init__(q, k, v, see, place, scale, softcap, slopes)
+        if softcap > (64.0 if self.dtype != torch.float32 else 0.0):
+            capped = softcap * torch.tanh(self.Q @ self.K.transpose(2, 3) * self.scale / softcap)
+            seen = torch.where(see[:, None], capped, torch.zeros_like(capped)).abs().amax(-1, keepdim=True)
+            before, self.ds = self.ds, torch.where(self.ds > 0, self.ds - softcap * 2.0 ** -21, self.ds) + 2.0 ** -20 * seen
+            self.out_tol = self.out_tol + 2 * (self.ds - before) * (self.p @ self.V.abs())
         if self.dtype == torch.float16:
             seen = see[:, None].double() @ self.V.abs()
             self.out_tol = self.out_tol - self.step * seen + 2.0 ** -32 * seen

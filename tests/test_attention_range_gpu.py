@@ -1,5 +1,5 @@
 """Attention where numbers of very different size meet: score gradients of large values, of losses that differ by many powers of ten between documents,
-tokens and queries; rows of many small weights: against float64 within the bounds of tests/attention_bounds.py."""
+tokens and queries; rows of many small weights, caps far above the scores: against float64 within the bounds of tests/attention_bounds.py."""
 import math
 import os
 import sys
@@ -32,13 +32,13 @@ def within(got, want, tol, what):
     R.within(torch.where(beyond, want, got.double()), want, tol, what)
 
 
-def run_training(tv, dev, q, k, v, go, causal=False, documents=None, softcap=0.0, prefix=None, scale=None):
+def run_training(tv, dev, q, k, v, go, causal=False, documents=None, softcap=0.0, prefix=None, scale=None, slopes=None):
     """Result and gradients within Tight's bounds; returns them."""
     b, tq, tk = q.shape[0], q.shape[1], k.shape[1]
     see, place = R.sees(b, tq, tk, causal, torch.full((b,), prefix or 0), documents)
-    ref = Tight(q, k, v, see, place, scale, softcap)
-    leaves = [x.to(dev).requires_grad_(True) for x in (q, k, v)]
-    out = tv.attention(*leaves, causal=causal, softcap=softcap, prefix=prefix, scale=scale, documents=None if documents is None else documents.to(dev))
+    ref = Tight(q, k, v, see, place, scale, softcap, slopes)
+    leaves = [x.clone().to(dev).requires_grad_(True) for x in (q, k, v)]
+    out = tv.attention(*leaves, causal=causal, softcap=softcap, prefix=prefix, scale=scale, slopes=None if slopes is None else slopes.to(dev), documents=None if documents is None else documents.to(dev))
     within(out, *ref.forward(), what="out")
     grads = torch.autograd.grad(out, leaves, go.to(dev))
     for name, got, (want, tol) in zip(("dq", "dk", "dv"), grads, ref.grads(go)):
@@ -157,3 +157,22 @@ def test_value_gradients_of_many_small_weights(tv, dev, kind, d, away):
     k[:, 3, :, 0] = 0.0
     go = torch.ones(1, 700, 2, d, dtype=TYPES[kind]) * 50
     run_training(tv, dev, q, k, v, go, scale=1.0)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("softcap", [64.0, 65.0, 1e3, 1e5, 1e7])
+@pytest.mark.parametrize("d", [64, 128])
+def test_caps_far_above_the_scores(tv, dev, kind, softcap, d):
+    """A cap bends the scores near it and leaves the others alone, whatever its size."""
+    dt = TYPES[kind]
+    g = torch.Generator().manual_seed(101 + d)
+    for spread, slopes in ((1.0, None), (8.0, torch.tensor([0.5, 0.01, 0.0, 0.1]))):
+        q, k, v, go = (normal(g, 2, 110, h, d, dtype=dt, scale=s) for h, s in ((4, spread), (2, 1.0), (2, 1.0), (4, 0.02)))
+        run_training(tv, dev, q, k, v, go, causal=True, softcap=softcap, slopes=slopes)
+        see, place = R.sees(2, 3, 110, True, torch.zeros(2, dtype=torch.int64), None, torch.tensor([107, 40]), torch.tensor([3, 3]))
+        want, tol = Tight(q[:, :3], k, v, see, place, None, softcap, slopes).forward()
+        cache = [x.transpose(1, 2).contiguous().to(dev) for x in (k, v)]
+        within(tv.cached_attention(q[:, :3].to(dev), *cache, torch.tensor([107, 40], device=dev), softcap=softcap, slopes=None if slopes is None else slopes.to(dev)), want, tol, "cached")
+    # scores near and beyond the cap
+    q, k, v, go = (normal(g, 1, 60, h, d, dtype=dt, scale=s) for h, s in ((2, softcap ** 0.5 if softcap <= 1e5 else 1.0), (2, softcap ** 0.5 if softcap <= 1e5 else 1.0), (2, 1.0), (2, 0.02)))
+    run_training(tv, dev, q, k, v, go, causal=True, softcap=softcap)
