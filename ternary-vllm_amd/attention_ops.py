@@ -17,6 +17,7 @@ import struct
 from typing import Optional, Union
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import custom_ops_mod as ops
@@ -54,6 +55,12 @@ def _vector(t: torch.Tensor, n: int, dtype: torch.dtype, device: torch.device, n
 def _same(t: torch.Tensor, like: torch.Tensor, name: str) -> None:
     if t.dtype != like.dtype or t.device != like.device:
         raise ValueError(f"{name}: {t.dtype} on {t.device}, the other operands are {like.dtype} on {like.device}")
+
+
+def _no_tangents(name: str, *tensors) -> None:
+    """Forward-mode derivatives are not formed: refused, where they would vanish silently."""
+    if forward_ad._current_level >= 0 and any(isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{name}: no forward-mode derivatives: pass tensors without tangents")
 
 
 # the current stream's handle without a Stream object around it (3 us less a call)
@@ -178,6 +185,7 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, table: torch.Tensor, interl
     ``interleaved``.  ``positions``: int64 ``[tokens]`` or ``[batch, tokens]``; ``table``: :func:`rotary_table`.  A position outside the table gives
     a row of NaN.  The rotation is evaluated in float32 and rounded once.  Query and key heads that lie next to each other (a joint projection) go as
     one tensor.  Differentiable in ``x``."""
+    _no_tangents("rotary", x, table)
     x = _heads(x, "rotary(x)")
     b, t, h, d = x.shape
     ops._gpu(positions, "rotary(positions)")
@@ -246,6 +254,7 @@ def rotary_cache(qkv: torch.Tensor, table: torch.Tensor, k_cache: torch.Tensor, 
     slot ``cache_len + t``: an int, or an int64 tensor of one value or ``[batch]``.  ``count`` (int64 ``[batch]``): how many of the ``tokens`` are real; the
     rows behind are zero in the result and nothing of them is written.  A position that is negative or beyond table or cache gives a
     row of NaN and writes nothing (an int ``cache_len`` is checked here instead).  No gradients."""
+    _no_tangents("rotary_cache", qkv, table, k_cache, v_cache)
     ops._gpu(qkv, "rotary_cache(qkv)")
     if qkv.dim() != 3 or qkv.dtype not in _FLOATS:
         raise ValueError(f"rotary_cache: qkv must be a float [batch, tokens, channels] tensor, got {tuple(qkv.shape)} {qkv.dtype}")
@@ -370,6 +379,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool = 
     ``causal``: query i sees keys ``j <= p``; with ``prefix`` (an int, or int64 ``[batch]``) also every ``j < prefix`` (an image or prompt that sees itself
     whole).  ``documents`` (int64 ``[batch, tokens]``, queries == keys): only keys of the query's own document are seen; a negative document is padding.
     A query that sees nothing gives zeros and passes no gradient."""
+    _no_tangents("attention", q, k, v, slopes)
     q, k, v = _heads(q, "attention(q)"), _heads(k, "attention(k)"), _heads(v, "attention(v)")
     b, tq, hq, d = q.shape
     _same(k, q, "attention(k)")
@@ -406,6 +416,7 @@ def cached_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     at slot ``cache_len + i`` and sees the slots up to its own, and with ``prefix`` (an int, or int64 ``[batch]``) every slot below it that
     holds a token.  ``scale``, ``softcap`` and ``slopes`` as for :func:`attention`.  Rows behind ``count`` are zero; a token whose slot is negative or beyond
     the cache gives a row of NaN (an int ``cache_len`` is checked here instead).  Only the filled part of the cache is read.  No gradients."""
+    _no_tangents("cached_attention", q, k_cache, v_cache, slopes)
     q = _heads(q, "cached_attention(q)")
     b, t, hq, d = q.shape
     if q.requires_grad and torch.is_grad_enabled():
