@@ -78,21 +78,44 @@ def _run(fn, device: torch.device, *args) -> None:
         ops._check(status)
 
 
-def _apply(fn, name: str, inputs, *rest) -> torch.Tensor:
-    """``fn.apply``, refused where recording it into a HIP graph would end the process: on a leaf whose gradient node was made by an
-    eager call on another stream and still lives, the backward pass would join that stream into the capture.  A node's own
-    metadata (it lives as long as the node) carries the stream of the call that made it."""
-    leaves = [x for x in inputs if x.requires_grad and x.is_leaf]
+def _held(leaf: torch.Tensor, stream: int) -> bool:
+    """Whether a graph that is alive holds the leaf's gradient node, other than one that calls recorded on `stream` made.  A leaf knows its node
+    weakly, so a mark on the node is there at the next look only if something else keeps the node alive."""
+    mark = object()
+    torch.autograd.graph.get_gradient_edge(leaf).node.metadata["tvl_mark"] = mark
+    metadata = torch.autograd.graph.get_gradient_edge(leaf).node.metadata
+    return metadata.pop("tvl_mark", None) is mark and metadata.get("tvl_stream") != stream
+
+
+def _recorded_leaves(name: str, *tensors: torch.Tensor):
+    """The leaves among the operands of a differentiable call that is being recorded into a HIP graph; refused where its backward pass would end the
+    process: a gradient node belongs to the stream of the operation that made it, whichever that was, and a captured backward pass that reaches a
+    node of another stream joins that stream into the capture.  Which stream a node belongs to cannot be asked, so only nodes that calls of this module
+    recorded on the same stream pass."""
+    if not torch.is_grad_enabled():
+        return ()
+    leaves = [x for x in tensors if isinstance(x, torch.Tensor) and x.requires_grad and x.is_leaf and x.is_cuda]
     if not leaves:
-        return fn.apply(*inputs, *rest)
-    stream = _raw_stream(inputs[0].device.index)
-    if torch.cuda.is_current_stream_capturing():
-        if any(torch.autograd.graph.get_gradient_edge(x).node.metadata.get("tvl_stream", stream) != stream for x in leaves):
-            raise RuntimeError(f"{name}: an eager graph of one of these leaves is still alive and belongs to another stream; its backward pass cannot be "
-                               "captured.  Delete or detach the eager results before the capture.")
-    y = fn.apply(*inputs, *rest)
-    for x in leaves:
-        torch.autograd.graph.get_gradient_edge(x).node.metadata.setdefault("tvl_stream", stream)
+        return ()
+    index = leaves[0].device.index
+    if torch.cuda.current_device() == index:
+        recording = torch.cuda.is_current_stream_capturing()
+    else:
+        with torch.cuda.device(index):
+            recording = torch.cuda.is_current_stream_capturing()
+    if not recording:
+        return ()
+    stream = _raw_stream(index)
+    if any(_held(x, stream) for x in leaves):
+        raise RuntimeError(f"{name}: another graph of one of these leaves is alive: an eager graph, whose gradient nodes belong to its own stream so that the backward pass "
+                           "cannot be captured (delete or detach the eager results before the capture), or another operation of this capture that took the leaf first")
+    return [(x, stream) for x in leaves]
+
+
+def _apply(fn, leaves, *args) -> torch.Tensor:
+    y = fn.apply(*args)
+    for x, stream in leaves:
+        torch.autograd.graph.get_gradient_edge(x).node.metadata["tvl_stream"] = stream
     return y
 
 
@@ -186,6 +209,7 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, table: torch.Tensor, interl
     a row of NaN.  The rotation is evaluated in float32 and rounded once.  Query and key heads that lie next to each other (a joint projection) go as
     one tensor.  Differentiable in ``x``."""
     _no_tangents("rotary", x, table)
+    leaves = _recorded_leaves("rotary", x)
     x = _heads(x, "rotary(x)")
     b, t, h, d = x.shape
     ops._gpu(positions, "rotary(positions)")
@@ -193,7 +217,7 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, table: torch.Tensor, interl
         raise ValueError(f"rotary: positions must be int64 [{t}] or [{b}, {t}] on {x.device}, got {tuple(positions.shape)} {positions.dtype} on {positions.device}")
     _check_table(table, d, x.device, "rotary")
     if x.requires_grad and torch.is_grad_enabled():
-        return _apply(_RotaryFn, "rotary", (x,), positions, table, bool(interleaved))
+        return _apply(_RotaryFn, leaves, x, positions, table, bool(interleaved))
     return _rotary(x, positions, table, interleaved, False)
 
 
@@ -380,6 +404,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool = 
     whole).  ``documents`` (int64 ``[batch, tokens]``, queries == keys): only keys of the query's own document are seen; a negative document is padding.
     A query that sees nothing gives zeros and passes no gradient."""
     _no_tangents("attention", q, k, v, slopes)
+    leaves = _recorded_leaves("attention", q, k, v)
     q, k, v = _heads(q, "attention(q)"), _heads(k, "attention(k)"), _heads(v, "attention(v)")
     b, tq, hq, d = q.shape
     _same(k, q, "attention(k)")
@@ -403,7 +428,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool = 
         if tq > 1 and documents.stride(1) != 1:
             documents = documents.contiguous()
     if (q.requires_grad or k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
-        return _apply(_AttentionFn, "attention", (q, k, v), bool(causal), scale, softcap, slopes, prefix if prefix is not None else value, documents)
+        return _apply(_AttentionFn, leaves, q, k, v, bool(causal), scale, softcap, slopes, prefix if prefix is not None else value, documents)
     return _attention(q, k, v, bool(causal), scale, softcap, slopes, at, value, documents, False)[0]
 
 

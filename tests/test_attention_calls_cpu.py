@@ -21,3 +21,18 @@ def test_forward_mode_derivatives_are_refused():
                 call()
             with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
                 call()
+
+
+def test_which_leaves_another_graph_holds():
+    """What a recorded call asks about its leaves: a node that lives because some graph holds it, whichever operation made it, unless marked as of the same stream."""
+    held = tv.attention_ops._held
+    x = torch.zeros(3, requires_grad=True)
+    assert not held(x, 7) and not held(x, 7)             # asking leaves nothing behind
+    y = x * 2
+    assert held(x, 7) and held(x, 7)
+    torch.autograd.graph.get_gradient_edge(x).node.metadata["tvl_stream"] = 7
+    assert not held(x, 7) and held(x, 8)
+    del y
+    assert not held(x, 8)
+    (x * 2).sum().backward()
+    assert not held(x, 7)

@@ -27,3 +27,59 @@ def test_forward_mode_is_refused_and_a_dual_level_changes_nothing(tv, dev):
         (g,) = torch.autograd.grad(tv.attention(y, x, x).sum(), y)
     (h,) = torch.autograd.grad(tv.attention(y, x, x).sum(), y)
     assert torch.equal(g, h)
+
+
+def test_capture_beside_a_live_graph_of_other_operations_is_refused(tv, dev):
+    """The leaf's gradient node was made by another operation of torch, on another stream than the captured one: refused, also if an eager call of
+    this module has used the leaf since; once those graphs are gone the capture works."""
+    q, k, v = (torch.randn(1, 20, 2, 64, device=dev, requires_grad=True) for _ in range(3))
+    table, pos, go = tv.rotary_table(32, 20, device=dev), torch.arange(20, device=dev), torch.randn(1, 20, 2, 64, device=dev)
+    odd = torch.randn(1, 20, 2, 128, device=dev)[..., ::2].detach().requires_grad_(True)       # copied inside the call
+    s = torch.cuda.Stream()
+    for call, leaf in ((lambda: tv.attention(q, k, v), q), (lambda: tv.attention(q, k, v), v), (lambda: tv.rotary(q, pos, table), q), (lambda: tv.rotary(odd, pos, table), odd)):
+        alive = leaf * 2
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            more = call()
+        torch.cuda.current_stream().wait_stream(s)
+        with pytest.raises(RuntimeError, match="alive"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=s):
+                call()
+        want = more.detach().clone()
+        (grad,) = torch.autograd.grad(more, leaf, go)
+        del alive, more
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            out = call()
+            (got,) = torch.autograd.grad(out, leaf, go)
+        for _ in range(3):
+            out.detach().zero_()
+            got.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want) and torch.equal(got, grad)
+        del out, got, graph
+
+
+def test_a_leaf_taken_twice_in_one_capture(tv, dev):
+    """Calls of one capture that share leaves, and a second capture on the same stream while the first one's graph is alive."""
+    x = torch.randn(1, 20, 4, 64, device=dev, requires_grad=True)
+    table, pos, go = tv.rotary_table(32, 20, device=dev), torch.arange(20, device=dev), torch.randn(1, 20, 4, 64, device=dev)
+
+    def step():
+        y = tv.attention(tv.rotary(x, pos, table), x, x, causal=True) + tv.attention(x, x, x)
+        return [y, *torch.autograd.grad(y, x, go)]
+
+    want = [y.detach().clone() for y in step()]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    graphs, outs = [], []
+    for _ in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=s):
+            outs.append(step())
+    for n in range(4):
+        graphs[n % 2].replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(want, outs[n % 2])), n
