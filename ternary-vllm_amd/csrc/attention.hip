@@ -29,9 +29,11 @@ static int check(const tvl_attention_args* a, const char* who, bool cached) {
     TVL_REQUIRE(a->heads > 0 && a->kv_heads > 0 && a->heads % a->kv_heads == 0, "%s: heads=%lld must be a multiple of kv_heads=%lld", who, (long long)a->heads, (long long)a->kv_heads);
     TVL_REQUIRE(a->dim >= 1 && a->dim <= ATTENTION_MAX_DIM, "%s: head dim %lld outside [1, %d]", who, (long long)a->dim, ATTENTION_MAX_DIM);
     TVL_REQUIRE(a->heads <= (1 << 16) && a->batch <= (1 << 20) && a->queries <= (1 << 30) && a->keys <= (1 << 30), "%s: batch, heads or tokens too large", who);
-    // every launch stays under 2^32 threads: at least 64 rows for each 256 of them, a cache's steps 16 rows for 512
-    const int64_t most = cached || a->queries > a->keys ? a->queries : a->keys;
-    TVL_REQUIRE(a->batch * a->heads * ceil_div(most, cached ? 16 : 64) < ((int64_t)1 << (cached ? 23 : 24)), "%s: too many rows for one launch", who);
+    // every launch stays under 2^32 threads: at least 64 rows for each 256 of them, a cache's steps 16 rows for 512, the gradient kernels 128 rows for up
+    // to 512, which a forward call that is asked for the log-sums is held to as well
+    const int64_t most = cached || a->queries > a->keys ? a->queries : a->keys, pairs = a->batch * a->heads;
+    TVL_REQUIRE(pairs * ceil_div(most, cached ? 16 : 64) < ((int64_t)1 << (cached ? 23 : 24)) && (cached || a->lse == nullptr || pairs * ceil_div(most, 128) < ((int64_t)1 << 23)),
+                "%s: too many rows for one launch", who);
     TVL_REQUIRE(a->scale == a->scale && a->scale - a->scale == 0.0f, "%s: scale must be finite", who);
     TVL_REQUIRE(a->softcap >= 0.0f && a->softcap - a->softcap == 0.0f, "%s: softcap must be finite and not negative", who);
     TVL_REQUIRE(cached || a->documents == nullptr || a->queries == a->keys, "%s: documents need as many queries as keys", who);

@@ -1,9 +1,14 @@
 """Calls of the attention operators that are refused, without a GPU."""
+import os
+import sys
+
 import pytest
 import torch
 from torch.autograd import forward_ad
 
-import ternary_vllm_amd as tv
+sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
+import ternary_vllm_amd as tv  # noqa: E402
+from test_attention_cpu import P, attention_args, grads_args  # noqa: E402
 
 
 def test_forward_mode_derivatives_are_refused():
@@ -36,3 +41,14 @@ def test_which_leaves_another_graph_holds():
     assert not held(x, 8)
     (x * 2).sum().backward()
     assert not held(x, 7)
+
+
+@pytest.mark.parametrize("batch,heads,tokens", [(1 << 20, 12, 1), (1 << 19, 16, 1), (1 << 20, 8, 64), (1 << 15, 16, 2048), (1, 8, 1 << 27)])
+def test_gradient_launches_beyond_the_grid_are_refused(batch, heads, tokens):
+    """The gradient kernels start up to 512 threads for every 128 rows: 2^32 threads are refused before anything is launched, by the forward call that
+    precedes them too."""
+    lib = tv.custom_ops_mod._lib
+    for dim in (64, 128):
+        a = attention_args(batch=batch, heads=heads, kv_heads=heads, queries=tokens, keys=tokens, dim=dim, o_batch=tokens * heads * dim, o_token=heads * dim, o_head=dim)
+        assert lib.tvl_attention_backward(a, grads_args(), P, 1 << 62, None) == 1 and b"too many" in lib.tvl_last_error()
+        assert lib.tvl_attention(a, None, 0, None) == 1 and b"too many" in lib.tvl_last_error()
