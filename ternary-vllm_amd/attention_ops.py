@@ -277,7 +277,8 @@ def rotary_cache(qkv: torch.Tensor, table: torch.Tensor, k_cache: torch.Tensor, 
     with more channels behind, is fine).  ``cache_len``: tokens of each sequence that are in the cache already, so token ``t`` gets position and
     slot ``cache_len + t``: an int, or an int64 tensor of one value or ``[batch]``.  ``count`` (int64 ``[batch]``): how many of the ``tokens`` are real; the
     rows behind are zero in the result and nothing of them is written.  A position that is negative or beyond table or cache gives a
-    row of NaN and writes nothing (an int ``cache_len`` is checked here instead).  No gradients."""
+    row of NaN and writes nothing: a table shorter than the cache leaves slots unwritten.  Without ``count``, an int ``cache_len`` whose tokens do not fit the
+    cache raises instead (the table's end is not looked at).  No gradients."""
     _no_tangents("rotary_cache", qkv, table, k_cache, v_cache)
     ops._gpu(qkv, "rotary_cache(qkv)")
     if qkv.dim() != 3 or qkv.dtype not in _FLOATS:
@@ -440,7 +441,7 @@ def cached_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     ``q [batch, tokens, heads, dim]``; caches ``[batch, kv_heads, slots, dim]``; ``cache_len`` and ``count`` as for :func:`rotary_cache`: token i of a sequence sits
     at slot ``cache_len + i`` and sees the slots up to its own, and with ``prefix`` (an int, or int64 ``[batch]``) every slot below it that
     holds a token.  ``scale``, ``softcap`` and ``slopes`` as for :func:`attention`.  Rows behind ``count`` are zero; a token whose slot is negative or beyond
-    the cache gives a row of NaN (an int ``cache_len`` is checked here instead).  Only the filled part of the cache is read.  No gradients."""
+    the cache gives a row of NaN (without ``count``, an int ``cache_len`` whose tokens do not fit raises instead).  Only the filled part of the cache is read.  No gradients."""
     _no_tangents("cached_attention", q, k_cache, v_cache, slopes)
     q = _heads(q, "cached_attention(q)")
     b, t, hq, d = q.shape
