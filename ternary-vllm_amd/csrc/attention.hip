@@ -54,6 +54,14 @@ static bool sized(const tvl_attention_args* a) {
            a->dim >= 1 && a->dim <= ATTENTION_MAX_DIM;
 }
 
+// A cap so far above every score that it bends none by a bit (its share of a score below 2^87 is under 2^-26 of it) is no cap: the quotient and the product with it
+// would leave float32's range.
+static tvl_attention_args without_far_cap(const tvl_attention_args& a) {
+    tvl_attention_args b = a;
+    if (b.softcap > 0x1p100f) b.softcap = 0.0f;
+    return b;
+}
+
 // parts of a workspace, each a multiple of 256 bytes
 static size_t round256(size_t v) { return (v + 255) & ~size_t(255); }
 static bool any_rows(const tvl_attention_args& a) { return a.queries > 0; }
@@ -88,7 +96,7 @@ int tvl_attention(const tvl_attention_args* a, void* workspace, size_t workspace
     DocumentSpan* spans = a->documents ? static_cast<DocumentSpan*>(workspace) : nullptr;
     if (spans)
         if (const int rc = launch_document_spans(*a, spans, st); rc != TVL_OK) return rc;
-    return launch_attention_forward(*a, false, spans, st);
+    return launch_attention_forward(without_far_cap(*a), false, spans, st);
 }
 
 size_t tvl_attention_backward_workspace_bytes(const tvl_attention_args* a) {
@@ -112,7 +120,7 @@ int tvl_attention_backward(const tvl_attention_args* a, const tvl_attention_grad
     float* slabs = reinterpret_cast<float*>(at + span_bytes(*a) + delta_bytes(*a));
     if (spans)
         if (const int rc = launch_document_spans(*a, spans, st); rc != TVL_OK) return rc;
-    return launch_attention_backward(*a, *g, spans, delta, slabs, st);
+    return launch_attention_backward(without_far_cap(*a), *g, spans, delta, slabs, st);
 }
 
 size_t tvl_cached_attention_workspace_bytes(const tvl_attention_args* a) {
@@ -124,7 +132,8 @@ int tvl_cached_attention(const tvl_attention_args* a, void* workspace, size_t wo
     if (a->batch == 0 || a->queries == 0) return TVL_OK;
     if (const int rc = check_workspace("cached_attention", tvl_cached_attention_workspace_bytes(a), workspace, workspace_bytes); rc != TVL_OK) return rc;
     hipStream_t st = (hipStream_t)stream;
-    return attention_step_serves(*a) ? launch_attention_step(*a, static_cast<float*>(workspace), st) : launch_attention_forward(*a, true, nullptr, st);
+    const tvl_attention_args b = without_far_cap(*a);
+    return attention_step_serves(b) ? launch_attention_step(b, static_cast<float*>(workspace), st) : launch_attention_forward(b, true, nullptr, st);
 }
 
 }  // extern "C"

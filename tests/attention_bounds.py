@@ -18,14 +18,19 @@ import attention_reference as R
 class Tight(R.Attention):
     def __init__(self, q, k, v, see, place, scale=None, softcap=0.0, slopes=None):
         super().__init__(q, k, v, see, place, scale, softcap, slopes)
+        b, tq, tk, hq, hk, d = self.shape
+        F32, m, half = R.F32, see[:, None], self.dtype == torch.float16
         if softcap > (64.0 if self.dtype != torch.float32 else 0.0):
+            # the reference's score error with this one in place of 2^-21 of the cap (not by a difference: a cap of 1e38 leaves nothing beside it)
+            size = self.Q.abs() @ self.K.abs().transpose(2, 3) * abs(self.scale)
             capped = softcap * torch.tanh(self.Q @ self.K.transpose(2, 3) * self.scale / softcap)
-            seen = torch.where(see[:, None], capped, torch.zeros_like(capped)).abs().amax(-1, keepdim=True)
-            before, self.ds = self.ds, torch.where(self.ds > 0, self.ds - softcap * 2.0 ** -21, self.ds) + 2.0 ** -20 * seen
-            self.out_tol = self.out_tol + 2 * (self.ds - before) * (self.p @ self.V.abs())
-        if self.dtype == torch.float16:
-            seen = see[:, None].double() @ self.V.abs()
-            self.out_tol = self.out_tol - self.step * seen + 2.0 ** -32 * seen
+            bias = slopes.double()[None, :, None, None] * (place[:, :, None] - torch.arange(tk)).abs().double()[:, None] if slopes is not None else torch.zeros_like(capped)
+            ds = F32 * ((d + 8) * size + 8 * (bias + 1) + 4 * (capped - bias).abs()) + 2.0 ** -20 * capped.abs()
+            self.ds = torch.where(m, ds, torch.zeros_like(ds)).amax(-1, keepdim=True)
+        W = self.p @ self.V.abs()
+        self.out_tol = self.u * (W + self.out.abs()) * 1.01 + (2 * self.ds + (tk + 16) * F32) * W + 1e-30
+        if half:
+            self.out_tol = self.out_tol + 2.0 ** -32 * (m.double() @ self.V.abs()) + 2.0 ** -25
 
     def grads(self, go):
         b, tq, tk, hq, hk, d = self.shape

@@ -176,3 +176,17 @@ def test_caps_far_above_the_scores(tv, dev, kind, softcap, d):
     # scores near and beyond the cap
     q, k, v, go = (normal(g, 1, 60, h, d, dtype=dt, scale=s) for h, s in ((2, softcap ** 0.5 if softcap <= 1e5 else 1.0), (2, softcap ** 0.5 if softcap <= 1e5 else 1.0), (2, 1.0), (2, 0.02)))
     run_training(tv, dev, q, k, v, go, causal=True, softcap=softcap)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("softcap", [2.0 ** 100, 1e38, 3.4e38])
+def test_caps_at_the_end_of_float32(tv, dev, kind, softcap):
+    dt = TYPES[kind]
+    g = torch.Generator().manual_seed(103)
+    q, k, v, go = (normal(g, 1, 70, h, 64, dtype=dt, scale=s) for h, s in ((4, 1.0), (2, 1.0), (2, 1.0), (4, 0.02)))
+    run_training(tv, dev, q, k, v, go, causal=True, softcap=softcap)
+    cache = [x.transpose(1, 2).contiguous().to(dev) for x in (k, v)]
+    for n in (1, 70):
+        see, place = R.sees(1, n, 70, True, torch.zeros(1, dtype=torch.int64), None, torch.tensor([70 - n]), torch.tensor([n]))
+        want, tol = Tight(q[:, :n], k, v, see, place, None, softcap).forward()
+        within(tv.cached_attention(q[:, :n].to(dev), *cache, 70 - n, softcap=softcap), want, tol, f"cached {n}")
