@@ -47,7 +47,7 @@ __device__ __forceinline__ void follow_range(const float (&ds)[N], Acc<R> (&acc)
 // before the first: whatever is not zero fits or moves it
 constexpr float FIT_START = 0x1p100f;
 
-// delta[row].  16 lanes per row, 16 bytes each: one read of both tensors, bound by HBM (A: 12 us, 5.6 TB/s; B: 11.7; C: 20 us, 3.9 TB/s).
+// delta[row] = sum over the head of out * grad_out, with the rounded output: one pass over two tensors in place of one over keys and values.  16 lanes per row, 16 bytes each: one read of both tensors, bound by HBM (A: 12 us, 5.6 TB/s; B: 11.7; C: 20 us, 3.9 TB/s).
 template <typename T, bool WIDE>
 __global__ void __launch_bounds__(256) attention_delta_kernel(tvl_attention_args a, tvl_attention_grads gr, float* __restrict__ delta, int blocks) {
     constexpr int PER = 16 / (int)sizeof(T);
@@ -75,10 +75,16 @@ __global__ void __launch_bounds__(256) attention_delta_kernel(tvl_attention_args
 // dq.  W waves x R queries; per 32 keys: S^T = K Q^T, dP^T = V dO^T, dS^T = P (dP - delta) bend (a lane holds one query), dQ^T += K^T dS^T.  Six operations per
 // pair and element.  A: 201 us (513 TFLOP/s), B: 386, C: 107.  The matrix cores are busy 39 % of the time at heads of 64 and 26 %
 // at 128: exponentials and conversions on the vector ALU and the operands' way out of LDS (no bank conflicts left) wait for each other with two waves per SIMD.
-template <typename T, int DP, Form FORM>
-__global__ void __launch_bounds__((64 * Shape<T, DP>::W), (Shape<T, DP>::OCCUPANCY)) attention_dq_kernel(tvl_attention_args a, tvl_attention_grads gr, const DocumentSpan* __restrict__ spans, const float* __restrict__ delta,
+//
+// delta' of the rounded output is off by its two roundings (weights, result), for rows whose weight lies on few keys as far as a score gradient's own rounding,
+// and all in one direction.  For 16-bit operands the sum of P (dP - delta') over a row, zero but for that error, is formed beside (`rest`, float32), and
+// sum of P bend K with it (`mean`, a product more out of the same operands): dq = scale (sum of dS K - rest mean), and delta = delta' + rest goes to the
+// pass over keys.
+// BARE: delta alone, for calls that want dk and dv only, so that they get the same bits.
+template <typename T, int DP, Form FORM, bool BARE>
+__global__ void __launch_bounds__((64 * Shape<T, DP>::W), (Shape<T, DP>::OCCUPANCY)) attention_dq_kernel(tvl_attention_args a, tvl_attention_grads gr, const DocumentSpan* __restrict__ spans, float* __restrict__ delta,
                                                            int tiles) {
-    constexpr bool WIDE = FORM != ODD;
+    constexpr bool WIDE = FORM != ODD, MEND = sizeof(T) == 2;
     constexpr int R = Shape<T, DP>::R, THREADS = 64 * Shape<T, DP>::W, QB = 128, CK = CHUNK<R>, N = VALUES<R>;
     typedef Tile<T, DP> L;
     typedef typename Operand<T>::elem E;
@@ -128,7 +134,8 @@ __global__ void __launch_bounds__((64 * Shape<T, DP>::W), (Shape<T, DP>::OCCUPAN
     const bool capped = FORM != PLAIN && a.softcap > 0.0f, biased = FORM != PLAIN && a.slopes != nullptr;
     const float to_log2 = a.scale * LOG2E, to_cap = capped ? a.scale / a.softcap : 0.0f, from_cap = a.softcap * LOG2E;
     const float pre = capped ? 1.0f : to_log2, unit = capped || biased ? 1.0f : to_log2;
-    Acc<R> acc[DP / R] = {};
+    Acc<R> acc[DP / R] = {}, mean[MEND && !BARE ? DP / R : 1] = {};
+    float rest = 0.0f;
 
     auto next = [&](int j) { return docs && j < reach ? docw.next(j / SPAN, (reach + SPAN - 1) / SPAN, lane) * SPAN : j; };
     const int lane_row = L::template lane_row<R>(lane), lane_col = L::template lane_column<R>(lane);
@@ -163,7 +170,7 @@ __global__ void __launch_bounds__((64 * Shape<T, DP>::W), (Shape<T, DP>::OCCUPAN
         auto piece = [&](int t) __attribute__((always_inline)) {
             const int jt = j0 + t;
             if (MASKED && jt >= wreach) return;
-            float s[N], dp[N];
+            float s[N], dp[N], bend[FORM == PLAIN ? 1 : N];
 #pragma unroll
             for (int n = 0; n < PIECE / R; ++n) {
                 Acc<R> u = {}, w = {};
@@ -175,14 +182,16 @@ __global__ void __launch_bounds__((64 * Shape<T, DP>::W), (Shape<T, DP>::OCCUPAN
 #pragma unroll
                 for (int x = 0; x < REGS<R>; ++x) { s[n * REGS<R> + x] = u[x]; dp[n * REGS<R> + x] = w[x]; }
             }
-            Frag<T> df[PIECE / CK];
+            [[maybe_unused]] Frag<T> df[PIECE / CK], pf[PIECE / CK];
             if (capped) {
 #pragma unroll
                 for (int x = 0; x < N; ++x) s[x] *= to_cap;
                 cap_tanh<T, FORM, N>(s, a.softcap);
 #pragma unroll
                 for (int x = 0; x < N; ++x) {
-                    dp[x] = product(dp[x] - dl, __builtin_fmaf(-s[x], s[x], 1.0f));
+                    bend[x] = __builtin_fmaf(-s[x], s[x], 1.0f);
+                    dp[x] -= dl;
+                    if constexpr (!MEND) dp[x] = product(dp[x], bend[x]);
                     s[x] *= from_cap;
                 }
             } else {
@@ -195,27 +204,56 @@ __global__ void __launch_bounds__((64 * Shape<T, DP>::W), (Shape<T, DP>::OCCUPAN
                 for (int x = 0; x < N; ++x) s[x] = __builtin_fmaf(-slope, fabsf((float)(here - piece_row<R>(x))), s[x] * pre);
             }
 #pragma unroll
-            for (int x = 0; x < N; ++x) dp[x] = product(dp[x], __builtin_amdgcn_exp2f(__builtin_fmaf(s[x], unit, -lse)));
+            for (int x = 0; x < N; ++x) {
+                s[x] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x], unit, -lse));
+                dp[x] = product(dp[x], s[x]);
+            }
             if (MASKED && (jt + PIECE > wall || !one_document)) {
+                auto hide = [&](int x) __attribute__((always_inline)) {
+                    dp[x] = 0.0f;
+                    if constexpr (MEND && !BARE) s[x] = 0.0f;
+                    if constexpr (MEND && !BARE && FORM != PLAIN) bend[x] = 0.0f;
+                };
                 const int left = mine - jt - 4 * g;
 #pragma unroll
                 for (int x = 0; x < N; ++x)
-                    if (piece_row<R>(x) >= left) dp[x] = 0.0f;
+                    if (piece_row<R>(x) >= left) hide(x);
                 if (!one_document) {
 #pragma unroll
                     for (int x = 0; x < N; ++x)
-                        if (!same_document(kdocs + t + 4 * g + piece_row<R>(x), doc)) dp[x] = 0.0f;
+                        if (!same_document(kdocs + t + 4 * g + piece_row<R>(x), doc)) hide(x);
+                }
+            }
+            if constexpr (MEND) {
+#pragma unroll
+                for (int x = 0; x < N; ++x) rest += dp[x];
+                if constexpr (BARE) return;
+                if constexpr (FORM != PLAIN) {
+                    if (capped) {
+#pragma unroll
+                        for (int x = 0; x < N; ++x) {
+                            dp[x] = product(dp[x], bend[x]);
+                            s[x] = product(s[x], bend[x]);
+                        }
+                    }
                 }
             }
             // score gradients are rounded to the operands' type for the last product; its sum is float32
             if constexpr (__is_same(T, f16)) follow_range<T, R>(dp, acc, fit);
 #pragma unroll
-            for (int x = 0; x < N; ++x) df[x / 8][x % 8] = (E)(__is_same(T, f16) ? product(dp[x], fit) : dp[x]);
+            for (int x = 0; x < N; ++x) {
+                df[x / 8][x % 8] = (E)(__is_same(T, f16) ? product(dp[x], fit) : dp[x]);
+                if constexpr (MEND) pf[x / 8][x % 8] = (E)s[x];
+            }
+            auto add = [&](int d, const Frag<T>& keys, int c) __attribute__((always_inline)) {
+                acc[d] = mma(keys, df[c], acc[d]);
+                if constexpr (MEND) mean[d] = mma(keys, pf[c], mean[d]);
+            };
             if (MASKED && (!one_document || (jt + PIECE > wall && wall < seq.end)) && holds_not_finite<T, DP, PIECE>(kt + t * L::ROW, lane)) {
 #pragma unroll
                 for (int c = 0; c < PIECE / CK; ++c)
 #pragma unroll
-                    for (int d = 0; d < DP / R; ++d) acc[d] = mma(finite_part<T>(L::template read_across<R>(kt + t * L::ROW, lane_col, c * CK, d)), df[c], acc[d]);
+                    for (int d = 0; d < DP / R; ++d) add(d, finite_part<T>(L::template read_across<R>(kt + t * L::ROW, lane_col, c * CK, d)), c);
 #pragma unroll 1
                 for (int row = 0; row < PIECE && jt + row < reach; ++row)
                     add_not_finite<T, DP, R>(kt, t + row, jt + row < mine && (one_document || (doc >= 0 && kdocs[t + row] == doc)), true, g, acc);
@@ -223,7 +261,7 @@ __global__ void __launch_bounds__((64 * Shape<T, DP>::W), (Shape<T, DP>::OCCUPAN
 #pragma unroll
                 for (int c = 0; c < PIECE / CK; ++c)
 #pragma unroll
-                    for (int d = 0; d < DP / R; ++d) acc[d] = mma(L::template read_across<R>(kt + t * L::ROW, lane_col, c * CK, d), df[c], acc[d]);
+                    for (int d = 0; d < DP / R; ++d) add(d, L::template read_across<R>(kt + t * L::ROW, lane_col, c * CK, d), c);
             }
         };
         piece(0);
@@ -242,15 +280,21 @@ __global__ void __launch_bounds__((64 * Shape<T, DP>::W), (Shape<T, DP>::OCCUPAN
         while (j0 < reach && clean(j0)) step(std::false_type{});
         while (j0 < reach && !clean(j0)) step(std::true_type{});
     }
-    if (i >= queries) return;
-    const float back = a.scale / fit;
+    if constexpr (MEND) {
+        rest = column_sum<R>(rest);
+        if (i < queries && g == 0) delta[((int64_t)b * a.heads + h) * queries + i] = dl + rest;
+    }
+    if (BARE || i >= queries) return;
+    const float back = a.scale / fit, off = -rest * a.scale;
     T* op = (T*)gr.dq + (((int64_t)b * queries + i) * a.heads + h) * dim;
 #pragma unroll
     for (int d = 0; d < DP / R; ++d)
 #pragma unroll
         for (int x = 0; x < REGS<R>; ++x) {
             const int col = d * R + result_row<R>(x, g);
-            if (col < dim) op[col] = from_float<T>(product(acc[d][x], back));
+            float v = product(acc[d][x], back);
+            if constexpr (MEND && !BARE) v = __builtin_fmaf(off, mean[d][x], v);
+            if (col < dim) op[col] = from_float<T>(v);
         }
 }
 
@@ -509,25 +553,34 @@ int attention_backward_parts(const tvl_attention_args& a) {
     return group;
 }
 
+template <typename T, int DP, Form FORM, bool BARE>
+static int launch_dq(const tvl_attention_args& a, const tvl_attention_grads& g, const DocumentSpan* spans, float* delta, hipStream_t st) {
+    const int64_t tiles = ceil_div(a.queries, 128);
+    const size_t bytes = 4 * GT * (size_t)Tile<T, DP>::ROW + (FORM == PLAIN ? 0 : 2 * GT * 8);
+    if (bytes > 65536) TVL_HIP_CHECK(hipFuncSetAttribute((const void*)attention_dq_kernel<T, DP, FORM, BARE>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+    hipLaunchKernelGGL((attention_dq_kernel<T, DP, FORM, BARE>), dim3((unsigned)(a.batch * a.heads * tiles)), dim3(64 * Shape<T, DP>::W), bytes, st, a, g, spans, delta, (int)tiles);
+    TVL_LAUNCH_CHECK();
+    return TVL_OK;
+}
+
 template <typename T, int DP, Form FORM>
-static int launch_gradients(const tvl_attention_args& a, const tvl_attention_grads& g, const DocumentSpan* spans, const float* delta, float* slabs, hipStream_t st) {
+static int launch_gradients(const tvl_attention_args& a, const tvl_attention_grads& g, const DocumentSpan* spans, float* delta, float* slabs, hipStream_t st) {
     if (g.dq && a.queries > 0) {
-        const int tiles = (int)ceil_div(a.queries, 128);
-        const size_t bytes = 4 * GT * (size_t)Tile<T, DP>::ROW + (FORM == PLAIN ? 0 : 2 * GT * 8);
-        if (bytes > 65536) TVL_HIP_CHECK(hipFuncSetAttribute((const void*)attention_dq_kernel<T, DP, FORM>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
-        hipLaunchKernelGGL((attention_dq_kernel<T, DP, FORM>), dim3((unsigned)(a.batch * a.heads * tiles)), dim3(64 * Shape<T, DP>::W), bytes, st, a, g, spans, delta, tiles);
-        TVL_LAUNCH_CHECK();
+        if (const int rc = launch_dq<T, DP, FORM, false>(a, g, spans, delta, st); rc != TVL_OK) return rc;
     }
+    if constexpr (sizeof(T) == 2)
+        if (!g.dq && g.dk && a.queries > 0 && a.keys > 0)
+            if (const int rc = launch_dq<T, DP, FORM, true>(a, g, spans, delta, st); rc != TVL_OK) return rc;
     if (g.dk && a.keys > 0) {
-        const int tiles = (int)ceil_div(a.keys, 128), parts = attention_backward_parts(a);
+        const int blocks = (int)ceil_div(a.keys, 128), parts = attention_backward_parts(a);
         const size_t bytes = 2 * (2 * GT * (size_t)Tile<T, DP>::ROW + 2 * GT * 4 + (FORM == PLAIN ? 0 : GT * 8));
         if (bytes > 65536) TVL_HIP_CHECK(hipFuncSetAttribute((const void*)attention_dkv_kernel<T, DP, FORM>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
-        hipLaunchKernelGGL((attention_dkv_kernel<T, DP, FORM>), dim3((unsigned)(a.batch * a.kv_heads * tiles * parts)), dim3(64 * Shape<T, DP>::W), bytes, st, a, g, spans, delta,
-                           tiles, parts, slabs);
+        hipLaunchKernelGGL((attention_dkv_kernel<T, DP, FORM>), dim3((unsigned)(a.batch * a.kv_heads * blocks * parts)), dim3(64 * Shape<T, DP>::W), bytes, st, a, g, spans, delta,
+                           blocks, parts, slabs);
         TVL_LAUNCH_CHECK();
         if (parts > 1) {
-            const int64_t n = a.batch * a.keys * a.kv_heads * a.dim, blocks = ceil_div(n, 256);
-            hipLaunchKernelGGL((attention_gather_kernel<T>), dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, st, slabs, parts, n, (T*)g.dk, (T*)g.dv);
+            const int64_t n = a.batch * a.keys * a.kv_heads * a.dim, most = ceil_div(n, 256);
+            hipLaunchKernelGGL((attention_gather_kernel<T>), dim3((unsigned)(most < 4096 ? most : 4096)), dim3(256), 0, st, slabs, parts, n, (T*)g.dk, (T*)g.dv);
             TVL_LAUNCH_CHECK();
         }
     }

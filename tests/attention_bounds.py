@@ -8,6 +8,8 @@ whatever other columns hold.
 Softmax weights: in the forward pass the largest weight of a row is 2^7 or more when float16 rounds it, so a small one is off by 2^-32 of the largest; the
 backward pass rounds 2^12 times the weight (at most 2^12), so by 2^-37.
 
+Delta: for 16-bit operands the sum of p dp in float32; the rounded output's part in it is corrected.
+
 Caps: 16-bit operands take a short tanh that is off by 2^-21 up to a cap of 64; beyond, and for float32, the error is relative: the quotient by the cap, the
 tanh (its own form and one hardware exponential and reciprocal) and the product with the cap are within 2^-20 of the capped score together."""
 import torch
@@ -46,6 +48,10 @@ class Tight(R.Attention):
         e_p = 2 * self.ds + (tk + 16) * F32
         e_dp = (d + 4) * F32 * (G.abs() @ V.abs().transpose(2, 3))
         e_delta = (G.abs() * (self.out_tol + u * self.out.abs())).sum(-1, keepdim=True) + (d + 4) * F32 * (G.abs() * self.out.abs()).sum(-1, keepdim=True)
+        off = e_delta
+        if self.dtype != torch.float32:
+            # the sum of p dp itself, in float32
+            e_delta = ((e_p + (tk + 16) * F32) * p * dp.abs() + p * e_dp).sum(-1, keepdim=True) + 8 * F32 * (delta.abs() + off)
         e = (e_p + u * 1.01) * core.abs() + p * (e_dp + e_delta) + 2.0 ** -19 * p * (dp - delta).abs() + 8 * F32 * p * (dp.abs() + delta.abs())
         size = core.abs() + e
         step = 2.0 ** -32 if half else 0.0
@@ -56,7 +62,9 @@ class Tight(R.Attention):
         ds = core * self.scale
         shared = lambda x: x.view(b, hk, n, tk, d).sum(2)
         dq, dk, dv = ds @ K, shared(ds.transpose(2, 3) @ Q), shared(p.transpose(2, 3) @ G)
-        dq_tol = e_q @ K.abs() + u * dq.abs() + least + (tk + 16) * F32 * (ds.abs() @ K.abs()) + 1e-30
+        # the correction of dq: what delta of the rounded output is off, times a mean of keys whose weights are rounded
+        mean = off * ((u * 1.01 * p + least * see) @ K.abs()) * abs(self.scale) if self.dtype != torch.float32 else 0.0
+        dq_tol = e_q @ K.abs() + mean + u * dq.abs() + least + (tk + 16) * F32 * (ds.abs() @ K.abs()) + 1e-30
         terms = n * tq + 16
         dk_tol = shared(e_k.transpose(2, 3) @ Q.abs()) + u * dk.abs() + least + terms * F32 * shared(ds.abs().transpose(2, 3) @ Q.abs()) + 1e-30
         e_w = (u * 1.01 + e_p) * p + (2.0 ** -37 * see if half else 0.0)

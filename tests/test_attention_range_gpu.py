@@ -190,3 +190,40 @@ def test_caps_at_the_end_of_float32(tv, dev, kind, softcap):
         see, place = R.sees(1, n, 70, True, torch.zeros(1, dtype=torch.int64), None, torch.tensor([70 - n]), torch.tensor([n]))
         want, tol = Tight(q[:, :n], k, v, see, place, None, softcap).forward()
         within(tv.cached_attention(q[:, :n].to(dev), *cache, 70 - n, softcap=softcap), want, tol, f"cached {n}")
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("b,t,causal,softcap", [(30, 2, True, 0.0), (30, 2, False, 4.0), (9, 3, True, 0.0), (4, 16, True, 3.0), (3, 65, False, 0.0), (2, 127, True, 0.0), (2, 127, False, 0.0)])
+def test_gradients_of_few_keys_keep_their_digits(tv, dev, kind, d, b, t, causal, softcap):
+    """Where a query sees few keys, the rounding of its result would be as large in its gradients as their own."""
+    g = torch.Generator().manual_seed(109 + t)
+    q, k, v, go = (normal(g, b, t, h, d, dtype=TYPES[kind], scale=s) for h, s in ((4, 1.0), (2, 1.0), (2, 1.0), (4, 0.02)))
+    _, dq, dk, dv = run_training(tv, dev, q, k, v, go, causal=causal, softcap=softcap)
+    for wanted in ((0,), (1,), (2,), (0, 2)):            # a gradient does not depend on which others are wanted
+        leaves = [x.clone().to(dev).requires_grad_(n in wanted) for n, x in enumerate((q, k, v))]
+        got = torch.autograd.grad(tv.attention(*leaves, causal=causal, softcap=softcap), [leaves[n] for n in wanted], go.to(dev))
+        assert all(torch.equal(x, (dq, dk, dv)[n]) for n, x in zip(wanted, got))
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("causal", [True, False])
+def test_gradients_of_short_documents_keep_their_digits(tv, dev, kind, causal):
+    """Documents of 1 to 90 tokens, in runs and interleaved, some padding between them."""
+    g = torch.Generator().manual_seed(113)
+    ids = torch.tensor(sum([[n] * s for n, s in enumerate((1, 2, 3, 60, 90, 5, 40, 64, 35))], []))
+    ids[70:74] = -1
+    for docs in (ids, torch.arange(300) % 7):
+        q, k, v, go = (normal(g, 1, 300, h, 64, dtype=TYPES[kind], scale=s) for h, s in ((2, 1.0), (2, 1.0), (2, 1.0), (2, 0.02)))
+        run_training(tv, dev, q, k, v, go, causal=causal, documents=docs[None])
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("softcap", [0.0, 20.0])
+def test_gradients_of_rows_whose_weight_lies_on_few_keys(tv, dev, kind, d, softcap):
+    """Long rows that a steep bias or large scores leave a few keys of."""
+    g = torch.Generator().manual_seed(127 + d)
+    for spread, slopes in ((0.5, torch.tensor([2.0, 1.0, 0.5, 0.25])), (4.0, None)):
+        q, k, v, go = (normal(g, 1, 400, h, d, dtype=TYPES[kind], scale=s) for h, s in ((4, spread), (2, 1.0), (2, 1.0), (4, 0.02)))
+        run_training(tv, dev, q, k, v, go, causal=True, softcap=softcap, slopes=slopes)
