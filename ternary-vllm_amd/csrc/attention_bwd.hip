@@ -294,6 +294,7 @@ __global__ void __launch_bounds__((64 * Shape<T, DP>::W), (Shape<T, DP>::OCCUPAN
             const int col = d * R + result_row<R>(x, g);
             float v = product(acc[d][x], back);
             if constexpr (MEND && !BARE) v = __builtin_fmaf(off, mean[d][x], v);
+            if (mine <= 1) v = 0.0f;      // a softmax over one key has no slope
             if (col < dim) op[col] = from_float<T>(v);
         }
 }
@@ -345,6 +346,8 @@ __global__ void __launch_bounds__((64 * Shape<T, DP>::W), (Shape<T, DP>::OCCUPAN
     const float pre = capped ? 1.0f : to_log2, unit = capped || biased ? 1.0f : to_log2;
     Acc<R> dk[DP / R] = {}, dv[DP / R] = {};
 
+    // queries in front of this one see key 0 at most: a softmax over one key has no slope
+    const int lone = keys <= 1 ? queries : (seq.causal && seq.prefix <= 1 ? 1 - seq.shift : 0);
     // query i sees key j from i = j - shift on (all of them for keys in the prefix)
     int begin = seq.causal && k0 >= seq.prefix ? k0 - seq.shift : 0;
     begin = begin < 0 ? 0 : begin / GT * GT;
@@ -447,9 +450,12 @@ __global__ void __launch_bounds__((64 * Shape<T, DP>::W), (Shape<T, DP>::OCCUPAN
             if (MASKED && masked) {
                 // query i = it + 4 g + row sees key j if j is in its sequence's prefix or not behind its place
                 const int from = j >= seq.end ? PIECE : (!seq.causal || j < seq.prefix ? -PIECE : j - seq.shift - it - 4 * g);
+                const int slope_from = kw == 0 && lone - it - 4 * g > from ? lone - it - 4 * g : from;
 #pragma unroll
-                for (int x = 0; x < N; ++x)
-                    if (piece_row<R>(x) < from) s[x] = dp[x] = 0.0f;
+                for (int x = 0; x < N; ++x) {
+                    if (piece_row<R>(x) < from) s[x] = 0.0f;
+                    if (piece_row<R>(x) < slope_from) dp[x] = 0.0f;
+                }
                 if (!one_document) {
 #pragma unroll
                     for (int x = 0; x < N; ++x)

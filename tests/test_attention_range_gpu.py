@@ -227,3 +227,21 @@ def test_gradients_of_rows_whose_weight_lies_on_few_keys(tv, dev, kind, d, softc
     for spread, slopes in ((0.5, torch.tensor([2.0, 1.0, 0.5, 0.25])), (4.0, None)):
         q, k, v, go = (normal(g, 1, 400, h, d, dtype=TYPES[kind], scale=s) for h, s in ((4, spread), (2, 1.0), (2, 1.0), (4, 0.02)))
         run_training(tv, dev, q, k, v, go, causal=True, softcap=softcap, slopes=slopes)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("softcap,slopes", [(0.0, False), (6.0, True)])
+def test_queries_of_one_key_have_no_score_gradient(tv, dev, kind, softcap, slopes):
+    """A softmax over one key is 1 whatever its score: zeros, not the rounding of a difference."""
+    g = torch.Generator().manual_seed(131)
+    sl = torch.tensor([0.5, 0.1, 0.01, 1.0]) if slopes else None
+    for b, tq, tk, causal, d in ((9, 1, 1, True, 64), (3, 1, 1, False, 128), (2, 70, 1, False, 64), (2, 150, 20, True, 64), (1, 40, 40, True, 33), (2, 300, 300, True, 128)):
+        q, k, v, go = (normal(g, b, t, h, d, dtype=TYPES[kind]) for t, h in ((tq, 4), (tk, 2), (tk, 2), (tq, 4)))
+        first = max(0, tq - tk) if causal else tq - 1                    # the last query that sees one key at most
+        if causal or tk == 1:
+            only = go.clone()
+            only[:, first + 1:] = 0                                      # gradients of those queries alone
+            _, dq, dk, _ = run_training(tv, dev, q, k, v, only, causal=causal, softcap=softcap, slopes=sl)
+            assert int(dq[:, : first + 1].count_nonzero()) == 0 and int(dk.count_nonzero()) == 0
+        _, dq, _, _ = run_training(tv, dev, q, k, v, go, causal=causal, softcap=softcap, slopes=sl)
+        assert int(dq[:, : first + 1].count_nonzero()) == 0
