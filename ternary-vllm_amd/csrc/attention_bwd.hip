@@ -21,31 +21,35 @@ template <typename T, int DP> struct Shape {
     static constexpr int R = DP == 64 && sizeof(T) == 2 ? 32 : 16, W = 128 / R, OCCUPANCY = 2;
 };
 
-// float16 score gradients are multiplied by a power of two `fit` in front of their rounding, one for every column (a query of dq, a key of dk), which
-// follows the largest one of the column so far: it is chosen so that this one lies in [2^7, 2^8), kept until one exceeds 2^15, and the column's sum
-// is rescaled when it moves, as a softmax's maximum is.  Nothing overflows however large values and output gradients are, a gradient below 2^-21 of
-// its column's largest is off by at most 2^-32 of that one, and no column depends on what another one holds.  (A power of two for a whole
-// sequence, from its largest output gradient, made infinities of large values and zeros of the gradients of small documents beside large ones.)
+// float16 score gradients (2^BACKWARD_LIFT times as large, as their weights are) are rounded in a range of their own for every column, a query of dq or a
+// key of dk, that follows the largest one of the column so far.  They stay as they are while that one lies in [1, 2^15]; else a power of two `fit` brings
+// it to [2^7, 2^8), and the column's sum is rescaled when that moves, as a softmax's maximum is.  Nothing overflows however large values and output
+// gradients are, a small one is off by at most 2^-25 of its column's largest, and no column depends on what another one holds.  (A power of two for
+// a whole sequence, from its largest output gradient, made infinities of large values and zeros of the gradients of small documents beside large ones.)
 // What is not finite spoils its own column.
-template <typename T, int R, int N, int D>
-__device__ __forceinline__ void follow_range(const float (&ds)[N], Acc<R> (&acc)[D], float& fit) {
-    float top = 0.0f;
+struct Range {
+    float fit = 1.0f, most = 0.0f;      // most: the largest one that fits
+    bool scaled = false;                // whether any lane's fit is not 1
+    template <int R, int N, int D> __device__ __forceinline__ void follow(const float (&ds)[N], Acc<R> (&acc)[D]) {
+        float top = 0.0f;
 #pragma unroll
-    for (int x = 0; x < N; ++x) top = fmaxf(top, fabsf(ds[x]));
-    top = column_max<R>(top);
-    const bool grow = top * fit > 32768.0f;
-    if (__any(grow)) {
-        // 2^(7 - exponent), not below 2^-100
-        const int e = (int)(__builtin_bit_cast(uint32_t, top) >> 23) - 127 - 7;
-        const float now = grow ? __builtin_bit_cast(float, (uint32_t)(127 - (e < 100 ? e : 100)) << 23) : fit;
-        const float shrink = now * __builtin_bit_cast(float, (254u << 23) - __builtin_bit_cast(uint32_t, fit));
-        fit = now;
+        for (int x = 0; x < N; ++x) top = fmaxf(top, fabsf(ds[x]));
+        if (__any(top > most)) {
+            top = column_max<R>(top);
+            float now = fit;
+            if (top > most) {
+                const int e = (int)(__builtin_bit_cast(uint32_t, top) >> 23) - 127 - 7;      // fit 2^-e, from 2^-100 to 2^100
+                now = top >= 1.0f && top <= 32768.0f ? 1.0f : __builtin_bit_cast(float, (uint32_t)(127 - (e < -100 ? -100 : (e > 100 ? 100 : e))) << 23);
+                most = __builtin_bit_cast(float, (269u << 23) - __builtin_bit_cast(uint32_t, now));      // 2^15 / fit
+            }
+            const float shrink = now * __builtin_bit_cast(float, (254u << 23) - __builtin_bit_cast(uint32_t, fit));
+            fit = now;
+            scaled = __any(fit != 1.0f);
 #pragma unroll
-        for (int d = 0; d < D; ++d) acc[d] *= shrink;
+            for (int d = 0; d < D; ++d) acc[d] *= shrink;
+        }
     }
-}
-// before the first: whatever is not zero fits or moves it
-constexpr float FIT_START = 0x1p100f;
+};
 
 // delta[row] = sum over the head of out * grad_out, with the rounded output: one pass over two tensors in place of one over keys and values.  16 lanes per row, 16 bytes each: one read of both tensors, bound by HBM (A: 12 us, 5.6 TB/s; B: 11.7; C: 20 us, 3.9 TB/s).
 template <typename T, bool WIDE>
@@ -115,6 +119,7 @@ __global__ void __launch_bounds__((64 * Shape<T, DP>::W), (Shape<T, DP>::OCCUPAN
         docw.start(spans + (int64_t)b * ((queries + SPAN - 1) / SPAN), queries, q0, QB);
     }
     Frag<T> qf[DP / CK], gf[DP / CK];
+    constexpr float UP = BACKWARD_LIFT<T>, DOWN = 1.0f / (float)(1 << (int)UP);      // weights and score gradients are formed 2^UP times as large
     float lse = 0.0f, dl = 0.0f;
 #pragma unroll
     for (int c = 0; c < DP / CK; ++c) {
@@ -126,10 +131,10 @@ __global__ void __launch_bounds__((64 * Shape<T, DP>::W), (Shape<T, DP>::OCCUPAN
     }
     if (i < queries) {
         const int64_t row = ((int64_t)b * a.heads + h) * queries + i;
-        lse = a.lse[row] * LOG2E;
+        lse = a.lse[row] * LOG2E - UP;
         dl = delta[row];
     }
-    float fit = __is_same(T, f16) ? FIT_START : 1.0f;
+    Range range;
     const float slope = a.slopes ? a.slopes[h] * LOG2E : 0.0f;
     const bool capped = FORM != PLAIN && a.softcap > 0.0f, biased = FORM != PLAIN && a.slopes != nullptr;
     const float to_log2 = a.scale * LOG2E, to_cap = capped ? a.scale / a.softcap : 0.0f, from_cap = a.softcap * LOG2E;
@@ -238,30 +243,45 @@ __global__ void __launch_bounds__((64 * Shape<T, DP>::W), (Shape<T, DP>::OCCUPAN
                     }
                 }
             }
-            // score gradients are rounded to the operands' type for the last product; its sum is float32
-            if constexpr (__is_same(T, f16)) follow_range<T, R>(dp, acc, fit);
+            // keys across, for both products; what is not finite in them must not reach queries that do not see it
+            const bool spoilt = MASKED && (!one_document || (jt + PIECE > wall && wall < seq.end)) && holds_not_finite<T, DP, PIECE>(kt + t * L::ROW, lane);
+            Frag<T> across[PIECE / CK][DP / R];
 #pragma unroll
-            for (int x = 0; x < N; ++x) {
-                df[x / 8][x % 8] = (E)(__is_same(T, f16) ? product(dp[x], fit) : dp[x]);
-                if constexpr (MEND) pf[x / 8][x % 8] = (E)s[x];
-            }
-            auto add = [&](int d, const Frag<T>& keys, int c) __attribute__((always_inline)) {
-                acc[d] = mma(keys, df[c], acc[d]);
-                if constexpr (MEND) mean[d] = mma(keys, pf[c], mean[d]);
-            };
-            if (MASKED && (!one_document || (jt + PIECE > wall && wall < seq.end)) && holds_not_finite<T, DP, PIECE>(kt + t * L::ROW, lane)) {
+            for (int c = 0; c < PIECE / CK; ++c)
+#pragma unroll
+                for (int d = 0; d < DP / R; ++d) across[c][d] = L::template read_across<R>(kt + t * L::ROW, lane_col, c * CK, d);
+            if (MASKED && spoilt) {
 #pragma unroll
                 for (int c = 0; c < PIECE / CK; ++c)
 #pragma unroll
-                    for (int d = 0; d < DP / R; ++d) add(d, finite_part<T>(L::template read_across<R>(kt + t * L::ROW, lane_col, c * CK, d)), c);
+                    for (int d = 0; d < DP / R; ++d) across[c][d] = finite_part<T>(across[c][d]);
+            }
+            // weights and score gradients are rounded to the operands' type for the last products; their sums are float32
+            if constexpr (MEND) {
+#pragma unroll
+                for (int x = 0; x < N; ++x) pf[x / 8][x % 8] = (E)s[x];
+#pragma unroll
+                for (int c = 0; c < PIECE / CK; ++c)
+#pragma unroll
+                    for (int d = 0; d < DP / R; ++d) mean[d] = mma(across[c][d], pf[c], mean[d]);
+            }
+            if constexpr (__is_same(T, f16)) {
+                range.follow<R>(dp, acc);
+                if (range.scaled) {
+#pragma unroll
+                    for (int x = 0; x < N; ++x) dp[x] = product(dp[x], range.fit);
+                }
+            }
+#pragma unroll
+            for (int x = 0; x < N; ++x) df[x / 8][x % 8] = (E)dp[x];
+#pragma unroll
+            for (int c = 0; c < PIECE / CK; ++c)
+#pragma unroll
+                for (int d = 0; d < DP / R; ++d) acc[d] = mma(across[c][d], df[c], acc[d]);
+            if (MASKED && spoilt) {
 #pragma unroll 1
                 for (int row = 0; row < PIECE && jt + row < reach; ++row)
                     add_not_finite<T, DP, R>(kt, t + row, jt + row < mine && (one_document || (doc >= 0 && kdocs[t + row] == doc)), true, g, acc);
-            } else {
-#pragma unroll
-                for (int c = 0; c < PIECE / CK; ++c)
-#pragma unroll
-                    for (int d = 0; d < DP / R; ++d) add(d, L::template read_across<R>(kt + t * L::ROW, lane_col, c * CK, d), c);
             }
         };
         piece(0);
@@ -281,11 +301,11 @@ __global__ void __launch_bounds__((64 * Shape<T, DP>::W), (Shape<T, DP>::OCCUPAN
         while (j0 < reach && !clean(j0)) step(std::true_type{});
     }
     if constexpr (MEND) {
-        rest = column_sum<R>(rest);
+        rest = column_sum<R>(rest) * DOWN;
         if (i < queries && g == 0) delta[((int64_t)b * a.heads + h) * queries + i] = dl + rest;
     }
     if (BARE || i >= queries) return;
-    const float back = a.scale / fit, off = -rest * a.scale;
+    const float back = a.scale / range.fit * DOWN, off = -rest * a.scale * DOWN;
     T* op = (T*)gr.dq + (((int64_t)b * queries + i) * a.heads + h) * dim;
 #pragma unroll
     for (int d = 0; d < DP / R; ++d)
@@ -339,7 +359,7 @@ __global__ void __launch_bounds__((64 * Shape<T, DP>::W), (Shape<T, DP>::OCCUPAN
             vf[c] = load_frag<T, WIDE>((const T*)a.v + b * a.v_batch + (int64_t)j * a.v_token + hk * a.v_head, g + (64 / R) * c, dim);
         }
     }
-    float fit = __is_same(T, f16) ? FIT_START : 1.0f;
+    Range range;
     constexpr float UP = BACKWARD_LIFT<T>;
     const bool capped = FORM != PLAIN && a.softcap > 0.0f, biased = FORM != PLAIN && a.slopes != nullptr;
     const float to_log2 = a.scale * LOG2E, to_cap = capped ? a.scale / a.softcap : 0.0f, from_cap = a.softcap * LOG2E;
@@ -463,34 +483,38 @@ __global__ void __launch_bounds__((64 * Shape<T, DP>::W), (Shape<T, DP>::OCCUPAN
                 }
             }
             // weights and score gradients are rounded to the operands' type for the last products; their sums are float32
-            if constexpr (__is_same(T, f16)) follow_range<T, R>(dp, dk, fit);
+            const bool spoilt = MASKED && masked && (holds_not_finite<T, DP, PIECE>(gt + t * L::ROW, lane) || holds_not_finite<T, DP, PIECE>(qt + t * L::ROW, lane));
+            auto across = [&](const char* tile, int c, int d) __attribute__((always_inline)) {
+                Frag<T> f = L::template read_across<R>(tile + t * L::ROW, lane_col, c * CK, d);
+                if (MASKED && spoilt) f = finite_part<T>(f);
+                return f;
+            };
 #pragma unroll
-            for (int x = 0; x < N; ++x) {
-                pf[x / 8][x % 8] = (E)s[x];
-                df[x / 8][x % 8] = (E)(__is_same(T, f16) ? product(dp[x], fit) : dp[x]);
+            for (int x = 0; x < N; ++x) pf[x / 8][x % 8] = (E)s[x];
+#pragma unroll
+            for (int c = 0; c < PIECE / CK; ++c)
+#pragma unroll
+                for (int d = 0; d < DP / R; ++d) dv[d] = mma(across(gt, c, d), pf[c], dv[d]);
+            if constexpr (__is_same(T, f16)) {
+                range.follow<R>(dp, dk);
+                if (range.scaled) {
+#pragma unroll
+                    for (int x = 0; x < N; ++x) dp[x] = product(dp[x], range.fit);
+                }
             }
-            if (MASKED && masked && (holds_not_finite<T, DP, PIECE>(gt + t * L::ROW, lane) || holds_not_finite<T, DP, PIECE>(qt + t * L::ROW, lane))) {
 #pragma unroll
-                for (int c = 0; c < PIECE / CK; ++c)
+            for (int x = 0; x < N; ++x) df[x / 8][x % 8] = (E)dp[x];
 #pragma unroll
-                    for (int d = 0; d < DP / R; ++d) {
-                        dv[d] = mma(finite_part<T>(L::template read_across<R>(gt + t * L::ROW, lane_col, c * CK, d)), pf[c], dv[d]);
-                        dk[d] = mma(finite_part<T>(L::template read_across<R>(qt + t * L::ROW, lane_col, c * CK, d)), df[c], dk[d]);
-                    }
+            for (int c = 0; c < PIECE / CK; ++c)
+#pragma unroll
+                for (int d = 0; d < DP / R; ++d) dk[d] = mma(across(qt, c, d), df[c], dk[d]);
+            if (MASKED && spoilt) {
 #pragma unroll 1
                 for (int row = 0; row < PIECE && it + row < queries; ++row) {
                     const bool sees = j < seq.limit(it + row) && (one_document || (doc >= 0 && qdocs[t + row] == doc));
                     add_not_finite<T, DP, R>(gt, t + row, sees, false, g, dv);
                     add_not_finite<T, DP, R>(qt, t + row, sees, true, g, dk);
                 }
-            } else {
-#pragma unroll
-                for (int c = 0; c < PIECE / CK; ++c)
-#pragma unroll
-                    for (int d = 0; d < DP / R; ++d) {
-                        dv[d] = mma(L::template read_across<R>(gt + t * L::ROW, lane_col, c * CK, d), pf[c], dv[d]);
-                        dk[d] = mma(L::template read_across<R>(qt + t * L::ROW, lane_col, c * CK, d), df[c], dk[d]);
-                    }
             }
         };
         piece(0);
@@ -513,7 +537,7 @@ __global__ void __launch_bounds__((64 * Shape<T, DP>::W), (Shape<T, DP>::OCCUPAN
         while (n < total && clean(n)) step(std::false_type{});
     }
     if (j >= keys) return;
-    const float down = 1.0f / (float)(1 << (int)UP), back = a.scale / fit * down;
+    const float down = 1.0f / (float)(1 << (int)UP), back = a.scale / range.fit * down;
     const int64_t row = (((int64_t)b * keys + j) * a.kv_heads + hk) * dim;
 #pragma unroll
     for (int d = 0; d < DP / R; ++d)

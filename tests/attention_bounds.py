@@ -1,9 +1,9 @@
 """Tighter element-wise bounds than tests/attention_reference.py where float16 loses digits: the size of its subnormal numbers counts relative to what the kernels
 scale by.
 
-Score gradients: every column (a query of dq, a key of dk) is multiplied by a power of two that brings its largest score gradient so far to 2^7 or more, up to
-2^15.  float16 holds multiples of 2^-24 at the lower end, so a rounding there is off by at most 2^-25 / 2^7 = 2^-32 of the column's own largest one,
-whatever other columns hold.
+Score gradients: every column (a query of dq, a key of dk) is rounded where its largest score gradient so far is between 1 and 2^15, or brought there by a
+power of two.  float16 holds multiples of 2^-24 at the lower end, so a rounding there is off by at most 2^-25 of the column's own largest one, whatever
+other columns hold.
 
 Softmax weights: in the forward pass the largest weight of a row is 2^7 or more when float16 rounds it, so a small one is off by 2^-32 of the largest; the
 backward pass rounds 2^12 times the weight (at most 2^12), so by 2^-37.
@@ -54,7 +54,7 @@ class Tight(R.Attention):
             e_delta = ((e_p + (tk + 16) * F32) * p * dp.abs() + p * e_dp).sum(-1, keepdim=True) + 8 * F32 * (delta.abs() + off)
         e = (e_p + u * 1.01) * core.abs() + p * (e_dp + e_delta) + 2.0 ** -19 * p * (dp - delta).abs() + 8 * F32 * p * (dp.abs() + delta.abs())
         size = core.abs() + e
-        step = 2.0 ** -32 if half else 0.0
+        step = 2.0 ** -25 if half else 0.0
         group = lambda x: x.view(b, hk, n, tq, tk)
         e_q = (e + step * size.amax(-1, keepdim=True) * see) * abs(self.scale)
         e_k = (e + step * group(size).amax((2, 3), keepdim=True).expand(b, hk, n, 1, tk).reshape(b, hq, 1, tk) * see) * abs(self.scale)
