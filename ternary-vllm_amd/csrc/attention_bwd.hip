@@ -1,5 +1,5 @@
 // Backward attention: delta = rowsum(out * grad_out), then dq per query tile and dk, dv per key tile.  The scores are formed again from
-// q, k and the saved log-sum, twice (14 instead of 10 operations per pair, head and element): every gradient is then summed in
+// q, k and the saved log-sum, twice (14 instead of 10 operations per pair, head and element, 16 for 16-bit operands): every gradient is then summed in
 // the registers of one workgroup, in a fixed order, without atomics.
 // GPU times below: A = 4 x 2048 causal tokens, 32 heads of 64, bf16; B = 8191 tokens in 7 documents, 16 / 4 heads of 128, capped, bf16; C = 128 x 197 tokens,
 // 12 heads of 64, f16.
@@ -14,9 +14,9 @@ template <int R> constexpr int VALUES = PIECE * R / 64;
 template <int R> __device__ __forceinline__ constexpr int piece_row(int x) { return x / REGS<R> * R + result_row<R>(x % REGS<R>, 0); }
 
 // Shape of a gradient kernel: W waves of R queries or keys each, 128 in all, its registers limited to OCCUPANCY waves per SIMD.  16-bit heads of 64
-// fit two waves per SIMD at R = 32, whose products read LDS half as often: the pass over 4 x 2048 causal tokens, 32 heads, bf16, takes 519 us, at R = 16
-// 659.  Longer rows and float32 fit them (but for a few registers) at R = 16 only: 8192 tokens, 16 heads of 128, f16 2613 us, at R = 32 with one wave
-// 2862; float32 (2 x 1024 causal, 8 heads) of 64 260 against 287, of 128 490 against 581.  Four waves per SIMD spill: 6571.
+// fit two waves per SIMD at R = 32, whose products read LDS half as often: the pass over 4 x 2048 causal tokens, 32 heads, bf16, takes 530 us, at R = 16
+// 730.  Longer rows and float32 fit them at R = 16 only (16-bit rows of 128 but for 1 to 3 registers of dk / dv, float32 ones but for 6 to 69): 8192 tokens, 16 heads of 128, f16
+// 2500 us, at R = 32 with one wave 3655 (bf16 2510 and 2690); float32 (4 x 2048 causal, 16 heads) of 64 1520 against 1556, of 128 2850 against 3014.
 template <typename T, int DP> struct Shape {
     static constexpr int R = DP == 64 && sizeof(T) == 2 ? 32 : 16, W = 128 / R, OCCUPANCY = 2;
 };
@@ -51,7 +51,7 @@ struct Range {
     }
 };
 
-// delta[row] = sum over the head of out * grad_out, with the rounded output: one pass over two tensors in place of one over keys and values.  16 lanes per row, 16 bytes each: one read of both tensors, bound by HBM (A: 12 us, 5.6 TB/s; B: 11.7; C: 20 us, 3.9 TB/s).
+// delta[row] = sum over the head of out * grad_out, with the rounded output: one pass over two tensors in place of one over keys and values.  16 lanes per row, 16 bytes each: one read of both tensors, bound by HBM (A: 12.4 us, 5.4 TB/s; B: 12.3; C: 15.8).
 template <typename T, bool WIDE>
 __global__ void __launch_bounds__(256) attention_delta_kernel(tvl_attention_args a, tvl_attention_grads gr, float* __restrict__ delta, int blocks) {
     constexpr int PER = 16 / (int)sizeof(T);
@@ -77,8 +77,9 @@ __global__ void __launch_bounds__(256) attention_delta_kernel(tvl_attention_args
 }
 
 // dq.  W waves x R queries; per 32 keys: S^T = K Q^T, dP^T = V dO^T, dS^T = P (dP - delta) bend (a lane holds one query), dQ^T += K^T dS^T.  Six operations per
-// pair and element.  A: 201 us (513 TFLOP/s), B: 386, C: 107.  The matrix cores are busy 39 % of the time at heads of 64 and 26 %
-// at 128: exponentials and conversions on the vector ALU and the operands' way out of LDS (no bank conflicts left) wait for each other with two waves per SIMD.
+// pair and element, eight for 16-bit operands (`mean` below).  A: 222 us (620 TFLOP/s), B: 383, C: 118.  The matrix cores are busy 41 % of the time at heads of 64 and 43 %
+// at 128: exponentials and conversions on the vector ALU and the operands' way out of LDS (no bank conflicts) wait for each other with two waves per SIMD.
+// float16's range costs a maximum per score and a branch in front of the last product: 4 x 2048 causal, 32 heads of 64 257 us.
 //
 // delta' of the rounded output is off by its two roundings (weights, result), for rows whose weight lies on few keys as far as a score gradient's own rounding,
 // and all in one direction.  For 16-bit operands the sum of P (dP - delta') over a row, zero but for that error, is formed beside (`rest`, float32), and
@@ -320,8 +321,8 @@ __global__ void __launch_bounds__((64 * Shape<T, DP>::W), (Shape<T, DP>::OCCUPAN
 }
 
 // dk, dv.  W waves x R keys; over the heads that share them and tiles of 64 queries: S = Q K^T, dP = dO V^T (a lane holds one key, K and V stay in
-// registers), dV^T += dO^T P, dK^T += Q^T dS.  Eight operations per pair and element.  A: 290 us (474 TFLOP/s), C: 180, B: 947 with a group's heads in one workgroup;
-// bound as dq is, matrix cores busy 31 % and 22 %.
+// registers), dV^T += dO^T P, dK^T += Q^T dS.  Eight operations per pair and element.  A: 292 us (471 TFLOP/s), C: 181, B: 630 in two parts;
+// bound as dq is, matrix cores busy 31 %.
 template <typename T, int DP, Form FORM>
 __global__ void __launch_bounds__((64 * Shape<T, DP>::W), (Shape<T, DP>::OCCUPANCY)) attention_dkv_kernel(tvl_attention_args a, tvl_attention_grads gr, const DocumentSpan* __restrict__ spans, const float* __restrict__ delta,
                                                             int tiles, int parts, float* __restrict__ slabs) {
@@ -571,9 +572,9 @@ __global__ void __launch_bounds__(256) attention_gather_kernel(const float* __re
 }
 
 // Parts of a group's heads: a key tile whose workgroup takes all heads in turn is the longest chain of the pass, so where the key tiles alone do not
-// give two workgroups per compute unit the heads are divided (float32 sums through memory, added in order by a second launch).  B in one part: 947 us, of
-// which the 45 tiles x 4 heads of the longest document's first keys are the chain; in two parts the chain is half as long and 67 MB of sums, written once and read
-// once, are 27 us.  The division itself has not been timed.
+// give two workgroups per compute unit the heads are divided (float32 sums through memory, added in order by a second launch of 13 us).  The backward pass in one part and
+// as divided, us: B 1351 and 1084; 8192 causal tokens, 16 / 4 heads of 128, bf16 2060 and 1424; 2048 tokens, 32 / 8 heads of 128 492 and 259; 1024 tokens, 32 heads of 64 over one
+// key head, f16 1120 and 100; 2 x 512 tokens, 16 / 4 heads of 64 100-120 and 85-119; 4 x 2048 tokens, 32 / 8 heads of 128, bf16, not divided further, 1112 and 1095.
 int attention_backward_parts(const tvl_attention_args& a) {
     if (a.queries == 0) return 1;      // sums of nothing: no workspace either
     const int64_t tiles = a.batch * a.kv_heads * ceil_div(a.keys, 128);

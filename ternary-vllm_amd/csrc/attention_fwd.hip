@@ -6,12 +6,12 @@ namespace tvl {
 // One workgroup: 4 waves x 32 queries of one head; keys and values come in tiles of 64 through LDS, two buffers, the next tile's loads in
 // flight while this one is used: its keys during the scores, its values during the rest, through one set of registers (two sets spill at heads of 128).  Per wave and tile: S^T = K Q^T (a lane holds 32 scores of ONE query: maximum and sum are plain loops
 // over its registers plus one exchange with the other half), weights 2^(s - m) rounded to the operands' type as the second product's operand,
-// O^T += V^T P^T.  m is kept until a score exceeds it by 8 (in powers of two): the weights stay below 2^8, exact in float32 sums, and the
+// O^T += V^T P^T.  m is kept until a score exceeds it by 8 (in powers of two): the weights stay below 2^8 (float16: 2^15, see LIFT), and the
 // accumulator is almost never rescaled.  Tiles that every query sees whole run in a loop without masks.
-// Heads of 128: 8192 x 8192, 16 heads, f16 697 us (790 TFLOP/s), causal bf16 16 / 4 heads 351 us (780), capped 568; heads of 64: 4 x 2048, 32 heads, bf16
-// 207 us (660 TFLOP/s), causal 148-157 us (440-465), 128 x 197, 12 heads, f16 62 us (246).  A score costs an exponential and about four other vector instructions
-// whatever the head's length, so heads of 64 are bound by the vector ALU; heads of 128 reach 70 % of the rate of a large library product.  One set of registers
-// instead of two, and banks without conflicts, took them from 883 to 697 us.
+// Heads of 128: 8192 x 8192, 16 heads, f16 645 us (850 TFLOP/s), causal bf16 16 / 4 heads 340 us (810), capped 540; heads of 64: 4 x 2048, 32 heads, bf16
+// 207 us (660 TFLOP/s), causal 152 us (452), 128 x 197, 12 heads, f16 64 us (238).  A score costs an exponential and about four other vector instructions
+// whatever the head's length, so heads of 64 are bound by the vector ALU; heads of 128 reach 76 % of the rate of a large library product.  One set of registers
+// instead of two, and banks without conflicts, took them from 883 to below 700 us; 16-bit forms of heads of 128 still keep some registers in scratch memory (19 to 22 in PLAIN, 60 to 168 in the others).
 template <typename T, int DP, bool CACHED, Form FORM>
 __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) attention_forward_kernel(tvl_attention_args a, const DocumentSpan* __restrict__ spans, int tiles) {
     constexpr bool WIDE = FORM != ODD;

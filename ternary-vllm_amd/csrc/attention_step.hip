@@ -267,6 +267,9 @@ static bool step_wide(const tvl_attention_args& a) {
     return wide_rows(a.q, a.dim, a.q_batch, a.q_token, a.q_head, z) && wide_rows(a.k, a.dim, a.k_batch, a.k_token, a.k_head, z) && wide_rows(a.v, a.dim, a.v_batch, a.v_token, a.v_head, z);
 }
 
+// Rows (tokens x heads of a group) that the cache kernel takes; more go to the tile kernel, which takes one head per workgroup and never cuts the keys.  Measured (us, us): 4
+// sequences, 4 key heads of 128, 64 rows here, 72 there: 1000 keys 18, 35; 4000 keys 25, 121; 28000 keys 77, 778; one sequence, 32 heads of 64, 64 rows here, 65 there: 14.8, 22.9;
+// 22, 71; 74, 456.  The bound keeps whole prompts with the tile kernel (8 x 745 over a fresh cache 56); long caches would be served by this one far beyond it, and are not yet.
 bool attention_step_serves(const tvl_attention_args& a) {
     const int64_t rows = a.queries * (a.heads / a.kv_heads);
     return rows <= 64;
@@ -274,7 +277,8 @@ bool attention_step_serves(const tvl_attention_args& a) {
 
 // Parts the keys are cut into: enough for one workgroup per compute unit, none shorter than 512 keys; a cache of up to 1024 slots stays whole, its
 // second launch costs more than the parts gain.  Measured (us, us): 32 pairs x 745 of 1024 slots whole 8.3, 4 parts 9.3; 256 pairs x 745 whole 11.9,
-// 2 parts 17.3; 32 pairs x 28000 x 128 in 8 parts 89.6, 16 parts 92.6; one pair x 32000 in 62 parts 20.5, 31 parts 23.8, 125 parts 20.1.
+// 2 parts 17.3; 32 pairs x 28000 x 128 in 8 parts 89.6, 16 parts 92.6; one pair x 32000 in 62 parts 20.5, 31 parts 23.8, 125 parts 20.1; one
+// pair x 1000 of 1024 slots whole 9.1, of 1025 in 3 parts 9.5; 4 pairs 9.3 and 9.4.
 int attention_step_splits(const tvl_attention_args& a) {
     const int64_t work = a.batch * a.kv_heads * ceil_div(a.queries * (a.heads / a.kv_heads), ROWS);
     const int64_t want = ceil_div(256, work), most = a.keys <= 1024 ? 1 : ceil_div(a.keys, 512);
