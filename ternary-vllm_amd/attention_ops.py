@@ -249,6 +249,18 @@ def _apart(t: torch.Tensor) -> bool:
     return True
 
 
+def _meet(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two views of one layout, each without elements that share memory, share some with each other: their distance is a sum of steps that both can take.
+    Views of different layouts are not looked at."""
+    if a.is_contiguous() or a.stride() != b.stride() or a.untyped_storage().data_ptr() != b.untyped_storage().data_ptr():
+        return False
+    away = {a.storage_offset() - b.storage_offset()}
+    for stride, size in sorted(((s, n) for s, n in zip(a.stride(), a.shape) if n > 1), reverse=True):
+        # what is left after this dimension is less than a step of it
+        away = {d - stride * k for d in away for k in (d // stride, d // stride + 1) if abs(k) < size}
+    return 0 in away
+
+
 def _check_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, like: torch.Tensor, b: int, d: int, name: str, written: bool):
     if (isinstance(k_cache, torch.Tensor) and isinstance(v_cache, torch.Tensor) and k_cache.dtype is like.dtype and v_cache.dtype is like.dtype
             and k_cache.device == like.device and v_cache.device == like.device and k_cache.dim() == 4 and k_cache.shape == v_cache.shape
@@ -297,7 +309,7 @@ def rotary_cache(qkv: torch.Tensor, table: torch.Tensor, k_cache: torch.Tensor, 
         raise ValueError(f"rotary_cache: rows of {width} channels do not hold {heads} query and 2 x {hk} key / value heads of {d}")
     _check_cache(k_cache, v_cache, qkv, b, d, "rotary_cache", True)
     ka, va = k_cache.data_ptr(), v_cache.data_ptr()
-    if k_cache.numel() and (ka == va or (abs(ka - va) < k_cache.nbytes and k_cache.is_contiguous() and v_cache.is_contiguous())):
+    if k_cache.numel() and (ka == va or (abs(ka - va) < k_cache.nbytes and k_cache.is_contiguous() and v_cache.is_contiguous()) or _meet(k_cache, v_cache)):
         raise ValueError("rotary_cache: k_cache and v_cache share memory")
     _check_table(table, d, qkv.device, "rotary_cache")
     at, stride, value, n, count = _lengths(cache_len, count, b, t, slots, qkv.device, "rotary_cache")

@@ -52,3 +52,20 @@ def test_gradient_launches_beyond_the_grid_are_refused(batch, heads, tokens):
         a = attention_args(batch=batch, heads=heads, kv_heads=heads, queries=tokens, keys=tokens, dim=dim, o_batch=tokens * heads * dim, o_token=heads * dim, o_head=dim)
         assert lib.tvl_attention_backward(a, grads_args(), P, 1 << 62, None) == 1 and b"too many" in lib.tvl_last_error()
         assert lib.tvl_attention(a, None, 0, None) == 1 and b"too many" in lib.tvl_last_error()
+
+
+def test_views_that_share_elements_are_found():
+    """Against the sets of their elements, for layouts of caches: heads beside each other, slots apart, layers of one tensor."""
+    meet, apart = tv.attention_ops._meet, tv.attention_ops._apart
+    big = torch.zeros(6, 4, 5, 7, 8)
+    views = [big[i:i + 2, h:h + 2, b, s:s + 4:st, e:e + 3] for i in (0, 1, 2) for h in (0, 1, 2) for b in (0, 1) for s, st in ((0, 1), (3, 1), (0, 2), (1, 2)) for e in (0, 2, 5)]
+    places = [set((torch.arange(big.numel()).view(big.shape).as_strided(v.shape, v.stride(), v.storage_offset())).flatten().tolist()) for v in views]
+    found = 0
+    for x, px in zip(views[::3], places[::3]):
+        assert apart(x)
+        for y, py in zip(views, places):
+            if x.stride() == y.stride() and x.shape == y.shape:
+                assert meet(x, y) == bool(px & py), (x.storage_offset(), y.storage_offset(), x.stride())
+                found += bool(px & py)
+    assert found > 100
+    assert not meet(views[0], views[0].clone()) and not meet(big[:, 0], big.clone()[:, 0])

@@ -83,3 +83,15 @@ def test_a_leaf_taken_twice_in_one_capture(tv, dev):
         graphs[n % 2].replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(want, outs[n % 2])), n
+
+
+def test_rotary_cache_refuses_interleaved_caches_that_share_slots(tv, dev):
+    table, qkv = tv.rotary_table(16, 9, device=dev), torch.randn(2, 3, 8 * 16, device=dev)
+    both = torch.zeros(2, 5, 9, 16, device=dev)
+    for k, v in ((both[:, :2], both[:, 1:3]), (both[:, 2:4], both[:, 1:3])):
+        with pytest.raises(ValueError, match="share"):
+            tv.rotary_cache(qkv, table, k, v, 0, 4)
+    k, v = torch.zeros(2, 2, 9, 16, device=dev), torch.zeros(2, 2, 9, 16, device=dev)
+    want = tv.rotary_cache(qkv, table, k, v, 4, 4)
+    assert torch.equal(tv.rotary_cache(qkv, table, both[:, :2], both[:, 2:4], 4, 4), want)
+    assert torch.equal(both[:, :2], k) and torch.equal(both[:, 2:4], v) and int(both[:, 4].count_nonzero()) == 0
