@@ -402,7 +402,7 @@ def main():
         traffic, traffic_note = None, None
         try:   # HBM-side bytes per launch from the committed rocprofv3 --pmc passes: valid for the profiled binary and shape only
             import hashlib
-            tpath = next(p_ for p_ in (os.path.join(ROOT, "profiles", f"r0{r_}_traffic.json") for r_ in (3, 2)) if os.path.exists(p_))
+            tpath = next(p_ for p_ in (os.path.join(ROOT, "profiles", f_) for f_ in ("traffic.json", "r03_traffic.json")) if os.path.exists(p_))
             with open(tpath) as f:
                 tj = json.load(f)
             with open(ops.LIBRARY_PATH, "rb") as f:
