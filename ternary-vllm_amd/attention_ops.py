@@ -30,6 +30,7 @@ _ROTARY_CACHE = struct.Struct("=8Q19q2i")
 _ATTENTION = struct.Struct("=11Q22q2f2i")
 _GRADS = struct.Struct("=5Q3q")
 
+_F32_MAX = torch.finfo(torch.float32).max
 _FLOATS = {torch.float32: ops.F32, torch.float16: ops.F16, torch.bfloat16: ops.BF16}
 
 
@@ -340,8 +341,8 @@ def _scale_cap(scale, softcap, d: int, name: str):
         return d ** -0.5, 0.0
     scale = d ** -0.5 if scale is None else float(scale)
     softcap = 0.0 if softcap is None else float(softcap)
-    if not math.isfinite(scale) or not (softcap >= 0.0 and math.isfinite(softcap)):
-        raise ValueError(f"{name}: scale={scale} must be finite, softcap={softcap} finite and not negative")
+    if not (abs(scale) <= _F32_MAX and 0.0 <= softcap <= _F32_MAX):
+        raise ValueError(f"{name}: scale={scale} must be finite, softcap={softcap} finite and not negative, in float32")
     return scale, softcap
 
 

@@ -69,3 +69,10 @@ def test_views_that_share_elements_are_found():
                 found += bool(px & py)
     assert found > 100
     assert not meet(views[0], views[0].clone()) and not meet(big[:, 0], big.clone()[:, 0])
+
+
+@pytest.mark.parametrize("scale,softcap", [(1e39, 0.0), (-1e39, 0.0), (float("inf"), 0.0), (float("nan"), 0.0), (1.0, 1e39), (1.0, float("inf")), (1.0, float("nan")), (1.0, -1.0)])
+def test_scales_and_caps_beyond_float32_are_refused(scale, softcap):
+    with pytest.raises(ValueError, match="scale"):
+        tv.attention_ops._scale_cap(scale, softcap, 64, "attention")
+    assert tv.attention_ops._scale_cap(3e38, 3e38, 64, "attention") == (3e38, 3e38)
